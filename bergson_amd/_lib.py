@@ -48,6 +48,35 @@ class BlockDesc(C.Structure):
     ]
 
 
+class AttentionShape(C.Structure):
+    """Mirror of ``bgx_attention_shape``."""
+
+    _fields_ = [
+        ("plan_dev", C.c_void_p),
+        ("lengths_dev", C.c_void_p),
+        ("rows", C.c_int64),
+        ("n_seqs", C.c_int32),
+        ("heads", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("dtype", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+
+class AttentionRows(C.Structure):
+    """Mirror of ``bgx_attention_rows``: an operand and its element strides."""
+
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("seq_stride", C.c_int64),
+        ("tok_stride", C.c_int64),
+        ("head_stride", C.c_int64),
+    ]
+
+
+_ROWS = C.POINTER(AttentionRows)
+
 # name -> (restype, argtypes); the one list every exported symbol is checked against
 SIGNATURES: dict[str, tuple] = {
     "bgx_abi_version": (C.c_int, []),
@@ -149,6 +178,36 @@ SIGNATURES: dict[str, tuple] = {
         [C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_void_p, C.c_int32, C.c_float, C.c_int32,
          C.c_int32, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
          C.c_size_t, C.c_int64, C.c_void_p],
+    ),
+    "bgx_layernorm_forward": (
+        C.c_int,
+        [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_float,
+         C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p],
+    ),
+    "bgx_layernorm_backward_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int32]),
+    "bgx_layernorm_backward": (
+        C.c_int,
+        [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64,
+         C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p],
+    ),
+    "bgx_attention_plan_bytes": (C.c_size_t, [C.c_int64, C.c_int32]),
+    "bgx_attention_plan": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "bgx_attention_forward": (C.c_int, [C.POINTER(AttentionShape), _ROWS, _ROWS, _ROWS, _ROWS, C.c_void_p, C.c_void_p]),
+    "bgx_attention_backward_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionShape)]),
+    "bgx_attention_backward": (
+        C.c_int,
+        [C.POINTER(AttentionShape), _ROWS, _ROWS, _ROWS, _ROWS, C.c_void_p, _ROWS, _ROWS, _ROWS, _ROWS, C.c_void_p,
+         C.c_size_t, C.c_void_p],
+    ),
+    "bgx_distill_forward": (
+        C.c_int,
+        [C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
+         C.c_void_p, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p],
+    ),
+    "bgx_distill_backward": (
+        C.c_int,
+        [C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
+         C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p],
     ),
 }
 

@@ -20,7 +20,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 LIB = PKG / "libbergson_amd.so"
-SOURCES = ["capi.hip", "collect.hip", "scan.hip", "adam.hip", "fullgrad.hip", "precond.hip"]
+SOURCES = ["capi.hip", "collect.hip", "scan.hip", "adam.hip", "fullgrad.hip", "precond.hip", "layernorm.hip", "attention.hip",
+           "distill.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
@@ -78,7 +79,7 @@ def build(verbose: bool = True) -> Path:
 
     temps = Path(tempfile.mkdtemp(prefix="bgx_build_"))
     try:
-        with ThreadPoolExecutor(max_workers=min(6, len(SOURCES))) as ex:
+        with ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
             objs = list(ex.map(lambda s: _compile(s, verbose, temps if s in INSPECTED else None), SOURCES))
         bad = isa_checks.all_violations({src: device_assembly(temps, src) for src in INSPECTED})
     finally:

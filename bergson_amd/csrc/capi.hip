@@ -136,6 +136,30 @@ int block_gemm_impl(const void* in, int in_dtype, int64_t in_stride, void* out, 
 int gram_accumulate_impl(const void* rows_dev, int dtype, int64_t stride, int64_t rows, const bgx_block_desc* blocks,
                          int n_blocks, void* ws, size_t ws_bytes, void* stream);
 
+int layernorm_forward_impl(const void* x, int64_t x_stride, const void* weight, const void* bias, int wdtype,
+                           int64_t rows, int d, int dtype, float eps, void* y, int64_t y_stride, float* mean,
+                           float* rstd, void* stream);
+size_t layernorm_backward_workspace_bytes(int64_t rows, int d);
+int layernorm_backward_impl(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* weight,
+                            int wdtype, const float* mean, const float* rstd, int64_t rows, int d, int dtype, void* dx,
+                            int64_t dx_stride, void* dweight, void* dbias, void* ws, size_t ws_bytes, void* stream);
+size_t attention_plan_bytes(int64_t rows, int n_seqs);
+int attention_plan_impl(const int32_t* cu, int n_seqs, int64_t rows, void* plan, size_t plan_bytes, void* stream);
+int attention_forward_impl(const bgx_attention_shape* shape, const bgx_attention_rows* q, const bgx_attention_rows* k,
+                           const bgx_attention_rows* v, const bgx_attention_rows* out, float* lse, void* stream);
+size_t attention_backward_workspace_bytes(const bgx_attention_shape* shape);
+int attention_backward_impl(const bgx_attention_shape* shape, const bgx_attention_rows* q, const bgx_attention_rows* k,
+                            const bgx_attention_rows* v, const bgx_attention_rows* out, const float* lse,
+                            const bgx_attention_rows* grad_out, const bgx_attention_rows* dq,
+                            const bgx_attention_rows* dk, const bgx_attention_rows* dv, void* ws, size_t ws_bytes,
+                            void* stream);
+int distill_forward_impl(const void* logits, int64_t stride, int64_t rows, int V, int dtype, const int64_t* ids,
+                         const void* teacher, int teacher_dtype, int K, const uint8_t* valid, float tau, float* losses,
+                         float* stats, void* stream);
+int distill_backward_impl(const void* logits, int64_t stride, int64_t rows, int V, int dtype, const int64_t* ids,
+                          const void* teacher, int teacher_dtype, int K, float tau, const float* stats,
+                          const float* grad, void* dlogits, int64_t dstride, void* stream);
+
 }  // namespace bgx
 
 extern "C" {
@@ -350,6 +374,68 @@ int bgx_scan_known_norms(const void* store_dev, int64_t n_rows, int64_t D, int64
   return bgx::scan_impl(store_dev, n_rows, D, store_row_stride, dtype, queries_dev, Q, query_scale, unit_norm, k,
                         row_base, topk_val_dev, topk_idx_dev, row_max_dev, row_mean_dev, scores_dev, nullptr,
                         row_sumsq_dev, workspace_dev, workspace_bytes, chunk_rows, stream);
+}
+
+int bgx_layernorm_forward(const void* x_dev, int64_t x_row_stride, const void* weight_dev, const void* bias_dev,
+                          int32_t weight_dtype, int64_t rows, int32_t d, int32_t dtype, float eps, void* y_dev,
+                          int64_t y_row_stride, float* mean_dev, float* rstd_dev, void* stream) {
+  return bgx::layernorm_forward_impl(x_dev, x_row_stride, weight_dev, bias_dev, weight_dtype, rows, d, dtype, eps, y_dev,
+                                     y_row_stride, mean_dev, rstd_dev, stream);
+}
+
+size_t bgx_layernorm_backward_workspace_bytes(int64_t rows, int32_t d) {
+  return bgx::layernorm_backward_workspace_bytes(rows, d);
+}
+
+int bgx_layernorm_backward(const void* dy_dev, int64_t dy_row_stride, const void* x_dev, int64_t x_row_stride,
+                           const void* weight_dev, int32_t weight_dtype, const float* mean_dev, const float* rstd_dev,
+                           int64_t rows, int32_t d, int32_t dtype, void* dx_dev, int64_t dx_row_stride,
+                           void* dweight_dev, void* dbias_dev, void* workspace_dev, size_t workspace_bytes,
+                           void* stream) {
+  return bgx::layernorm_backward_impl(dy_dev, dy_row_stride, x_dev, x_row_stride, weight_dev, weight_dtype, mean_dev,
+                                      rstd_dev, rows, d, dtype, dx_dev, dx_row_stride, dweight_dev, dbias_dev,
+                                      workspace_dev, workspace_bytes, stream);
+}
+
+size_t bgx_attention_plan_bytes(int64_t rows, int32_t n_seqs) { return bgx::attention_plan_bytes(rows, n_seqs); }
+
+int bgx_attention_plan(const int32_t* cu_seqlens_dev, int32_t n_seqs, int64_t rows, void* plan_dev, size_t plan_bytes,
+                       void* stream) {
+  return bgx::attention_plan_impl(cu_seqlens_dev, n_seqs, rows, plan_dev, plan_bytes, stream);
+}
+
+int bgx_attention_forward(const bgx_attention_shape* shape, const bgx_attention_rows* q, const bgx_attention_rows* k,
+                          const bgx_attention_rows* v, const bgx_attention_rows* out, float* lse_dev, void* stream) {
+  return bgx::attention_forward_impl(shape, q, k, v, out, lse_dev, stream);
+}
+
+size_t bgx_attention_backward_workspace_bytes(const bgx_attention_shape* shape) {
+  return bgx::attention_backward_workspace_bytes(shape);
+}
+
+int bgx_attention_backward(const bgx_attention_shape* shape, const bgx_attention_rows* q, const bgx_attention_rows* k,
+                           const bgx_attention_rows* v, const bgx_attention_rows* out, const float* lse_dev,
+                           const bgx_attention_rows* grad_out, const bgx_attention_rows* dq,
+                           const bgx_attention_rows* dk, const bgx_attention_rows* dv, void* workspace_dev,
+                           size_t workspace_bytes, void* stream) {
+  return bgx::attention_backward_impl(shape, q, k, v, out, lse_dev, grad_out, dq, dk, dv, workspace_dev,
+                                      workspace_bytes, stream);
+}
+
+int bgx_distill_forward(const void* logits_dev, int64_t row_stride, int64_t rows, int32_t V, int32_t dtype,
+                        const int64_t* ids_dev, const void* teacher_dev, int32_t teacher_dtype, int32_t K,
+                        const uint8_t* valid_dev, float temperature, float* losses_dev, float* stats_dev,
+                        void* stream) {
+  return bgx::distill_forward_impl(logits_dev, row_stride, rows, V, dtype, ids_dev, teacher_dev, teacher_dtype, K,
+                                   valid_dev, temperature, losses_dev, stats_dev, stream);
+}
+
+int bgx_distill_backward(const void* logits_dev, int64_t row_stride, int64_t rows, int32_t V, int32_t dtype,
+                         const int64_t* ids_dev, const void* teacher_dev, int32_t teacher_dtype, int32_t K,
+                         float temperature, const float* stats_dev, const float* grad_dev, void* dlogits_dev,
+                         int64_t dlogits_row_stride, void* stream) {
+  return bgx::distill_backward_impl(logits_dev, row_stride, rows, V, dtype, ids_dev, teacher_dev, teacher_dtype, K,
+                                    temperature, stats_dev, grad_dev, dlogits_dev, dlogits_row_stride, stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,370 @@
+// Layer norm, forward and backward.
+//
+//   mean = sum x / d, rstd = 1 / sqrt(sum (x - mean)^2 / d + eps), xh = (x - mean) rstd, y = xh w + b
+//   h = dy w,  dx = rstd (h - mean(h) - xh mean(h xh)),  dw = sum_rows dy xh,  db = sum_rows dy
+//
+// Bound by memory traffic: the forward pass reads a row once and writes one, the backward pass reads two and
+// writes one; a row stays in registers between the statistics and their use (the variance is formed from
+// deviations of a mean that is already there, so a row with a large common offset loses nothing).  All sums in
+// fp32.  A row belongs to WPR waves; with NE elements a lane, the widths up to 64 * WPR * NE are covered.
+#include "rows.hpp"
+
+namespace bgx {
+
+constexpr int LN_MAX_D = 16384;
+constexpr int LN_WAVES = 4;             // waves per workgroup
+constexpr int LN_PARTS_MAX = 512;       // workgroups of a backward pass that form dw / db: rows of partial sums
+
+struct NormArgs {
+  const void* x;
+  const void* dy;
+  const void* weight;
+  const void* bias;
+  void* y;              // forward: y; backward: dx
+  float* mean;
+  float* rstd;
+  float* parts;         // backward: [workgroups][2][d] partial sums of dw, db
+  int64_t rows;
+  int64_t x_stride, dy_stride, y_stride;
+  int d;
+  float eps;
+};
+
+// Sum over the WPR waves of a row: with more than one, through LDS (slot: a pair of alternating buffers, so that
+// one barrier per sum is enough).
+template <int WPR>
+__device__ inline float2 row_sum2(float2 v, float2 (*slot)[LN_WAVES], int& turn) {
+  v.x = wave_sum(v.x);
+  v.y = wave_sum(v.y);
+  if constexpr (WPR > 1) {
+    const int w = threadIdx.x / WAVE;
+    if ((threadIdx.x & (WAVE - 1)) == 0) slot[turn][w] = v;
+    __syncthreads();
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < WPR; ++i) {
+      s.x += slot[turn][i].x;
+      s.y += slot[turn][i].y;
+    }
+    turn ^= 1;
+    return s;
+  }
+  return v;
+}
+
+template <typename T, typename WT, int NE, int WPR>
+__global__ __launch_bounds__(LN_WAVES* WAVE) void layernorm_forward_kernel(NormArgs A) {
+  constexpr int EPL = Chunk<T>::N, NC = NE / EPL;
+  __shared__ float2 slot[2][LN_WAVES];
+  int turn = 0;
+  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+  const int64_t step = (int64_t)gridDim.x * (LN_WAVES / WPR);
+  const int first = WPR == 1 ? lane : (int)threadIdx.x;
+  for (int64_t r = (int64_t)blockIdx.x * (LN_WAVES / WPR) + (WPR == 1 ? wave : 0); r < A.rows; r += step) {
+    const T* xr = (const T*)A.x + r * A.x_stride;
+    float x[NE];
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * WPR * WAVE + first) * EPL;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (col < A.d) v = load_chunk_tail(xr, col, A.d);
+      Chunk<T>::unpack(v, x + c * EPL);
+    }
+#pragma unroll
+    for (int e = 0; e < NE; ++e) s.x += x[e];
+    const float mean = row_sum2<WPR>(s, slot, turn).x / A.d;
+    float2 q = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        const bool in = (c * WPR * WAVE + first) * EPL + e < A.d;
+        const float dev = in ? x[c * EPL + e] - mean : 0.f;
+        x[c * EPL + e] = dev;
+        q.x = fmaf(dev, dev, q.x);
+      }
+    const float rstd = 1.0f / sqrtf(row_sum2<WPR>(q, slot, turn).x / A.d + A.eps);
+    T* yr = (T*)A.y + r * A.y_stride;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * WPR * WAVE + first) * EPL;
+      if (col >= A.d) continue;
+      float o[EPL];
+#pragma unroll
+      for (int k = 0; k < EPL; k += Chunk<WT>::N) {  // weights of a wider type take two chunks
+        float w[Chunk<WT>::N], b[Chunk<WT>::N];
+        Chunk<WT>::unpack(load_chunk_tail((const WT*)A.weight, col + k, A.d), w);
+        if (A.bias != nullptr) {
+          Chunk<WT>::unpack(load_chunk_tail((const WT*)A.bias, col + k, A.d), b);
+        } else {
+#pragma unroll
+          for (int e = 0; e < Chunk<WT>::N; ++e) b[e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < Chunk<WT>::N; ++e) o[k + e] = fmaf(x[c * EPL + k + e] * rstd, w[e], b[e]);
+      }
+      store_chunk_tail(yr, col, A.d, Chunk<T>::pack(o));
+    }
+    if (A.mean != nullptr && first == 0) {
+      A.mean[r] = mean;
+      A.rstd[r] = rstd;
+    }
+  }
+}
+
+// PARAMS: the workgroup also sums dy xh and dy over its rows, column by column in registers (a lane keeps the same
+// columns for every row), adds its waves' sums through LDS in a fixed order and writes one row of partial sums.
+template <typename T, typename WT, int NE, int WPR, bool PARAMS>
+__global__ __launch_bounds__(LN_WAVES* WAVE) void layernorm_backward_kernel(NormArgs A) {
+  constexpr int EPL = Chunk<T>::N, NC = NE / EPL;
+  __shared__ float2 slot[2][LN_WAVES];
+  __shared__ float colsum[PARAMS && WPR == 1 ? WAVE * NE : 1];
+  int turn = 0;
+  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+  const int64_t step = (int64_t)gridDim.x * (LN_WAVES / WPR);
+  const int first = WPR == 1 ? lane : (int)threadIdx.x;
+  float dw[PARAMS ? NE : 1], db[PARAMS ? NE : 1];
+  if constexpr (PARAMS) {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) dw[e] = db[e] = 0.f;
+  }
+  for (int64_t r = (int64_t)blockIdx.x * (LN_WAVES / WPR) + (WPR == 1 ? wave : 0); r < A.rows; r += step) {
+    const T* xr = (const T*)A.x + r * A.x_stride;
+    const T* gr = (const T*)A.dy + r * A.dy_stride;
+    const float mean = A.mean[r], rstd = A.rstd[r];
+    float x[NE], h[NE];
+    float2 s = make_float2(0.f, 0.f);  // sums of h and of h xh
+    uint4 xv[NC], gv[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * WPR * WAVE + first) * EPL;
+      xv[c] = gv[c] = make_uint4(0u, 0u, 0u, 0u);
+      if (col < A.d) {
+        xv[c] = load_chunk_tail(xr, col, A.d);
+        gv[c] = load_chunk_tail(gr, col, A.d);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * WPR * WAVE + first) * EPL;
+      Chunk<T>::unpack(xv[c], x + c * EPL);
+      Chunk<T>::unpack(gv[c], h + c * EPL);
+#pragma unroll
+      for (int k = 0; k < EPL; k += Chunk<WT>::N) {
+        float w[Chunk<WT>::N];
+        uint4 wv = make_uint4(0u, 0u, 0u, 0u);
+        if (col < A.d) wv = load_chunk_tail((const WT*)A.weight, col + k, A.d);
+        Chunk<WT>::unpack(wv, w);
+#pragma unroll
+        for (int e = 0; e < Chunk<WT>::N; ++e) {
+          const int i = c * EPL + k + e;
+          const bool in = col + k + e < A.d;
+          const float xh = in ? (x[i] - mean) * rstd : 0.f;
+          if constexpr (PARAMS) {
+            dw[i] = fmaf(h[i], xh, dw[i]);
+            db[i] += h[i];
+          }
+          x[i] = xh;
+          h[i] *= w[e];
+          s.x += h[i];
+          s.y = fmaf(h[i], xh, s.y);
+        }
+      }
+    }
+    if (A.y == nullptr) continue;
+    s = row_sum2<WPR>(s, slot, turn);
+    const float mh = s.x / A.d, mx = s.y / A.d;
+    T* dxr = (T*)A.y + r * A.y_stride;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * WPR * WAVE + first) * EPL;
+      if (col >= A.d) continue;
+      float o[EPL];
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) o[e] = rstd * (h[c * EPL + e] - mh - x[c * EPL + e] * mx);
+      store_chunk_tail(dxr, col, A.d, Chunk<T>::pack(o));
+    }
+  }
+  if constexpr (PARAMS) {
+    float* part = A.parts + (int64_t)blockIdx.x * 2 * A.d;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float* acc = which == 0 ? dw : db;
+      if constexpr (WPR == 1) {
+        for (int w = 1; w < LN_WAVES; ++w) {  // wave w hands its sums to wave 0
+          __syncthreads();
+          if (wave == w) {
+#pragma unroll
+            for (int e = 0; e < NE; ++e) colsum[e * WAVE + lane] = acc[e];
+          }
+          __syncthreads();
+          if (wave == 0) {
+#pragma unroll
+            for (int e = 0; e < NE; ++e) acc[e] += colsum[e * WAVE + lane];
+          }
+        }
+      }
+      if (WPR > 1 || wave == 0) {
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+          const int col = ((e / EPL) * WPR * WAVE + first) * EPL + e % EPL;
+          if (col < A.d) part[(int64_t)which * A.d + col] = acc[e];
+        }
+      }
+    }
+  }
+}
+
+// dw[c], db[c] = sum over the n_parts rows of partial sums, in a fixed order: 16 groups of rows per column, joined
+// through LDS.  grid.y = 0: dw, 1: db.
+__global__ __launch_bounds__(1024) void layernorm_params_kernel(const float* __restrict__ parts, int n_parts, int d,
+                                                                void* dw, void* db, int dtype) {
+  __shared__ float sums[16][64];
+  const int col = blockIdx.x * 64 + (threadIdx.x & 63), group = threadIdx.x >> 6;
+  float s = 0.f;
+  if (col < d)
+    for (int i = group; i < n_parts; i += 16) s += parts[((int64_t)i * 2 + blockIdx.y) * d + col];
+  sums[group][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (group == 0 && col < d) {
+#pragma unroll
+    for (int g = 1; g < 16; ++g) s += sums[g][threadIdx.x];
+    void* out = blockIdx.y == 0 ? dw : db;
+    if (out != nullptr) store_as(out, col, s, dtype);
+  }
+}
+
+static int ln_check(int64_t rows, int d, int dtype, int wdtype) {
+  BGX_REQUIRE(rows >= 0 && d >= 1, BGX_E_ARG, "layer norm: rows=%lld d=%d", (long long)rows, d);
+  BGX_REQUIRE(d <= LN_MAX_D, BGX_E_SHAPE, "layer norm: d=%d, the kernels hold rows of at most %d elements", d, LN_MAX_D);
+  BGX_REQUIRE(dtype >= BGX_F32 && dtype <= BGX_BF16, BGX_E_DTYPE, "layer norm: dtype %d", dtype);
+  BGX_REQUIRE(wdtype == dtype || wdtype == BGX_F32, BGX_E_DTYPE,
+              "layer norm: weight dtype %d; it is that of x (%d) or fp32", wdtype, dtype);
+  return 0;
+}
+
+static int ln_grid(int64_t rows, int wpr, int most) {
+  const int64_t wgs = (rows + LN_WAVES / wpr - 1) / (LN_WAVES / wpr);
+  return (int)(wgs < most ? wgs : most);
+}
+
+// Elements per lane and waves per row: one wave up to 2048 elements, the whole workgroup beyond.
+#define BGX_LN_WIDTHS(d, CALL)      \
+  if ((d) <= 512) CALL(8, 1)        \
+  else if ((d) <= 1024) CALL(16, 1) \
+  else if ((d) <= 2048) CALL(32, 1) \
+  else if ((d) <= 4096) CALL(16, 4) \
+  else if ((d) <= 8192) CALL(32, 4) \
+  else CALL(64, 4)
+
+template <typename T, typename WT>
+static int ln_forward(const NormArgs& A, hipStream_t stream) {
+#define BGX_LN_CALL(NE, WPR)                                                                                   \
+  {                                                                                                            \
+    layernorm_forward_kernel<T, WT, NE, WPR><<<ln_grid(A.rows, WPR, 8192), LN_WAVES * WAVE, 0, stream>>>(A);   \
+  }
+  BGX_LN_WIDTHS(A.d, BGX_LN_CALL)
+#undef BGX_LN_CALL
+  BGX_HIP(hipGetLastError());
+  return 0;
+}
+
+template <typename T, typename WT, bool PARAMS>
+static int ln_backward(const NormArgs& A, int grid, hipStream_t stream) {
+#define BGX_LN_CALL(NE, WPR) \
+  { layernorm_backward_kernel<T, WT, NE, WPR, PARAMS><<<grid, LN_WAVES * WAVE, 0, stream>>>(A); }
+  BGX_LN_WIDTHS(A.d, BGX_LN_CALL)
+#undef BGX_LN_CALL
+  BGX_HIP(hipGetLastError());
+  return 0;
+}
+
+int layernorm_forward_impl(const void* x, int64_t x_stride, const void* weight, const void* bias, int wdtype,
+                           int64_t rows, int d, int dtype, float eps, void* y, int64_t y_stride, float* mean,
+                           float* rstd, void* stream) {
+  if (int rc = ln_check(rows, d, dtype, wdtype)) return rc;
+  if (rows == 0) return 0;
+  BGX_REQUIRE(x && y && weight, BGX_E_ARG, "layer norm: null x, y or weight");
+  BGX_REQUIRE((mean == nullptr) == (rstd == nullptr), BGX_E_ARG, "layer norm: mean and rstd come together");
+  BGX_REQUIRE(x_stride >= d && y_stride >= d, BGX_E_ARG, "layer norm: row strides %lld, %lld below d=%d",
+              (long long)x_stride, (long long)y_stride, d);
+  NormArgs A{};
+  A.x = x;
+  A.weight = weight;
+  A.bias = bias;
+  A.y = y;
+  A.mean = mean;
+  A.rstd = rstd;
+  A.rows = rows;
+  A.x_stride = x_stride;
+  A.y_stride = y_stride;
+  A.d = d;
+  A.eps = eps;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == BGX_F32) return ln_forward<float, float>(A, s);
+  if (dtype == BGX_F16) return wdtype == BGX_F32 ? ln_forward<f16_t, float>(A, s) : ln_forward<f16_t, f16_t>(A, s);
+  return wdtype == BGX_F32 ? ln_forward<bf16_t, float>(A, s) : ln_forward<bf16_t, bf16_t>(A, s);
+}
+
+static int ln_wpr(int d) { return d <= 2048 ? 1 : 4; }
+
+size_t layernorm_backward_workspace_bytes(int64_t rows, int d) {
+  if (rows <= 0 || d <= 0 || d > LN_MAX_D) return 0;
+  return (size_t)ln_grid(rows, ln_wpr(d), LN_PARTS_MAX) * 2 * d * sizeof(float);
+}
+
+int layernorm_backward_impl(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* weight,
+                            int wdtype, const float* mean, const float* rstd, int64_t rows, int d, int dtype, void* dx,
+                            int64_t dx_stride, void* dweight, void* dbias, void* ws, size_t ws_bytes, void* stream) {
+  if (int rc = ln_check(rows, d, dtype, wdtype)) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  const bool params = dweight != nullptr || dbias != nullptr;
+  if (!params && (dx == nullptr || rows == 0)) return 0;
+  BGX_REQUIRE(rows == 0 || (dy && x && weight && mean && rstd), BGX_E_ARG, "layer norm backward: null operand");
+  BGX_REQUIRE(rows == 0 || (x_stride >= d && dy_stride >= d && (dx == nullptr || dx_stride >= d)), BGX_E_ARG,
+              "layer norm backward: row stride below d=%d", d);
+  if (params) {
+    const size_t need = layernorm_backward_workspace_bytes(rows, d);
+    BGX_REQUIRE(need == 0 || (ws != nullptr && ws_bytes >= need), BGX_E_WORKSPACE,
+                "layer norm backward: workspace of %zu bytes, %zu needed", ws_bytes, need);
+  }
+  const int parts = params ? ln_grid(rows, ln_wpr(d), LN_PARTS_MAX) : 0;
+  if (rows > 0) {
+    NormArgs A{};
+    A.x = x;
+    A.dy = dy;
+    A.weight = weight;
+    A.y = dx;
+    A.mean = const_cast<float*>(mean);
+    A.rstd = const_cast<float*>(rstd);
+    A.parts = (float*)ws;
+    A.rows = rows;
+    A.x_stride = x_stride;
+    A.dy_stride = dy_stride;
+    A.y_stride = dx_stride;
+    A.d = d;
+    const int grid = params ? parts : ln_grid(rows, ln_wpr(d), 8192);
+    int rc;
+#define BGX_LN_BACKWARD(T, WT) rc = params ? ln_backward<T, WT, true>(A, grid, s) : ln_backward<T, WT, false>(A, grid, s)
+    if (dtype == BGX_F32)
+      BGX_LN_BACKWARD(float, float);
+    else if (dtype == BGX_F16 && wdtype == BGX_F32)
+      BGX_LN_BACKWARD(f16_t, float);
+    else if (dtype == BGX_F16)
+      BGX_LN_BACKWARD(f16_t, f16_t);
+    else if (wdtype == BGX_F32)
+      BGX_LN_BACKWARD(bf16_t, float);
+    else
+      BGX_LN_BACKWARD(bf16_t, bf16_t);
+#undef BGX_LN_BACKWARD
+    if (rc) return rc;
+  }
+  if (params) {
+    layernorm_params_kernel<<<dim3((d + 63) / 64, 2), 1024, 0, s>>>((const float*)ws, parts, d, dweight, dbias, wdtype);
+    BGX_HIP(hipGetLastError());
+  }
+  return 0;
+}
+
+}  // namespace bgx

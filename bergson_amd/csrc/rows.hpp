@@ -1,0 +1,139 @@
+// Row access of the model operators (layer norm, distillation, attention): 16-byte chunks of a row that may start
+// on any element, with the row's ragged end handled element by element, and reductions over a wave.
+#pragma once
+
+#include <type_traits>
+
+#include "common.hpp"
+
+namespace bgx {
+
+// Elements per 16-byte chunk and the conversions of one chunk.
+template <typename T>
+struct Chunk;
+template <>
+struct Chunk<float> {
+  static constexpr int N = 4;
+  __device__ static void unpack(const uint4& v, float* f) {
+    f[0] = __uint_as_float(v.x);
+    f[1] = __uint_as_float(v.y);
+    f[2] = __uint_as_float(v.z);
+    f[3] = __uint_as_float(v.w);
+  }
+  __device__ static uint4 pack(const float* f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+template <>
+struct Chunk<bf16_t> {
+  static constexpr int N = 8;
+  __device__ static void unpack(const uint4& v, float* f) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  __device__ static uint4 pack(const float* f) {
+    return make_uint4(f32x2_to_bf16x2_bits(f[0], f[1]), f32x2_to_bf16x2_bits(f[2], f[3]),
+                      f32x2_to_bf16x2_bits(f[4], f[5]), f32x2_to_bf16x2_bits(f[6], f[7]));
+  }
+};
+template <>
+struct Chunk<f16_t> {
+  static constexpr int N = 8;
+  __device__ static void unpack(const uint4& v, float* f) {
+    const f16x8 h = __builtin_bit_cast(f16x8, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (float)h[i];
+  }
+  __device__ static uint4 pack(const float* f) {
+    return make_uint4(f32x2_to_f16x2_bits(f[0], f[1]), f32x2_to_f16x2_bits(f[2], f[3]),
+                      f32x2_to_f16x2_bits(f[4], f[5]), f32x2_to_f16x2_bits(f[6], f[7]));
+  }
+};
+
+// The element type of a 16-byte chunk decides how far its address may be from a 16-byte boundary: global memory
+// takes vector accesses at any element, so rows of odd length need no path of their own.
+typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
+typedef raw4 raw4_by2 __attribute__((aligned(2)));
+typedef raw4 raw4_by4 __attribute__((aligned(4)));
+template <typename T>
+using raw4_any = typename std::conditional<sizeof(T) == 2, raw4_by2, raw4_by4>::type;
+
+template <typename T>
+__device__ inline uint4 load_chunk_any(const T* p) {
+  typedef __attribute__((address_space(1))) const raw4_any<T>* global_ptr;
+  const raw4 v = *(global_ptr)(uintptr_t)p;
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+template <typename T>
+__device__ inline void store_chunk_any(T* p, const uint4& v) {
+  typedef __attribute__((address_space(1))) raw4_any<T>* global_ptr;
+  *(global_ptr)(uintptr_t)p = raw4{v.x, v.y, v.z, v.w};
+}
+
+template <typename T>
+__device__ inline uint32_t load_bits(const T* p) {
+  if constexpr (sizeof(T) == 4)
+    return *reinterpret_cast<const uint32_t*>(p);
+  else
+    return *reinterpret_cast<const uint16_t*>(p);
+}
+template <typename T>
+__device__ inline void store_bits(T* p, uint32_t b) {
+  if constexpr (sizeof(T) == 4)
+    *reinterpret_cast<uint32_t*>(p) = b;
+  else
+    *reinterpret_cast<uint16_t*>(p) = (uint16_t)b;
+}
+
+// Elements col .. col + N - 1 of a row of `len` elements; what lies past the end reads as zero and is not touched.
+template <typename T>
+__device__ inline uint4 load_chunk_tail(const T* row, int64_t col, int64_t len) {
+  constexpr int N = Chunk<T>::N;
+  if (col + N <= len) return load_chunk_any(row + col);
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (col + e < len) {
+      const uint32_t b = load_bits(row + col + e);
+      if constexpr (sizeof(T) == 4)
+        w[e] = b;
+      else
+        w[e >> 1] |= (e & 1) ? (b << 16) : b;
+    }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T>
+__device__ inline void store_chunk_tail(T* row, int64_t col, int64_t len, const uint4& v) {
+  constexpr int N = Chunk<T>::N;
+  if (col + N <= len) {
+    store_chunk_any(row + col, v);
+    return;
+  }
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (col + e < len) {
+      if constexpr (sizeof(T) == 4)
+        store_bits(row + col + e, w[e]);
+      else
+        store_bits(row + col + e, (e & 1) ? (w[e >> 1] >> 16) : (w[e >> 1] & 0xffffu));
+    }
+}
+
+// Sum / maximum over the 64 lanes of a wave; every lane gets the result, formed in the same order on every lane.
+__device__ inline float wave_sum(float v) {
+#pragma unroll
+  for (int m = 1; m < WAVE; m <<= 1) v += __shfl_xor(v, m, WAVE);
+  return v;
+}
+__device__ inline float wave_max(float v) {
+#pragma unroll
+  for (int m = 1; m < WAVE; m <<= 1) v = fmaxf(v, __shfl_xor(v, m, WAVE));
+  return v;
+}
+
+}  // namespace bgx

@@ -508,6 +508,120 @@ int bgx_gram_accumulate(const void* rows_dev, int32_t dtype, int64_t row_stride,
                         int32_t n_blocks, void* workspace_dev,
                         size_t workspace_bytes, void* stream);
 
+/* ---- operators of the model's own passes ---------------------------------
+ * What runs between the hooked Linear modules of a collection step
+ * (bergson/collector/collector.py:926-985 runs the model's forward pass, a
+ * loss and its backward pass): the norms, the attention, the loss.  All sums
+ * and statistics are fp32.  The entry points allocate nothing, keep nothing
+ * between calls and may be captured into a HIP graph.
+ *
+ * bgx_layernorm_forward: y[r] = (x[r] - mean) * rstd * weight + bias over rows
+ *   of d <= 16384 elements; rows start at any element (strides in elements,
+ *   last dimension contiguous).  weight / bias [d] in `weight_dtype`: that of x
+ *   or fp32; bias may be NULL.  mean_dev / rstd_dev [rows] fp32, both or neither.
+ * bgx_layernorm_backward: dx (NULL to skip), and when dweight_dev or dbias_dev
+ *   is given their sums over the rows, formed in a fixed order through the
+ *   workspace (bgx_layernorm_backward_workspace_bytes; needed only then). */
+int bgx_layernorm_forward(const void* x_dev, int64_t x_row_stride,
+                          const void* weight_dev, const void* bias_dev,
+                          int32_t weight_dtype, int64_t rows, int32_t d,
+                          int32_t dtype, float eps, void* y_dev,
+                          int64_t y_row_stride, float* mean_dev,
+                          float* rstd_dev, void* stream);
+size_t bgx_layernorm_backward_workspace_bytes(int64_t rows, int32_t d);
+int bgx_layernorm_backward(const void* dy_dev, int64_t dy_row_stride,
+                           const void* x_dev, int64_t x_row_stride,
+                           const void* weight_dev, int32_t weight_dtype,
+                           const float* mean_dev, const float* rstd_dev,
+                           int64_t rows, int32_t d, int32_t dtype, void* dx_dev,
+                           int64_t dx_row_stride, void* dweight_dev,
+                           void* dbias_dev, void* workspace_dev,
+                           size_t workspace_bytes, void* stream);
+
+/* Causal self-attention over whole sequences with grouped heads.  Query head h
+ * reads key/value head h / (heads / kv_heads).  Two layouts:
+ *   batch   (plan_dev NULL): n_seqs sequences of rows / n_seqs positions each;
+ *           lengths_dev [n_seqs] int32 or NULL cuts each to its first rows
+ *   packed  (plan_dev from bgx_attention_plan): sequences back to back in
+ *           `rows` rows
+ * Rows that belong to no sequence are not read; their outputs and gradients
+ * are zero.  Operands: element strides between sequences (batch layout),
+ * positions and heads, the head_dim (1..128) elements contiguous, any element
+ * alignment; stride 0 broadcasts an input.  scale must be positive.
+ * lse_dev [heads, rows] fp32 is what the backward pass needs of the softmax
+ * (NULL: forward only). */
+typedef struct bgx_attention_shape {
+  const void* plan_dev;
+  const int32_t* lengths_dev;
+  int64_t rows;
+  int32_t n_seqs;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+  float scale;
+} bgx_attention_shape;
+
+typedef struct bgx_attention_rows {
+  void* data;
+  int64_t seq_stride;
+  int64_t tok_stride;
+  int64_t head_stride;
+} bgx_attention_rows;
+
+/* bgx_attention_plan turns the sequences' boundaries cu_seqlens_dev
+ * [n_seqs + 1] int32 (device data, ascending, within 0..rows) into the list of
+ * tiles the kernels walk, longest first: bgx_attention_plan_bytes(rows, n_seqs)
+ * bytes, valid for every call with these boundaries.  Boundaries that are not
+ * ascending or lie outside 0..rows are clamped: which rows then count is
+ * unspecified, no access leaves the operands. */
+size_t bgx_attention_plan_bytes(int64_t rows, int32_t n_seqs);
+int bgx_attention_plan(const int32_t* cu_seqlens_dev, int32_t n_seqs,
+                       int64_t rows, void* plan_dev, size_t plan_bytes,
+                       void* stream);
+int bgx_attention_forward(const bgx_attention_shape* shape,
+                          const bgx_attention_rows* q,
+                          const bgx_attention_rows* k,
+                          const bgx_attention_rows* v,
+                          const bgx_attention_rows* out, float* lse_dev,
+                          void* stream);
+size_t bgx_attention_backward_workspace_bytes(const bgx_attention_shape* shape);
+int bgx_attention_backward(const bgx_attention_shape* shape,
+                           const bgx_attention_rows* q,
+                           const bgx_attention_rows* k,
+                           const bgx_attention_rows* v,
+                           const bgx_attention_rows* out, const float* lse_dev,
+                           const bgx_attention_rows* grad_out,
+                           const bgx_attention_rows* dq,
+                           const bgx_attention_rows* dk,
+                           const bgx_attention_rows* dv, void* workspace_dev,
+                           size_t workspace_bytes, void* stream);
+
+/* Distillation from a teacher's highest logits.  Per row (token) with
+ *   p = softmax(teacher / t) over the K entries with 0 <= id < V,
+ *   q = softmax(logits / t) over all V:
+ *   loss = t^2 sum_k p_k (log p_k - log q[id_k])
+ * losses_dev [rows] fp32; ids_dev [rows, K] int64 and teacher_dev [rows, K]
+ * (teacher_dtype) contiguous, K <= 1024, entries with an id outside 0..V-1 are
+ * none, an id may come more than once.  Rows without entries, and rows with
+ * valid_dev[r] == 0 (NULL = all valid), have loss 0 and gradient 0.
+ * stats_dev [rows, 2] fp32 is what the backward pass needs (NULL: losses only);
+ * bgx_distill_backward writes
+ *   dlogits = grad[r] * t * (q - sum of p over the entries of that id). */
+int bgx_distill_forward(const void* logits_dev, int64_t row_stride,
+                        int64_t rows, int32_t V, int32_t dtype,
+                        const int64_t* ids_dev, const void* teacher_dev,
+                        int32_t teacher_dtype, int32_t K,
+                        const uint8_t* valid_dev, float temperature,
+                        float* losses_dev, float* stats_dev, void* stream);
+int bgx_distill_backward(const void* logits_dev, int64_t row_stride,
+                         int64_t rows, int32_t V, int32_t dtype,
+                         const int64_t* ids_dev, const void* teacher_dev,
+                         int32_t teacher_dtype, int32_t K, float temperature,
+                         const float* stats_dev, const float* grad_dev,
+                         void* dlogits_dev, int64_t dlogits_row_stride,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

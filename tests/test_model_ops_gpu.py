@@ -1,0 +1,519 @@
+"""Layer norm, causal attention and top-k distillation against their definitions in 64 bits, elementwise within the
+bounds derived in model_reference.py; plus what must hold exactly: rows outside every sequence, masked tokens,
+repeated runs, other layouts of the same values, captured graphs."""
+import pytest
+import torch
+
+import bergson_amd as B
+from model_reference import assert_within, attention_reference, distill_reference, norm_reference
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+ids_of = lambda v: str(v).removeprefix("torch.").replace(" ", "")
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---- layer norm ---------------------------------------------------------------------------------------------------
+
+def _norm_case(rows, d, dtype, w_dtype, seed, device):
+    g = _gen(seed)
+    x = (torch.randn(rows, d, generator=g) * 2 + 0.5).to(dtype).to(device)
+    w = (1 + 0.3 * torch.randn(d, generator=g)).to(w_dtype).to(device)
+    b = (0.2 * torch.randn(d, generator=g)).to(w_dtype).to(device)
+    dy = torch.randn(rows, d, generator=g).to(dtype).to(device)
+    return x, w, b, dy
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("rows,d", [(1, 1), (1, 768), (3, 7), (5, 64), (37, 129), (66, 511), (9, 512), (4, 513),
+                                    (130, 1001), (7, 2047), (6, 2049), (5, 4096), (3, 5001), (2, 8193), (2, 16384),
+                                    (2100, 40)], ids=str)
+def test_layer_norm(device, rows, d, dtype):
+    x, w, b, dy = _norm_case(rows, d, dtype, dtype, rows * 31 + d, device)
+    for t in (x, w, b):
+        t.requires_grad_()
+    y = B.layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    ref = norm_reference(x, w, b, 1e-5, dy, dtype, dtype)
+    for name, got in (("y", y), ("dx", dx), ("dw", dw), ("db", db)):
+        assert got.dtype == dtype
+        assert_within(got, *ref[name], name)
+    with torch.no_grad():
+        assert torch.equal(B.layer_norm(x, w, b), y)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=ids_of)
+@pytest.mark.parametrize("d", [96, 1500, 5000])
+def test_layer_norm_fp32_weights(device, dtype, d):
+    x, w, b, dy = _norm_case(21, d, dtype, torch.float32, d, device)
+    for t in (x, w, b):
+        t.requires_grad_()
+    y = B.layer_norm(x, w, b, 1e-3)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    ref = norm_reference(x, w, b, 1e-3, dy, dtype, torch.float32)
+    for name, got in (("y", y), ("dx", dx), ("dw", dw), ("db", db)):
+        assert_within(got, *ref[name], name)
+
+
+def test_layer_norm_subsets_of_gradients(device):
+    """Frozen weights (a collection run), no bias, frozen input: each gradient equals the one of the full call."""
+    x, w, b, dy = _norm_case(70, 300, torch.bfloat16, torch.bfloat16, 5, device)
+    full = [t.clone().requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad(B.layer_norm(*full), full, dy)
+    for need in ((True, False, False), (False, True, False), (False, False, True), (False, True, True), (True, True, False)):
+        leaves = [t.clone().requires_grad_(n) for t, n in zip((x, w, b), need)]
+        asked = [t for t in leaves if t.requires_grad]
+        got = iter(torch.autograd.grad(B.layer_norm(*leaves), asked, dy))
+        for n, ref in zip(need, want):
+            if n:
+                assert torch.equal(next(got), ref)
+    xx, ww = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = B.layer_norm(xx, ww)
+    ref = norm_reference(x, w, None, 1e-5, dy, torch.bfloat16, torch.bfloat16)
+    dx, dw = torch.autograd.grad(y, (xx, ww), dy)
+    for name, got in (("y", y), ("dx", dx), ("dw", dw)):
+        assert_within(got, *ref[name], name)
+
+
+def test_layer_norm_layouts(device):
+    """Rows of a wider matrix, an odd storage offset, transposed and broadcast inputs: the values of a plain copy."""
+    g = _gen(3)
+    base = torch.randn(40, 210, generator=g).to(torch.bfloat16).to(device)
+    w, b = torch.rand(101, generator=g).to(torch.bfloat16).to(device), torch.zeros(101, dtype=torch.bfloat16, device=device)
+    views = [base[:, 3:104], base[::2, 7:108], base[:, :101].reshape(4, 10, 101).transpose(0, 1),
+             base.t()[:101].t(), base[:1, :101].expand(6, 101)]
+    for v in views:
+        a, c = v.detach().requires_grad_(), v.contiguous().clone().requires_grad_()
+        ya, yc = B.layer_norm(a, w, b), B.layer_norm(c, w, b)
+        assert torch.equal(ya, yc)
+        da, = torch.autograd.grad(ya.sum(), a)    # a broadcast output gradient
+        dc, = torch.autograd.grad(yc, c, torch.ones_like(yc))
+        assert torch.equal(da, dc)
+
+
+def test_layer_norm_empty_and_extreme(device):
+    w = torch.ones(16, device=device, requires_grad=True)
+    x = torch.zeros(0, 16, device=device, requires_grad=True)
+    y = B.layer_norm(x, w, w)
+    assert y.shape == (0, 16)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.zeros_like(y))
+    assert dx.shape == (0, 16) and dw.abs().sum() == 0
+    # constant rows: xh = 0, dx finite; a NaN or an infinity stays in its row
+    x = torch.full((3, 16), 1e4, device=device)
+    x[1, 3], x[2, 5] = float("nan"), float("inf")
+    y = B.layer_norm(x, w.detach(), None)
+    assert (y[0] == 0).all() and y[1].isnan().all() and y[2].isnan().any()
+    # a large common offset does not swallow the deviations
+    g = _gen(9)
+    x = (4096 + torch.randn(8, 600, generator=g)).to(device)
+    ref = norm_reference(x, torch.ones(600), None, 1e-5, None, torch.float32, torch.float32)
+    assert_within(B.layer_norm(x, torch.ones(600, device=device)), *ref["y"], "offset")
+
+
+# ---- causal attention ---------------------------------------------------------------------------------------------
+
+def _qkv(lead, heads, kv_heads, dim, dtype, seed, device, gain=1.2):
+    g = _gen(seed)
+    make = lambda n: (gain * torch.randn(*lead, n, dim, generator=g)).to(dtype).to(device)
+    return make(heads), make(kv_heads), make(kv_heads), make(heads)
+
+
+def _check_sequences(q, k, v, do, out, grads, spans, scale, dtype):
+    """Every sequence within its bounds, everything outside the sequences exactly zero."""
+    flat = lambda t: t.detach().reshape(-1, *t.shape[-2:])
+    q, k, v, do, out = map(flat, (q, k, v, do, out))
+    grads = [flat(t) for t in grads]
+    covered = torch.zeros(q.shape[0], dtype=torch.bool, device=q.device)
+    for a, b in spans:
+        covered[a:b] = True
+        if a == b:
+            continue
+        ref = attention_reference(q[a:b], k[a:b], v[a:b], scale, do[a:b], dtype)
+        for name, got in zip(("o", "dq", "dk", "dv"), (out, *grads)):
+            assert_within(got[a:b], *ref[name], f"{name} of rows {a}:{b}")
+    for t in (out, *grads):
+        assert (t[~covered] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (4, 2, 128), (3, 1, 32), (2, 1, 96), (1, 1, 80), (2, 2, 20),
+                                                (1, 1, 7)], ids=str)
+@pytest.mark.parametrize("lengths", [[1], [2, 33], [64, 1, 31, 65], [129, 127, 300]], ids=str)
+def test_attention_packed(device, lengths, heads, kv_heads, dim, dtype):
+    T = sum(lengths)
+    q, k, v, do = _qkv((T,), heads, kv_heads, dim, dtype, T + dim, device)
+    cu = torch.tensor([0] + lengths).cumsum(0).to(torch.int32).to(device)
+    for t in (q, k, v):
+        t.requires_grad_()
+    out = B.causal_attention(q, k, v, cu_seqlens=cu)
+    grads = torch.autograd.grad(out, (q, k, v), do)
+    ends = cu.tolist()
+    _check_sequences(q, k, v, do, out, grads, list(zip(ends, ends[1:])), dim ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("N,S,lengths", [(1, 1, None), (2, 130, None), (3, 200, [200, 0, 77]), (4, 64, [1, 64, 65, -3])],
+                         ids=str)
+def test_attention_batch(device, N, S, lengths, dtype):
+    """lengths beyond the width or below zero count as the width and zero."""
+    q, k, v, do = _qkv((N, S), 4, 2, 64, dtype, N * S, device)
+    for t in (q, k, v):
+        t.requires_grad_()
+    dev = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=device)
+    out = B.causal_attention(q, k, v, lengths=dev, scale=0.21)
+    grads = torch.autograd.grad(out, (q, k, v), do)
+    spans = [(n * S, n * S + min(max(l, 0), S)) for n, l in enumerate(lengths or [S] * N)]
+    _check_sequences(q, k, v, do, out, grads, spans, 0.21, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+def test_attention_rows_outside_the_sequences(device, dtype):
+    """NaN in rows before, after and between nothing reaches the sequences; those rows come out as zeros."""
+    T, cu_list = 400, [40, 100, 100, 260]
+    q, k, v, do = _qkv((T,), 2, 1, 64, dtype, 8, device)
+    outside = torch.ones(T, dtype=torch.bool, device=device)
+    outside[40:260] = False
+    for t in (q, k, v, do):
+        t[outside] = float("nan")
+    for t in (q, k, v):
+        t.requires_grad_()
+    cu = torch.tensor(cu_list, dtype=torch.int32, device=device)
+    out = B.causal_attention(q, k, v, cu_seqlens=cu)
+    grads = torch.autograd.grad(out, (q, k, v), do)
+    _check_sequences(q, k, v, do, out, grads, list(zip(cu_list, cu_list[1:])), 0.125, dtype)
+    # the same in the batch layout
+    qb, kb, vb, dob = (t.detach()[:400].reshape(2, 200, *t.shape[1:]).clone() for t in (q, k, v, do))
+    for t in (qb, kb, vb, dob):
+        t.nan_to_num_(nan=0.5)
+        t[0, 90:] = float("nan")
+        t[1, 7:] = float("inf")
+    for t in (qb, kb, vb):
+        t.requires_grad_()
+    out = B.causal_attention(qb, kb, vb, lengths=torch.tensor([90, 7], dtype=torch.int32, device=device))
+    grads = torch.autograd.grad(out, (qb, kb, vb), dob)
+    _check_sequences(qb, kb, vb, dob, out, grads, [(0, 90), (200, 207)], 0.125, dtype)
+
+
+def test_attention_layouts_and_broadcast(device):
+    """Views of one projection, heads before positions, shared keys by expand: the bits of plain copies, and the
+    gradient of a broadcast input is the sum over its copies."""
+    g = _gen(4)
+    qkv = torch.randn(2, 150, 3, 3 * 64, generator=g).to(torch.bfloat16).to(device)
+    do = torch.randn(2, 150, 3, 64, generator=g).to(torch.bfloat16).to(device)
+    views = [qkv.split(64, -1), [t.transpose(1, 2).contiguous().transpose(1, 2) for t in qkv.split(64, -1)]]
+    odd = torch.randn(2, 150, 3, 3 * 64 + 1, generator=g).to(torch.bfloat16).to(device)
+    odd[..., 1:].copy_(qkv)
+    views.append(odd[..., 1:].split(64, -1))
+    plain = [t.contiguous().requires_grad_() for t in views[0]]
+    want = B.causal_attention(*plain)
+    want_grads = torch.autograd.grad(want, plain, do)
+    for view in views:
+        leaves = [t.detach().requires_grad_() for t in view]
+        out = B.causal_attention(*leaves)
+        assert torch.equal(out, want)
+        for got, ref in zip(torch.autograd.grad(out, leaves, do), want_grads):
+            assert torch.equal(got, ref)
+    # a transposed output gradient and a broadcast one
+    leaves = [t.detach().requires_grad_() for t in views[0]]
+    out = B.causal_attention(*leaves)
+    a = torch.autograd.grad(out, leaves, do.transpose(1, 2).contiguous().transpose(1, 2), retain_graph=True)
+    assert all(torch.equal(x, y) for x, y in zip(a, want_grads))
+    a = torch.autograd.grad(out, leaves, torch.ones((), dtype=do.dtype, device=device).expand_as(out), retain_graph=True)
+    b = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    one = plain[1].detach()[:, :, :1].clone().requires_grad_()
+    shared = B.causal_attention(plain[0].detach(), one.expand(2, 150, 3, 64), plain[2].detach())
+    copied = plain[1].detach()[:, :, :1].repeat(1, 1, 3, 1).requires_grad_()
+    ref = B.causal_attention(plain[0].detach(), copied, plain[2].detach())
+    assert torch.equal(shared, ref)
+    got, = torch.autograd.grad(shared, one, do)
+    full, = torch.autograd.grad(ref, copied, do)
+    assert torch.equal(got, full.sum(2, keepdim=True))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+def test_attention_far_scores(device, dtype):
+    """Scores hundreds apart, -inf in a key (its weight is 0 wherever it is seen), keys at the type's lowest values."""
+    q, k, v, do = _qkv((140,), 1, 1, 32, dtype, 6, device, gain=6.0)
+    cu = torch.tensor([0, 140], dtype=torch.int32, device=device)
+    for t in (q, k, v):
+        t.requires_grad_()
+    out = B.causal_attention(q, k, v, cu_seqlens=cu, scale=1.0)
+    grads = torch.autograd.grad(out, (q, k, v), do)
+    _check_sequences(q, k, v, do, out, grads, [(0, 140)], 1.0, dtype)
+    # the first 64 keys give scores of -inf: the rows after them see only the rest
+    q2, k2 = q.detach().abs() + 0.1, k.detach().clone()
+    k2[:64, 0] = float("-inf")
+    out = B.causal_attention(q2.to(dtype), k2, v.detach(), cu_seqlens=cu)
+    rest = B.causal_attention(q2.to(dtype)[64:], k2[64:], v.detach()[64:],
+                              cu_seqlens=torch.tensor([0, 76], dtype=torch.int32, device=device))
+    ref = attention_reference(q2.to(dtype)[64:], k2[64:], v.detach()[64:], 32 ** -0.5, None, dtype)
+    assert_within(out[64:], *ref["o"], "rows that see finite scores")
+    assert_within(rest, *ref["o"], "the same rows alone")
+    assert out[:64].isnan().all()     # softmax of nothing but -inf
+
+
+def test_attention_small_gradients_in_fp16(device):
+    """Output gradients near fp16's smallest normal number: dS itself would vanish among the subnormals."""
+    q, k, v, do = _qkv((260,), 2, 1, 64, torch.float16, 12, device)
+    do = (do.float() * 2.0 ** -12).half()
+    do[:100] *= 2.0 ** -2
+    cu = torch.tensor([0, 260], dtype=torch.int32, device=device)
+    for t in (q, k, v):
+        t.requires_grad_()
+    grads = torch.autograd.grad(B.causal_attention(q, k, v, cu_seqlens=cu), (q, k, v), do)
+    big = torch.autograd.grad(B.causal_attention(q, k, v, cu_seqlens=cu), (q, k, v), (do.float() * 2.0 ** 12).half())
+    for small, large in zip(grads, big):
+        # scaled by a power of two: the same up to the rounding of the results among the subnormals
+        assert (small.double() - large.double() * 2.0 ** -12).abs().max() <= 2.0 ** -25 + 2.0 ** -11 * small.abs().max()
+    _check_sequences(q, k, v, do, B.causal_attention(q, k, v, cu_seqlens=cu), grads, [(0, 260)], 0.125, torch.float16)
+
+
+def test_attention_plan_of_many_sequences(device):
+    """More sequences than the planning workgroup has threads, empty ones among them, long ones at the end."""
+    g = _gen(2)
+    lengths = torch.randint(0, 4, (2600,), generator=g).tolist() + [500, 0, 300]
+    T = sum(lengths) + 5
+    q, k, v, _ = _qkv((T,), 1, 1, 32, torch.bfloat16, 1, device)
+    ends = [0] + torch.tensor(lengths).cumsum(0).tolist()
+    cu = torch.tensor(ends, dtype=torch.int32, device=device)
+    out = B.causal_attention(q, k, v, cu_seqlens=cu)
+    width = max(lengths)
+    N = len(lengths)
+    idx = (torch.tensor(ends[:-1])[:, None] + torch.arange(width)).clamp_max(T - 1).to(device)
+    lens = torch.tensor(lengths, dtype=torch.int32, device=device)
+    picked = [B.causal_attention(q[idx[a:a + 200]], k[idx[a:a + 200]], v[idx[a:a + 200]], lengths=lens[a:a + 200])
+              for a in range(0, N, 200)]
+    batch = torch.cat(picked)
+    keep = torch.arange(width, device=device) < lens[:, None]
+    assert torch.equal(out[:ends[-1]], batch[keep]) and (out[ends[-1]:] == 0).all()
+
+
+def test_attention_malformed_boundaries_stay_in_bounds(device):
+    """Boundaries that are not ascending or lie outside the rows: nothing is promised of the rows, but the call ends,
+    and a following call on the same memory is right."""
+    q, k, v, _ = _qkv((300,), 2, 2, 64, torch.bfloat16, 3, device)
+    for bad in ([0, 500, 200], [-7, 40, 300], [250, 100, 50], [0, 300, 0, 300, 0, 300]):
+        out = B.causal_attention(q, k, v, cu_seqlens=torch.tensor(bad, dtype=torch.int32, device=device))
+        assert out.shape == q.shape
+    cu = torch.tensor([0, 300], dtype=torch.int32, device=device)
+    torch.cuda.synchronize()
+    assert torch.equal(B.causal_attention(q, k, v, cu_seqlens=cu), B.causal_attention(q[None], k[None], v[None])[0])
+
+
+def test_attention_empty_inputs(device):
+    for shape, kw in (((0, 2, 32), dict(cu_seqlens=torch.zeros(1, dtype=torch.int32, device=device))),
+                      ((0, 5, 2, 32), {}), ((3, 0, 2, 32), {})):
+        q = torch.zeros(shape, device=device, requires_grad=True)
+        out = B.causal_attention(q, q, q, **kw)
+        assert out.shape == shape
+        assert torch.autograd.grad(out.sum(), q)[0].shape == shape
+    q = torch.randn(5, 2, 32, device=device, requires_grad=True)   # rows, but no sequence
+    out = B.causal_attention(q, q, q, cu_seqlens=torch.zeros(1, dtype=torch.int32, device=device))
+    assert (out == 0).all() and (torch.autograd.grad(out.sum(), q)[0] == 0).all()
+
+
+# ---- distillation -------------------------------------------------------------------------------------------------
+
+def _distill_case(rows, V, K, dtype, seed, device, t_dtype=None):
+    g = _gen(seed)
+    z = 2.5 * torch.randn(rows, V, generator=g)
+    top = torch.topk(z + torch.randn(rows, V, generator=g), K, dim=1)
+    grad = torch.rand(rows, generator=g) + 0.5
+    return z.to(dtype).to(device), top.indices.to(device), top.values.to(t_dtype or dtype).to(device), grad.to(device)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("rows,V,K,tau", [(1, 1, 1, 1.0), (3, 7, 2, 2.0), (5, 1000, 1, 1.0), (4, 2049, 300, 0.5),
+                                          (33, 511, 64, 3.0), (2, 50257, 8, 1.0), (2, 5000, 1024, 1.0)], ids=str)
+def test_distillation(device, rows, V, K, tau, dtype):
+    z, ids, t, grad = _distill_case(rows, V, K, dtype, V + K, device)
+    z.requires_grad_()
+    loss = B.topk_distillation(z, ids, t, temperature=tau)
+    dz, = torch.autograd.grad(loss, z, grad)
+    ref = distill_reference(z, ids, t, tau, None, grad, dtype)
+    assert loss.dtype == torch.float32 and dz.dtype == dtype
+    assert_within(loss, *ref["loss"], "loss")
+    assert_within(dz, *ref["dz"], "dz")
+    with torch.no_grad():
+        assert torch.equal(B.topk_distillation(z, ids, t, temperature=tau), loss)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+def test_distillation_entries(device, dtype):
+    """Missing entries, the same id twice, ids past the vocabulary, tokens without entries, excluded tokens with NaN
+    logits, a teacher entry of -inf."""
+    z, ids, t, grad = _distill_case(7, 300, 6, dtype, 5, device, torch.float32)
+    ids[0, 3:] = -1
+    ids[1, 4] = ids[1, 0]
+    ids[1, 5] = ids[1, 0]
+    ids[2, 0], ids[2, 1] = 300, 1 << 40
+    ids[3] = -1
+    t[4, 2] = float("-inf")
+    t[6] = float("-inf")
+    valid = torch.tensor([True, True, True, True, True, False, True], device=device)
+    z[3] = float("nan")
+    z[5] = float("inf")
+    z.requires_grad_()
+    loss = B.topk_distillation(z, ids, t, temperature=1.5, valid=valid)
+    dz, = torch.autograd.grad(loss, z, grad)
+    ref = distill_reference(z, ids, t, 1.5, valid, grad, dtype)
+    assert_within(loss, *ref["loss"], "loss")
+    assert_within(dz, *ref["dz"], "dz")
+    assert (loss[[3, 5, 6]] == 0).all() and (dz[[3, 5, 6]] == 0).all()
+
+
+def test_distillation_infinite_logits(device):
+    """A vocabulary masked with -inf: those entries have no mass and no gradient; a teacher entry among them makes its
+    token's loss infinite and leaves the others alone.  NaN stays in its token."""
+    z, ids, t, grad = _distill_case(4, 200, 3, torch.float32, 9, device)
+    keep = torch.zeros(4, 200, dtype=torch.bool, device=device).scatter_(1, ids, True)
+    keep |= torch.rand(4, 200, generator=_gen(1)).to(device) > 0.5
+    z[~keep] = float("-inf")
+    z[1, ids[1, 0]] = float("-inf")
+    z[2, 11] = float("nan")
+    z.requires_grad_()
+    loss = B.topk_distillation(z, ids, t)
+    dz, = torch.autograd.grad(loss, z, grad)
+    assert loss[1] == float("inf") and loss[2].isnan() and dz[2].isnan().any()
+    assert (dz[[0, 3]][~keep[[0, 3]]] == 0).all()
+    rows = [0, 3]
+    ref = distill_reference(z[rows].clamp_min(-1e4), ids[rows], t[rows], 1.0, None, grad[rows], torch.float32)
+    assert_within(loss[rows], *ref["loss"], "loss")
+    assert_within(dz[rows], *ref["dz"], "dz")
+
+
+def test_distillation_layouts(device):
+    """[N, S, V] views, rows of a wider matrix, an odd offset, int ids that are views: the bits of plain copies."""
+    z, ids, t, grad = _distill_case(12, 333, 5, torch.bfloat16, 2, device)
+    want_leaf = z.clone().requires_grad_()
+    want = B.topk_distillation(want_leaf, ids, t)
+    want_dz, = torch.autograd.grad(want, want_leaf, grad)
+    wide = torch.zeros(12, 400, dtype=z.dtype, device=device)
+    wide[:, 5:338] = z
+    for view in (wide[:, 5:338], z.t().contiguous().t()):
+        leaf = view.detach().requires_grad_()
+        loss = B.topk_distillation(leaf, ids.t().contiguous().t(), t)
+        assert torch.equal(loss, want)
+        assert torch.equal(torch.autograd.grad(loss, leaf, grad)[0], want_dz)
+    leaf = z.reshape(3, 4, 333).clone().requires_grad_()
+    loss = B.topk_distillation(leaf, ids.reshape(3, 4, 5), t.reshape(3, 4, 5))
+    assert loss.shape == (3, 4) and torch.equal(loss.flatten(), want)
+    assert torch.equal(torch.autograd.grad(loss.sum(), leaf)[0].reshape(12, 333),
+                       torch.autograd.grad(B.topk_distillation(want_leaf, ids, t).sum(), want_leaf)[0])
+    empty = torch.zeros(0, 333, device=device, requires_grad=True)
+    loss = B.topk_distillation(empty, ids[:0], t[:0])
+    assert loss.shape == (0,) and torch.autograd.grad(loss.sum(), empty)[0].shape == (0, 333)
+
+
+# ---- all of them --------------------------------------------------------------------------------------------------
+
+def _calls(device):
+    """(function of leaves, leaves, output gradient) of each operator at a size of a few tiles."""
+    x, w, b, dy = _norm_case(300, 768, torch.bfloat16, torch.bfloat16, 1, device)
+    q, k, v, do = _qkv((500,), 4, 2, 64, torch.float16, 2, device)
+    cu = torch.tensor([0, 130, 131, 420], dtype=torch.int32, device=device)
+    z, ids, t, g = _distill_case(40, 3001, 16, torch.bfloat16, 3, device)
+    return {"norm": (lambda *a: B.layer_norm(*a), (x, w, b), dy),
+            "attention": (lambda *a: B.causal_attention(*a, cu_seqlens=cu), (q, k, v), do),
+            "distill": (lambda a: B.topk_distillation(a, ids, t), (z,), g)}
+
+
+@pytest.mark.parametrize("which", ["norm", "attention", "distill"])
+def test_same_bits_every_time(device, which):
+    fn, leaves, grad = _calls(device)[which]
+    leaves = [t.requires_grad_() for t in leaves]
+    first = None
+    for _ in range(3):
+        out = fn(*leaves)
+        res = (out, *torch.autograd.grad(out, leaves, grad))
+        if first is None:
+            first = res
+        assert all(torch.equal(a, b) for a, b in zip(first, res))
+
+
+@pytest.mark.parametrize("which", ["norm", "attention", "distill"])
+def test_captured_and_replayed(device, which):
+    """Forward and backward in one graph, new values in the same leaves, eager work between the replays."""
+    fn, leaves, grad = _calls(device)[which]
+    static = [t.clone().requires_grad_() for t in leaves]
+
+    def step(args):
+        out = fn(*args)
+        return (out.detach(), *torch.autograd.grad(out, args, grad))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(static)
+    for i in range(4):
+        fresh = [(t.float() * (1 + 0.1 * i)).to(t.dtype) for t in leaves]
+        with torch.no_grad():
+            for s, f in zip(static, fresh):
+                s.copy_(f)
+        graph.replay()
+        want = step([f.requires_grad_() for f in fresh])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, want))
+
+
+@pytest.mark.parametrize("which", ["norm", "attention", "distill"])
+def test_on_another_stream(device, which):
+    fn, leaves, grad = _calls(device)[which]
+    leaves = [t.requires_grad_() for t in leaves]
+    out = fn(*leaves)
+    want = (out, *torch.autograd.grad(out, leaves, grad))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    results = []
+    for s in streams:      # two calls in flight at once
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            out = fn(*leaves)
+            results.append((out, *torch.autograd.grad(out, leaves, grad)))
+    torch.cuda.synchronize()
+    for res in results:
+        assert all(torch.equal(a, b) for a, b in zip(res, want))
+
+
+def test_gradients_against_differences(device):
+    """Directional derivatives of a scalar of each operator's fp32 output against central differences of the
+    operator's definition in 64 bits: the difference quotient is off by O(step^2), the kernel by its fp32 bounds."""
+    g = _gen(21)
+    x, w, b, dy = _norm_case(4, 50, torch.float32, torch.float32, 7, device)
+    q, k, v, do = _qkv((70,), 2, 1, 16, torch.float32, 7, device)
+    z, ids, t, gr = _distill_case(3, 90, 4, torch.float32, 7, device)
+    cu = torch.tensor([0, 70], dtype=torch.int32, device=device)
+    cases = [
+        (lambda *a: B.layer_norm(*a), (x, w, b), dy,
+         lambda x, w, b: norm_reference(x, w, b, 1e-5, None, torch.float32, torch.float32)["y"][0]),
+        (lambda *a: B.causal_attention(*a, cu_seqlens=cu), (q, k, v), do,
+         lambda q, k, v: attention_reference(q, k, v, 0.25, None, torch.float32)["o"][0]),
+        (lambda a: B.topk_distillation(a, ids, t), (z,), gr,
+         lambda z: distill_reference(z, ids, t, 1.0, None, None, torch.float32)["loss"][0]),
+    ]
+    for fn, leaves, grad, definition in cases:
+        leaves = [l.requires_grad_() for l in leaves]
+        grads = torch.autograd.grad(fn(*leaves), leaves, grad)
+        point = [l.detach().cpu().double() for l in leaves]
+        weight = grad.detach().cpu().double()
+        for i, gi in enumerate(grads):
+            direction = torch.randn(point[i].shape, generator=g, dtype=torch.float64)
+            step = 1e-5
+            ends = []
+            for sign in (1, -1):
+                moved = [p + sign * step * direction if j == i else p for j, p in enumerate(point)]
+                ends.append((definition(*moved) * weight).sum())
+            slope = (ends[0] - ends[1]) / (2 * step)
+            got = (gi.detach().cpu().double() * direction).sum()
+            size = (gi.detach().cpu().double() * direction).abs().sum()
+            # quotient: third derivatives times step^2 (1e-10) and 64-bit cancellation 1e-16 / 1e-5; kernel: fp32
+            # sums of up to a hundred terms, 2^-24 each
+            assert (got - slope).abs() <= 1e-5 * size + 1e-7, (i, got, slope)
