@@ -193,6 +193,7 @@ SIGNATURES: dict[str, tuple] = {
     "bgx_attention_plan_bytes": (C.c_size_t, [C.c_int64, C.c_int32]),
     "bgx_attention_plan": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]),
     "bgx_attention_forward": (C.c_int, [C.POINTER(AttentionShape), _ROWS, _ROWS, _ROWS, _ROWS, C.c_void_p, C.c_void_p]),
+    "bgx_attention_saved_bytes": (C.c_size_t, [C.POINTER(AttentionShape)]),
     "bgx_attention_backward_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionShape)]),
     "bgx_attention_backward": (
         C.c_int,

@@ -35,7 +35,12 @@ struct AttnView {
 
 struct AttnArgs {
   AttnView q, k, v, o, grad_o, dq, dk, dv;
-  float* lse;             // [Hq][rows]: log2 of the row's sum of 2^(scale log2(e) s)
+  // Of the softmax, per head and row: a shift of the exponents (the largest score in units of log 2) and the sum of
+  // 2^(score - shift).  Kept apart: the rounding of a shift cancels between a row's weights and their sum, that of a
+  // logarithm of the sum would not.
+  float* shift;           // [Hq][rows]
+  float* sum;             // [Hq][rows]
+  void* rest;             // [rows][Hq][D], 16-bit types: o minus its rounded value, rounded
   float* delta;           // [Hq][rows]
   float* peak;            // [Hq][rows]: largest |do| of the row (fp16 only)
   const int4* table;      // packed: {first row, length, tile, limit} per tile of AT_TILE rows, heaviest first
@@ -146,7 +151,7 @@ struct Staged {
 struct AttnItem {
   int64_t seq;   // sequence index of the batch layout (0 when packed)
   int64_t row0;  // first packed row of the sequence (0 in the batch layout)
-  int64_t stat;  // index of the sequence's first row in lse / delta
+  int64_t stat;  // index of the sequence's first row among all rows
   int len;       // rows of the sequence
   int limit;     // rows up to here (len .. limit - 1) belong to no sequence and become zero
   int tile;
@@ -205,26 +210,65 @@ __device__ inline const T* attn_rows(const AttnView& v, const AttnItem& it, int 
   return (const T*)v.p + it.seq * v.seq + it.row0 * v.tok + head * v.head;
 }
 
-// 32 rows (one per lane % 32) of an accumulator set [d, row] times `f`, as rows of the output
-template <typename T, int DP>
-__device__ inline void store_rows(const AttnView& view, const AttnItem& it, int head, int row, const f32x16 (&acc)[DP / 32],
-                                  float f, bool zero, int D, int lane) {
-  T* out = const_cast<T*>(attn_rows<T>(view, it, head)) + row * view.tok;
+// 32 rows (one per lane % 32) of an accumulator set [d, row], times `f`, written as rows of D elements from `out` (this
+// lane's row).  An accumulator holds 4 consecutive elements here and the next 4 in the wave's other half: at 16 bits two
+// such runs are exchanged between the halves, so that every store has 16 bytes.  REST: what the rounding cuts off
+// goes to `rest` in the same layout.
+template <typename T, int DP, bool REST = false>
+__device__ inline void store_rows(T* out, T* rest, const f32x16 (&acc)[DP / 32], float f, bool in, int D, int lane) {
+  const int half = lane >> 5;
 #pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt)
+  for (int dt = 0; dt < DP / 32; ++dt) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int d = dt * 32 + 8 * b + 4 * (lane >> 5);
+      for (int b = 0; b < 4; ++b) {
+        float v[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (d + e < D) store_as(out, d + e, zero ? 0.f : acc[dt][4 * b + e] * f, Elem<T>::code);
+        for (int e = 0; e < 4; ++e) v[e] = acc[dt][4 * b + e] * f;
+        const int d = dt * 32 + 8 * b + 4 * half;
+        if (in && d < D) store_chunk_tail(out, d, D, Chunk<T>::pack(v));
+      }
+    } else {
+#pragma unroll
+      for (int pair = 0; pair < 2; ++pair) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = acc[dt][8 * pair + e] * f;
+        const int d = dt * 32 + 8 * (2 * pair + half);
+        auto exchange = [](const uint4& w) {
+          const auto a = __builtin_amdgcn_permlane32_swap(w.x, w.z, false, false);
+          const auto b = __builtin_amdgcn_permlane32_swap(w.y, w.w, false, false);
+          return make_uint4(a[0], b[0], a[1], b[1]);
+        };
+        const uint4 w = Chunk<T>::pack(v);
+        const uint4 whole = exchange(w);
+        if (in && d < D) store_chunk_tail(out, d, D, whole);
+        if constexpr (REST) {
+          float r[8];
+          Chunk<T>::unpack(w, r);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) r[e] = v[e] - r[e];
+          const uint4 low = exchange(Chunk<T>::pack(r));
+          if (in && d < D) store_chunk_tail(rest, d, D, low);
+        }
+      }
     }
+  }
 }
 
+// this lane's half of a row becomes zero
 template <typename T, int DP>
-__device__ inline void zero_rows(const AttnView& view, const AttnItem& it, int head, int row, int D, int lane) {
-  f32x16 none[DP / 32];
-  store_rows<T, DP>(view, it, head, row, none, 0.f, true, D, lane);
+__device__ inline void zero_row(T* out, int D, int lane) {
+#pragma unroll
+  for (int c = 0; c < DP / Chunk<T>::N / 2; ++c) {
+    const int d = (2 * c + (lane >> 5)) * Chunk<T>::N;
+    if (d < D) store_chunk_tail(out, d, D, make_uint4(0u, 0u, 0u, 0u));
+  }
+}
+
+template <typename T>
+__device__ inline T* attn_row(const AttnView& v, const AttnItem& it, int head, int row) {
+  return const_cast<T*>(attn_rows<T>(v, it, head)) + row * v.tok;
 }
 
 // first-operand fragments of one row kept in registers (zeros for rows past the end)
@@ -259,7 +303,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_forward_kernel(AttnAr
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
   const int first = it.tile * AT_TILE, mine = first + wave * 32, row = mine + (lane & 31), half = lane >> 5;
   if (first >= it.len) {  // nothing of the sequence in this tile
-    if (row < it.limit) zero_rows<T, DP>(A.o, it, qh, row, A.D, lane);
+    if (row < it.limit) zero_row<T, DP>(attn_row<T>(A.o, it, qh, row), A.D, lane);
     return;
   }
   const T* q = attn_rows<T>(A.q, it, qh);
@@ -348,12 +392,22 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_forward_kernel(AttnAr
   }
   const float2 ls = both_halves(l);
   l = ls.x + ls.y;
-  if (row < it.len) {
-    store_rows<T, DP>(A.o, it, qh, row, o, 1.0f / l, false, A.D, lane);
-    if (A.lse != nullptr && half == 0) A.lse[(int64_t)qh * A.rows + it.stat + row] = m * c + log2f(l);
-  } else if (row < it.limit) {
-    zero_rows<T, DP>(A.o, it, qh, row, A.D, lane);
+  const bool in = row < it.len;
+  T* out = attn_row<T>(A.o, it, qh, row);
+  if (A.shift == nullptr) {
+    store_rows<T, DP>(out, nullptr, o, 1.0f / l, in, A.D, lane);
+  } else {
+    if (in && half == 0) {
+      const int64_t stat = (int64_t)qh * A.rows + it.stat + row;
+      A.shift[stat] = m * c;
+      A.sum[stat] = l;
+    }
+    if constexpr (sizeof(T) == 2)
+      store_rows<T, DP, true>(out, (T*)A.rest + ((it.stat + row) * A.Hq + qh) * A.D, o, 1.0f / l, in, A.D, lane);
+    else
+      store_rows<T, DP>(out, nullptr, o, 1.0f / l, in, A.D, lane);
   }
+  if (!in && row < it.limit) zero_row<T, DP>(out, A.D, lane);
 }
 
 // ---- backward: queries -------------------------------------------------------------------------------------------
@@ -371,7 +425,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_backward_q_kernel(Att
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
   const int first = it.tile * AT_TILE, mine = first + wave * 32, row = mine + (lane & 31), half = lane >> 5;
   if (first >= it.len) {
-    if (row < it.limit) zero_rows<T, DP>(A.dq, it, qh, row, A.D, lane);
+    if (row < it.limit) zero_row<T, DP>(attn_row<T>(A.dq, it, qh, row), A.D, lane);
     return;
   }
   const bool in = row < it.len;
@@ -382,11 +436,20 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_backward_q_kernel(Att
   float delta = 0.f, peak = 0.f;
   {
     load_own<T, DP>(attn_rows<T>(A.o, it, qh), A.o.tok, row, in, A.D, lane, qf);
+    uint4 rf[KS];
+    if constexpr (sizeof(T) == 2)
+      load_own<T, DP>((const T*)A.rest + (it.stat * A.Hq + qh) * A.D, (int64_t)A.Hq * A.D, row, in, A.D, lane, rf);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       float a[M::EPL], b[M::EPL];
       Chunk<T>::unpack(qf[ks], a);
       Chunk<T>::unpack(gf[ks], b);
+      if constexpr (sizeof(T) == 2) {  // delta stands against dp in fp32: it needs o unrounded
+        float r[M::EPL];
+        Chunk<T>::unpack(rf[ks], r);
+#pragma unroll
+        for (int e = 0; e < M::EPL; ++e) a[e] += r[e];
+      }
 #pragma unroll
       for (int e = 0; e < M::EPL; ++e) {
         delta = fmaf(a[e], b[e], delta);
@@ -407,7 +470,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_backward_q_kernel(Att
   // row's power of two is taken out of it (in the exponent of P, at no cost) and put back on dq.
   float lift = 0.f;
   if constexpr (HALF) lift = peak > 0.f && peak < INFINITY ? -(float)ilogbf(peak) : 0.f;
-  const float shift = in ? A.lse[stat] - lift : 0.f;
+  const float shift = in ? A.shift[stat] - lift : 0.f, over_sum = in ? 1.0f / A.sum[stat] : 0.f;
   const float c = A.scale * AT_LOG2E;
   f32x16 dq[DT];
 #pragma unroll
@@ -465,10 +528,9 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_backward_q_kernel(Att
       sv.store(lds[(t + 1) & 1][1]);
     }
   }
-  if (in)
-    store_rows<T, DP>(A.dq, it, qh, row, dq, A.scale * exp2_of(-lift), false, A.D, lane);
-  else if (row < it.limit)
-    zero_rows<T, DP>(A.dq, it, qh, row, A.D, lane);
+  T* out = attn_row<T>(A.dq, it, qh, row);
+  store_rows<T, DP>(out, nullptr, dq, A.scale * over_sum * exp2_of(-lift), in, A.D, lane);
+  if (!in && row < it.limit) zero_row<T, DP>(out, A.D, lane);
 }
 
 // ---- backward: keys and values -----------------------------------------------------------------------------------
@@ -479,7 +541,8 @@ __global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(At
   constexpr int BQ = attn_block_keys<T>(), KS = DP / (2 * M::EPL), SUB = BQ / 32, G = 32 / M::GROUP, DT = DP / 32;
   constexpr int BYTES = BQ * Tile<T, DP>::PITCH;
   __shared__ __attribute__((aligned(16))) char lds[2][2][BYTES];
-  __shared__ __attribute__((aligned(16))) float stats[2][3][BQ];
+  constexpr int NSTAT = std::is_same<T, bf16_t>::value ? 2 : 3;
+  __shared__ __attribute__((aligned(16))) float stats[2][NSTAT][BQ];
   AttnItem it;
   int kvh, qh0;
   if (!attn_item(A, true, it, kvh, qh0)) return;
@@ -487,8 +550,8 @@ __global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(At
   const int first = it.tile * AT_TILE, mine = first + wave * 32, row = mine + (lane & 31), half = lane >> 5;
   if (first >= it.len) {
     if (row < it.limit) {
-      zero_rows<T, DP>(A.dk, it, kvh, row, A.D, lane);
-      zero_rows<T, DP>(A.dv, it, kvh, row, A.D, lane);
+      zero_row<T, DP>(attn_row<T>(A.dk, it, kvh, row), A.D, lane);
+      zero_row<T, DP>(attn_row<T>(A.dv, it, kvh, row), A.D, lane);
     }
     return;
   }
@@ -504,7 +567,9 @@ __global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(At
   const float c = A.scale * AT_LOG2E;
   const int t0 = first / BQ, per_head = (it.len + BQ - 1) / BQ - t0, n_tiles = per_head * A.group;
   Staged<T, DP, BQ> sq, sg;
-  float stage[3] = {0.f, 0.f, 0.f};
+  float stage[NSTAT];
+#pragma unroll
+  for (int i = 0; i < NSTAT; ++i) stage[i] = 0.f;
   auto load = [&](int t) {
     const int qh = qh0 + t / per_head, q0 = (t0 + t % per_head) * BQ;
     sq.load(attn_rows<T>(A.q, it, qh), A.q.tok, q0, it.len, A.D);
@@ -512,7 +577,13 @@ __global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(At
     if (threadIdx.x < BQ) {
       const bool ok = q0 + (int)threadIdx.x < it.len;
       const int64_t stat = (int64_t)qh * A.rows + it.stat + q0 + threadIdx.x;
-      stage[0] = ok ? A.lse[stat] : 0.f;
+      const float sum = ok ? A.sum[stat] : 1.f;
+      stage[0] = ok ? A.shift[stat] : 0.f;
+      // at 16 bits the sum joins the exponent (its rounding there is far below that of the weights); in fp32 it does not
+      if constexpr (sizeof(T) == 2)
+        stage[0] += log2f(sum);
+      else
+        stage[2] = 1.0f / sum;
       stage[1] = ok ? A.delta[stat] : 0.f;
       if constexpr (HALF) stage[2] = ok ? A.peak[stat] : 0.f;
     }
@@ -521,9 +592,8 @@ __global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(At
     sq.store(lds[b][0]);
     sg.store(lds[b][1]);
     if (threadIdx.x < BQ) {
-      stats[b][0][threadIdx.x] = stage[0];
-      stats[b][1][threadIdx.x] = stage[1];
-      if constexpr (HALF) stats[b][2][threadIdx.x] = stage[2];
+#pragma unroll
+      for (int i = 0; i < NSTAT; ++i) stats[b][i][threadIdx.x] = stage[i];
     }
   };
   // fp16: dS carries a power of two that keeps it out of the subnormals, the one that fits the largest |do| seen so
@@ -564,13 +634,17 @@ __global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(At
       for (int u = 0; u < SUB; ++u) {
         if (q0 + u * 32 + 31 < mine) continue;  // all of these queries come before this wave's keys
         f32x16 s, dp;
-        float lse[16];
+        float lse[16], over_sum[sizeof(T) == 4 ? 16 : 1];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           const float4 a = *reinterpret_cast<const float4*>(&st[0][u * 32 + 8 * b + 4 * half]);
           const float4 d = *reinterpret_cast<const float4*>(&st[1][u * 32 + 8 * b + 4 * half]);
           lse[4 * b] = a.x, lse[4 * b + 1] = a.y, lse[4 * b + 2] = a.z, lse[4 * b + 3] = a.w;
           dp[4 * b] = -d.x, dp[4 * b + 1] = -d.y, dp[4 * b + 2] = -d.z, dp[4 * b + 3] = -d.w;
+          if constexpr (sizeof(T) == 4) {
+            const float4 w = *reinterpret_cast<const float4*>(&st[2][u * 32 + 8 * b + 4 * half]);
+            over_sum[4 * b] = w.x, over_sum[4 * b + 1] = w.y, over_sum[4 * b + 2] = w.z, over_sum[4 * b + 3] = w.w;
+          }
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = 0.f;
@@ -582,6 +656,7 @@ __global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(At
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           s[i] = exp2_of(fmaf(s[i], c, -lse[i]));
+          if constexpr (sizeof(T) == 4) s[i] *= over_sum[i];
           dp[i] = HALF ? s[i] * raise * dp[i] : s[i] * dp[i];
         }
         if (q0 + u * 32 < mine + 31) {
@@ -602,12 +677,13 @@ __global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(At
     }
     if (more) store((t + 1) & 1);
   }
-  if (in) {
-    store_rows<T, DP>(A.dk, it, kvh, row, dk, A.scale * exp2_of(-(float)lift), false, A.D, lane);
-    store_rows<T, DP>(A.dv, it, kvh, row, dv, 1.0f, false, A.D, lane);
-  } else if (row < it.limit) {
-    zero_rows<T, DP>(A.dk, it, kvh, row, A.D, lane);
-    zero_rows<T, DP>(A.dv, it, kvh, row, A.D, lane);
+  T* out_k = attn_row<T>(A.dk, it, kvh, row);
+  T* out_v = attn_row<T>(A.dv, it, kvh, row);
+  store_rows<T, DP>(out_k, nullptr, dk, A.scale * exp2_of(-(float)lift), in, A.D, lane);
+  store_rows<T, DP>(out_v, nullptr, dv, 1.0f, in, A.D, lane);
+  if (!in && row < it.limit) {
+    zero_row<T, DP>(out_k, A.D, lane);
+    zero_row<T, DP>(out_v, A.D, lane);
   }
 }
 
@@ -773,8 +849,22 @@ int attention_plan_impl(const int32_t* cu, int n_seqs, int64_t rows, void* plan,
   return 0;
 }
 
+// the saved buffer: shift and sum of every head and row, then the rest of the output
+size_t attention_saved_bytes(const bgx_attention_shape* a) {
+  if (a == nullptr || a->rows <= 0 || a->heads <= 0 || a->head_dim <= 0) return 0;
+  const size_t n = (size_t)a->rows * a->heads;
+  return n * 2 * sizeof(float) + (a->dtype == BGX_F32 ? 0 : n * a->head_dim * dtype_size(a->dtype));
+}
+
+static void attn_saved(AttnArgs& A, const bgx_attention_shape* a, void* saved) {
+  const int64_t n = a->rows * a->heads;
+  A.shift = (float*)saved;
+  A.sum = saved == nullptr ? nullptr : A.shift + n;
+  A.rest = saved == nullptr ? nullptr : A.sum + n;
+}
+
 int attention_forward_impl(const bgx_attention_shape* a, const bgx_attention_rows* q, const bgx_attention_rows* k,
-                           const bgx_attention_rows* v, const bgx_attention_rows* o, float* lse, void* stream) {
+                           const bgx_attention_rows* v, const bgx_attention_rows* o, void* saved, void* stream) {
   if (int rc = attn_check(a, "attention")) return rc;
   if (a->rows == 0) return 0;
   BGX_REQUIRE(q && k && v && o && q->data && k->data && v->data && o->data, BGX_E_ARG, "attention: null operand");
@@ -783,7 +873,7 @@ int attention_forward_impl(const bgx_attention_shape* a, const bgx_attention_row
   A.k = attn_view(k);
   A.v = attn_view(v);
   A.o = attn_view(o);
-  A.lse = lse;
+  attn_saved(A, a, saved);
   const int64_t grid = attn_items(a) * a->heads;
   BGX_REQUIRE(grid < (1ll << 31), BGX_E_SHAPE, "attention: %lld workgroups", (long long)grid);
   BGX_ATTN_LAUNCH(attention_forward_kernel, a->dtype, a->head_dim, dim3((unsigned)grid), (hipStream_t)stream, A);
@@ -796,7 +886,7 @@ size_t attention_backward_workspace_bytes(const bgx_attention_shape* a) {
 }
 
 int attention_backward_impl(const bgx_attention_shape* a, const bgx_attention_rows* q, const bgx_attention_rows* k,
-                            const bgx_attention_rows* v, const bgx_attention_rows* o, const float* lse,
+                            const bgx_attention_rows* v, const bgx_attention_rows* o, const void* saved,
                             const bgx_attention_rows* grad_o, const bgx_attention_rows* dq, const bgx_attention_rows* dk,
                             const bgx_attention_rows* dv, void* ws, size_t ws_bytes, void* stream) {
   if (int rc = attn_check(a, "attention backward")) return rc;
@@ -804,7 +894,7 @@ int attention_backward_impl(const bgx_attention_shape* a, const bgx_attention_ro
   const bgx_attention_rows* all[] = {q, k, v, o, grad_o, dq, dk, dv};
   for (const bgx_attention_rows* t : all)
     BGX_REQUIRE(t != nullptr && t->data != nullptr, BGX_E_ARG, "attention backward: null operand");
-  BGX_REQUIRE(lse != nullptr, BGX_E_ARG, "attention backward: null lse");
+  BGX_REQUIRE(saved != nullptr, BGX_E_ARG, "attention backward: null saved");
   const size_t need = attention_backward_workspace_bytes(a);
   BGX_REQUIRE(ws != nullptr && ws_bytes >= need, BGX_E_WORKSPACE, "attention backward: workspace of %zu bytes, %zu needed",
               ws_bytes, need);
@@ -817,7 +907,7 @@ int attention_backward_impl(const bgx_attention_shape* a, const bgx_attention_ro
   A.dq = attn_view(dq);
   A.dk = attn_view(dk);
   A.dv = attn_view(dv);
-  A.lse = const_cast<float*>(lse);
+  attn_saved(A, a, const_cast<void*>(saved));
   A.delta = (float*)ws;
   A.peak = A.delta + a->rows * a->heads;
   const int64_t items = attn_items(a);

@@ -146,10 +146,11 @@ int layernorm_backward_impl(const void* dy, int64_t dy_stride, const void* x, in
 size_t attention_plan_bytes(int64_t rows, int n_seqs);
 int attention_plan_impl(const int32_t* cu, int n_seqs, int64_t rows, void* plan, size_t plan_bytes, void* stream);
 int attention_forward_impl(const bgx_attention_shape* shape, const bgx_attention_rows* q, const bgx_attention_rows* k,
-                           const bgx_attention_rows* v, const bgx_attention_rows* out, float* lse, void* stream);
+                           const bgx_attention_rows* v, const bgx_attention_rows* out, void* saved, void* stream);
+size_t attention_saved_bytes(const bgx_attention_shape* shape);
 size_t attention_backward_workspace_bytes(const bgx_attention_shape* shape);
 int attention_backward_impl(const bgx_attention_shape* shape, const bgx_attention_rows* q, const bgx_attention_rows* k,
-                            const bgx_attention_rows* v, const bgx_attention_rows* out, const float* lse,
+                            const bgx_attention_rows* v, const bgx_attention_rows* out, const void* saved,
                             const bgx_attention_rows* grad_out, const bgx_attention_rows* dq,
                             const bgx_attention_rows* dk, const bgx_attention_rows* dv, void* ws, size_t ws_bytes,
                             void* stream);
@@ -405,20 +406,22 @@ int bgx_attention_plan(const int32_t* cu_seqlens_dev, int32_t n_seqs, int64_t ro
 }
 
 int bgx_attention_forward(const bgx_attention_shape* shape, const bgx_attention_rows* q, const bgx_attention_rows* k,
-                          const bgx_attention_rows* v, const bgx_attention_rows* out, float* lse_dev, void* stream) {
-  return bgx::attention_forward_impl(shape, q, k, v, out, lse_dev, stream);
+                          const bgx_attention_rows* v, const bgx_attention_rows* out, void* saved_dev, void* stream) {
+  return bgx::attention_forward_impl(shape, q, k, v, out, saved_dev, stream);
 }
+
+size_t bgx_attention_saved_bytes(const bgx_attention_shape* shape) { return bgx::attention_saved_bytes(shape); }
 
 size_t bgx_attention_backward_workspace_bytes(const bgx_attention_shape* shape) {
   return bgx::attention_backward_workspace_bytes(shape);
 }
 
 int bgx_attention_backward(const bgx_attention_shape* shape, const bgx_attention_rows* q, const bgx_attention_rows* k,
-                           const bgx_attention_rows* v, const bgx_attention_rows* out, const float* lse_dev,
+                           const bgx_attention_rows* v, const bgx_attention_rows* out, const void* saved_dev,
                            const bgx_attention_rows* grad_out, const bgx_attention_rows* dq,
                            const bgx_attention_rows* dk, const bgx_attention_rows* dv, void* workspace_dev,
                            size_t workspace_bytes, void* stream) {
-  return bgx::attention_backward_impl(shape, q, k, v, out, lse_dev, grad_out, dq, dk, dv, workspace_dev,
+  return bgx::attention_backward_impl(shape, q, k, v, out, saved_dev, grad_out, dq, dk, dv, workspace_dev,
                                       workspace_bytes, stream);
 }
 

@@ -548,8 +548,9 @@ int bgx_layernorm_backward(const void* dy_dev, int64_t dy_row_stride,
  * are zero.  Operands: element strides between sequences (batch layout),
  * positions and heads, the head_dim (1..128) elements contiguous, any element
  * alignment; stride 0 broadcasts an input.  scale must be positive.
- * lse_dev [heads, rows] fp32 is what the backward pass needs of the softmax
- * (NULL: forward only). */
+ * saved_dev (bgx_attention_saved_bytes; NULL: forward only) receives what the
+ * backward pass needs of the forward pass beside out: the softmax statistics,
+ * and for 16-bit types what the rounding of out has cut off. */
 typedef struct bgx_attention_shape {
   const void* plan_dev;
   const int32_t* lengths_dev;
@@ -579,18 +580,20 @@ size_t bgx_attention_plan_bytes(int64_t rows, int32_t n_seqs);
 int bgx_attention_plan(const int32_t* cu_seqlens_dev, int32_t n_seqs,
                        int64_t rows, void* plan_dev, size_t plan_bytes,
                        void* stream);
+size_t bgx_attention_saved_bytes(const bgx_attention_shape* shape);
 int bgx_attention_forward(const bgx_attention_shape* shape,
                           const bgx_attention_rows* q,
                           const bgx_attention_rows* k,
                           const bgx_attention_rows* v,
-                          const bgx_attention_rows* out, float* lse_dev,
+                          const bgx_attention_rows* out, void* saved_dev,
                           void* stream);
 size_t bgx_attention_backward_workspace_bytes(const bgx_attention_shape* shape);
 int bgx_attention_backward(const bgx_attention_shape* shape,
                            const bgx_attention_rows* q,
                            const bgx_attention_rows* k,
                            const bgx_attention_rows* v,
-                           const bgx_attention_rows* out, const float* lse_dev,
+                           const bgx_attention_rows* out,
+                           const void* saved_dev,
                            const bgx_attention_rows* grad_out,
                            const bgx_attention_rows* dq,
                            const bgx_attention_rows* dk,

@@ -146,11 +146,14 @@ def test_c_abi_refusals():
     assert fwd(shape(rows=11)) == -1 and b"one width" in lib.bgx_last_error()
     assert fwd(shape(rows=1 << 31)) == -3
     assert fwd(shape(rows=0, n_seqs=0)) == 0
-    bwd = lambda s, lse=P, ws=P, nbytes=1 << 20: lib.bgx_attention_backward(
-        s, rows, rows, rows, rows, lse, rows, rows, rows, rows, ws, nbytes, None)
-    assert bwd(shape(), lse=None) == -1 and b"lse" in lib.bgx_last_error()
+    bwd = lambda s, saved=P, ws=P, nbytes=1 << 20: lib.bgx_attention_backward(
+        s, rows, rows, rows, rows, saved, rows, rows, rows, rows, ws, nbytes, None)
+    assert bwd(shape(), saved=None) == -1 and b"saved" in lib.bgx_last_error()
     assert bwd(shape(), ws=None) == -4 and bwd(shape(), nbytes=16) == -4
     assert lib.bgx_attention_backward_workspace_bytes(shape()) == 10 * 4 * 4
+    # two statistics per head and row; at 16 bits also what the output's rounding cuts off
+    assert lib.bgx_attention_saved_bytes(shape()) == 10 * 4 * (2 * 4 + 16 * 2)
+    assert lib.bgx_attention_saved_bytes(shape(dtype=0)) == 10 * 4 * 2 * 4
     assert lib.bgx_attention_plan_bytes(1000, 3) == (1000 // 128 + 3 + 2) * 16
     assert lib.bgx_attention_plan(P, 3, 1000, P, 16, None) == -4
     assert lib.bgx_attention_plan(None, 3, 1000, P, 1 << 20, None) == -1

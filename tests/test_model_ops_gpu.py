@@ -517,3 +517,32 @@ def test_gradients_against_differences(device):
             # quotient: third derivatives times step^2 (1e-10) and 64-bit cancellation 1e-16 / 1e-5; kernel: fp32
             # sums of up to a hundred terms, 2^-24 each
             assert (got - slope).abs() <= 1e-5 * size + 1e-7, (i, got, slope)
+
+
+@pytest.mark.parametrize("which", ["norm", "attention", "distill"])
+def test_differentiable_once(device, which):
+    fn, leaves, grad = _calls(device)[which]
+    leaves = [t.requires_grad_() for t in leaves]
+    want = torch.autograd.grad(fn(*leaves), leaves, grad)
+    got = torch.autograd.grad(fn(*leaves), leaves, grad, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        got[0].float().sum().backward()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+def test_attention_gradients_that_cancel(device, dtype):
+    """Sequences of one token: the softmax is constant, dq and dk vanish; what is left is the fp32 rounding of
+    dp - delta, two sums of D products in different orders."""
+    q, k, v, do = _qkv((40,), 4, 2, 64, dtype, 30, device)
+    cu = torch.arange(41, dtype=torch.int32, device=device)
+    for t in (q, k, v):
+        t.requires_grad_()
+    dq, dk, dv = torch.autograd.grad(B.causal_attention(q, k, v, cu_seqlens=cu), (q, k, v), do)
+    vq, kq = (t.detach().repeat_interleave(2, 1).double() for t in (v, k))
+    # o is v exactly in fp32 and held with twice the type's bits: half a step of it squared is the type's share
+    half = torch.finfo(dtype).eps / 2
+    e = (2 * 64 * 2.0 ** -24 + (half * half if dtype != torch.float32 else 2.0 ** -24)) * (do.double() * vq).abs().sum(2)
+    assert (dq.double().abs() <= 0.125 * e[..., None] * kq.abs() * 1.01 + 1e-7).all()
+    bound = 0.125 * (e[..., None] * q.detach().double().abs()).unflatten(1, (2, 2)).sum(2)
+    assert (dk.double().abs() <= bound * 1.01 + 1e-7).all()
