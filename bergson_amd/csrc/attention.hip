@@ -17,14 +17,17 @@
 // Scores, softmax statistics, probabilities' sums and all accumulators are fp32.  For 16-bit inputs P and dS are
 // rounded to the inputs' type as operands of the matrix instructions (the products of 16-bit operands are what runs
 // at the card's rate; each rounding is relative to the value, and their sum over a row averages out).
-#include "rows.hpp"
+#include <initializer_list>
+
 #include "mma32.hpp"
+#include "rows.hpp"
 
 namespace bgx {
 
 constexpr int AT_WAVES = 4;
 constexpr int AT_THREADS = AT_WAVES * WAVE;
-constexpr int AT_TILE = 32 * AT_WAVES;  // rows a workgroup owns: 32 per wave
+constexpr int AT_TILES[2] = {128, 32};  // rows a workgroup owns (see Work)
+constexpr int AT_FEW = 512;  // fewer workgroups of 128 rows than this: workgroups of 32 rows
 constexpr int AT_MAX_D = 128;
 constexpr float AT_LOG2E = 1.4426950408889634f;
 
@@ -43,7 +46,7 @@ struct AttnArgs {
   void* rest;             // [rows][Hq][D], 16-bit types: o minus its rounded value, rounded
   float* delta;           // [Hq][rows]
   float* peak;            // [Hq][rows]: largest |do| of the row (fp16 only)
-  const int4* table;      // packed: {first row, length, tile, limit} per tile of AT_TILE rows, heaviest first
+  const int4* table;      // packed: {first row, length, tile, limit} per tile of rows, heaviest first
   const int32_t* lengths; // batch layout: [N] or NULL
   int64_t rows;           // N * S, or the packed rows
   int N, S, tiles;        // tiles: per sequence (batch layout) or entries (packed)
@@ -124,28 +127,106 @@ __device__ inline float2 both_halves(float x) {
   return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// `rows` rows of D elements from `base` as a buffer: a load past them returns zeros and touches no memory, so that the
+// ragged end of a sequence costs no branch (a branch around a load makes the compiler wait for the load where the paths
+// meet).  Rows are at least D elements apart.
+template <typename T>
+__device__ inline __amdgpu_buffer_rsrc_t row_buffer(const T* base, int64_t tok, int rows, int D) {
+  const int bytes = rows > 0 ? (int)(((rows - 1) * tok + D) * (int64_t)sizeof(T)) : 0;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, bytes, 0x00020000);
+}
+constexpr uint32_t NO_ROW = 0x7ffffff0u;  // an offset past every buffer
+
+__device__ inline uint4 buffer_load16(__amdgpu_buffer_rsrc_t r, uint32_t offset, uint32_t pass) {
+  typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
+  const raw4 v = __builtin_bit_cast(raw4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)offset, (int)pass, 0));
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+__device__ inline float buffer_load4(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
+  return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, (int)offset, 0, 0));
+}
+
 // BK rows of a [rows, D] operand on their way to an LDS tile: loaded into registers a tile ahead, stored after the
-// current tile's work.  Rows from `len` on and columns from D on become zeros and are not read.
+// current tile's work.  Rows past the end and columns from D on become zeros.  A thread keeps one
+// chunk of columns and takes every RPI-th row: its place in a tile is one 32-bit offset, made once; what changes from
+// tile to tile is a uniform base.
 template <typename T, int DP, int BK>
 struct Staged {
-  static constexpr int CH = Tile<T, DP>::CHUNKS, PER = (BK * CH + AT_THREADS - 1) / AT_THREADS;
+  static constexpr int CH = Tile<T, DP>::PITCH / 16;  // threads per row (with DP = 96 a quarter of them idles)
+  static constexpr int RPI = AT_THREADS / CH, PER = BK / RPI;
+  static_assert(BK % RPI == 0, "whole passes over a tile");
   uint4 v[PER];
-  __device__ void load(const T* base, int64_t tok, int row0, int len, int D) {
+  uint32_t offset, pass;
+  __device__ void init(int64_t tok, int D) {
+    const int chunk = threadIdx.x % CH, row = threadIdx.x / CH;
+    offset = chunk * Chunk<T>::N < D ? (uint32_t)(row * (int)tok + chunk * Chunk<T>::N) * (uint32_t)sizeof(T) : NO_ROW;
+    pass = (uint32_t)(RPI * (int)tok) * (uint32_t)sizeof(T);
+  }
+  // rows: how many rows there are from the tile's first on
+  __device__ void load(const T* base, int64_t tok, int rows, int D) {
+    const __amdgpu_buffer_rsrc_t r = row_buffer(base, tok, min(rows, BK), D);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int idx = threadIdx.x + i * AT_THREADS, row = idx / CH, col = (idx % CH) * Chunk<T>::N;
-      v[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (row < BK && row0 + row < len && col < D) v[i] = load_chunk_tail(base + (row0 + row) * tok, col, D);
-    }
+    for (int i = 0; i < PER; ++i) v[i] = buffer_load16(r, offset, i * pass);
   }
   __device__ void store(char* tile) const {
+    if (DP == 96 && (int)threadIdx.x % CH >= Tile<T, DP>::CHUNKS) return;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int idx = threadIdx.x + i * AT_THREADS, row = idx / CH;
-      if (row < BK) *reinterpret_cast<uint4*>(tile + Tile<T, DP>::at(row, idx % CH)) = v[i];
-    }
+    for (int i = 0; i < PER; ++i)
+      *reinterpret_cast<uint4*>(tile + Tile<T, DP>::at(threadIdx.x / CH + i * RPI, threadIdx.x % CH)) = v[i];
   }
 };
+
+// ---- how a workgroup's waves divide the work ---------------------------------------------------------------------
+// A workgroup owns 32 * RW rows (queries, or keys in the kernel for dk and dv) and walks the other side in tiles of
+// STEP rows.  RW = 4: every wave owns 32 rows and takes each tile whole.  RW = 1: all four waves share 32 rows, each
+// takes a quarter of every tile, and their sums are joined through LDS at the end -- four times the workgroups with
+// a quarter of the walk each, at four times the traffic to LDS: for calls that would not fill the chip otherwise.
+template <typename T, int DP, int RW>
+struct Work {
+  static constexpr int ROWS = 32 * RW, SPLIT = AT_WAVES / RW;
+  static constexpr int SUB = RW == 4 && sizeof(T) == 2 ? 2 : 1;  // blocks of 32 a wave takes of a tile
+  static constexpr int STEP = 32 * SUB * SPLIT;
+  // waves a SIMD has room for without spilling registers to memory (the compiler's budget: 512 / 2 or 512)
+  static constexpr int WAVES_Q = sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : (RW == 4 || DP <= 64 ? 2 : 1);
+  static constexpr int WAVES_KV = sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : (DP <= 64 ? 2 : 1);
+  static constexpr int BYTES = STEP * Tile<T, DP>::PITCH;
+  static constexpr int BUFFERS = 4 * BYTES <= 65536 ? 2 : 1;  // two workgroups of a CU fit at 16 bits
+  static constexpr int JOIN = (SPLIT - 1) * RW * (DP / 32) * 16 * WAVE * 4;
+  static constexpr int LDS = 2 * BUFFERS * BYTES > JOIN ? 2 * BUFFERS * BYTES : JOIN;
+};
+
+// Sums of the waves that share rows: the others hand theirs to the first through LDS, which adds them in order.
+template <typename W, int DT>
+__device__ inline void join_waves(f32x16 (&acc)[DT], char* lds, int part, int lane) {
+  if constexpr (W::SPLIT > 1) {
+    static_assert(W::ROWS == 32, "one group of waves");
+    float4* box = reinterpret_cast<float4*>(lds);
+    __syncthreads();
+    if (part > 0) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          box[(((part - 1) * DT + dt) * 4 + b) * WAVE + lane] =
+              make_float4(acc[dt][4 * b], acc[dt][4 * b + 1], acc[dt][4 * b + 2], acc[dt][4 * b + 3]);
+    }
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int w = 0; w < W::SPLIT - 1; ++w) {
+            const float4 v = box[((w * DT + dt) * 4 + b) * WAVE + lane];
+            acc[dt][4 * b] += v.x;
+            acc[dt][4 * b + 1] += v.y;
+            acc[dt][4 * b + 2] += v.z;
+            acc[dt][4 * b + 3] += v.w;
+          }
+    }
+  }
+}
 
 // ---- what a workgroup works on -----------------------------------------------------------------------------------
 struct AttnItem {
@@ -173,6 +254,7 @@ __device__ inline void spread_heads(int u, int streams, int group, int& stream, 
 
 // keys: the workgroup owns key rows (all query heads of one key/value head, first tile heaviest) instead of query rows
 // (one query head, last tile heaviest).
+template <int ROWS>
 __device__ inline bool attn_item(const AttnArgs& A, bool keys, AttnItem& it, int& kv_head, int& q_head) {
   const int group = keys ? 1 : A.group;
   int g;
@@ -185,7 +267,7 @@ __device__ inline bool attn_item(const AttnArgs& A, bool keys, AttnItem& it, int
     it.row0 = it.stat = e.x;
     it.len = e.y;
     it.limit = e.w;
-    const int tiles = (e.y + AT_TILE - 1) / AT_TILE;
+    const int tiles = (e.y + ROWS - 1) / ROWS;
     it.tile = keys && e.y > 0 ? tiles - 1 - e.z : e.z;
   } else {
     const int per = A.N * A.Hk * group, rank = blockIdx.x / per;
@@ -226,7 +308,7 @@ __device__ inline void store_rows(T* out, T* rest, const f32x16 (&acc)[DP / 32],
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = acc[dt][4 * b + e] * f;
         const int d = dt * 32 + 8 * b + 4 * half;
-        if (in && d < D) store_chunk_tail(out, d, D, Chunk<T>::pack(v));
+        if (in && d < D) store_chunk_any(out + d, Chunk<T>::pack(v));
       }
     } else {
 #pragma unroll
@@ -242,14 +324,14 @@ __device__ inline void store_rows(T* out, T* rest, const f32x16 (&acc)[DP / 32],
         };
         const uint4 w = Chunk<T>::pack(v);
         const uint4 whole = exchange(w);
-        if (in && d < D) store_chunk_tail(out, d, D, whole);
+        if (in && d < D) store_chunk_any(out + d, whole);
         if constexpr (REST) {
           float r[8];
           Chunk<T>::unpack(w, r);
 #pragma unroll
           for (int e = 0; e < 8; ++e) r[e] = v[e] - r[e];
           const uint4 low = exchange(Chunk<T>::pack(r));
-          if (in && d < D) store_chunk_tail(rest, d, D, low);
+          if (in && d < D) store_chunk_any(rest + d, low);
         }
       }
     }
@@ -262,7 +344,7 @@ __device__ inline void zero_row(T* out, int D, int lane) {
 #pragma unroll
   for (int c = 0; c < DP / Chunk<T>::N / 2; ++c) {
     const int d = (2 * c + (lane >> 5)) * Chunk<T>::N;
-    if (d < D) store_chunk_tail(out, d, D, make_uint4(0u, 0u, 0u, 0u));
+    if (d < D) store_chunk_any(out + d, make_uint4(0u, 0u, 0u, 0u));
   }
 }
 
@@ -271,37 +353,33 @@ __device__ inline T* attn_row(const AttnView& v, const AttnItem& it, int head, i
   return const_cast<T*>(attn_rows<T>(v, it, head)) + row * v.tok;
 }
 
-// first-operand fragments of one row kept in registers (zeros for rows past the end)
+// first-operand fragments of one row kept in registers: row `row` of `rows` from `base` (zeros past the end)
 template <typename T, int DP>
-__device__ inline void load_own(const T* base, int64_t tok, int row, bool in, int D, int lane, uint4 (&f)[DP / (2 * Attn<T>::EPL)]) {
+__device__ inline void load_own(const T* base, int64_t tok, int row, int rows, int D, int lane, uint4 (&f)[DP / (2 * Attn<T>::EPL)]) {
   constexpr int EPL = Attn<T>::EPL;
+  const __amdgpu_buffer_rsrc_t r = row_buffer(base, tok, rows, D);
 #pragma unroll
   for (int ks = 0; ks < DP / (2 * EPL); ++ks) {
     const int col = (2 * ks + (lane >> 5)) * EPL;
-    f[ks] = make_uint4(0u, 0u, 0u, 0u);
-    if (in && col < D) f[ks] = load_chunk_tail(base + row * tok, col, D);
+    f[ks] = buffer_load16(r, col < D && row < rows ? (uint32_t)(row * (int)tok + col) * (uint32_t)sizeof(T) : NO_ROW, 0);
   }
 }
 
 __device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
-template <typename T>
-constexpr int attn_block_keys() {
-  return sizeof(T) == 4 ? 32 : 64;
-}
-
 // ---- forward -----------------------------------------------------------------------------------------------------
-template <typename T, int DP>
-__global__ __launch_bounds__(AT_THREADS, 2) void attention_forward_kernel(AttnArgs A) {
+template <typename T, int DP, int RW>
+__global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_Q)) void attention_forward_kernel(AttnArgs A) {
   using M = Attn<T>;
-  constexpr int BK = attn_block_keys<T>(), KS = DP / (2 * M::EPL), SUB = BK / 32, G = 32 / M::GROUP, DT = DP / 32;
-  constexpr int BYTES = BK * Tile<T, DP>::PITCH;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][BYTES];
+  using W = Work<T, DP, RW>;
+  constexpr int BK = W::STEP, KS = DP / (2 * M::EPL), SUB = W::SUB, G = 32 / M::GROUP, DT = DP / 32;
+  __shared__ __attribute__((aligned(16))) char lds[W::LDS];
   AttnItem it;
   int kvh, qh;
-  if (!attn_item(A, false, it, kvh, qh)) return;
+  if (!attn_item<W::ROWS>(A, false, it, kvh, qh)) return;
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
-  const int first = it.tile * AT_TILE, mine = first + wave * 32, row = mine + (lane & 31), half = lane >> 5;
+  const int part = wave / RW;  // which of the waves that share rows
+  const int first = it.tile * W::ROWS, mine = first + (wave % RW) * 32, row = mine + (lane & 31), half = lane >> 5;
   if (first >= it.len) {  // nothing of the sequence in this tile
     if (row < it.limit) zero_row<T, DP>(attn_row<T>(A.o, it, qh, row), A.D, lane);
     return;
@@ -310,7 +388,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_forward_kernel(AttnAr
   const T* k = attn_rows<T>(A.k, it, kvh);
   const T* v = attn_rows<T>(A.v, it, kvh);
   uint4 qf[KS];
-  load_own<T, DP>(q, A.q.tok, row, row < it.len, A.D, lane, qf);
+  load_own<T, DP>(q + first * A.q.tok, A.q.tok, row - first, it.len - first, A.D, lane, qf);
   f32x16 o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -318,22 +396,26 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_forward_kernel(AttnAr
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
   float m = -INFINITY, l = 0.f;
   const float c = A.scale * AT_LOG2E;
-  const int n_tiles = (min(first + AT_TILE, it.len) + BK - 1) / BK;
+  const int n_tiles = (min(first + W::ROWS, it.len) + BK - 1) / BK;
   Staged<T, DP, BK> sk, sv;
-  sk.load(k, A.k.tok, 0, it.len, A.D);
-  sv.load(v, A.v.tok, 0, it.len, A.D);
-  sk.store(lds[0][0]);
-  sv.store(lds[0][1]);
+  sk.init(A.k.tok, A.D);
+  sv.init(A.v.tok, A.D);
+  sk.load(k, A.k.tok, it.len, A.D);
+  sv.load(v, A.v.tok, it.len, A.D);
+  sk.store(lds);
+  sv.store(lds + W::BYTES);
   for (int t = 0; t < n_tiles; ++t) {
     __syncthreads();  // this tile is in LDS, and nobody reads the other buffer any more
     const bool more = t + 1 < n_tiles;
     if (more) {
-      sk.load(k, A.k.tok, (t + 1) * BK, it.len, A.D);
-      sv.load(v, A.v.tok, (t + 1) * BK, it.len, A.D);
+      const int next = (t + 1) * BK;
+      sk.load(k + next * A.k.tok, A.k.tok, it.len - next, A.D);
+      sv.load(v + next * A.v.tok, A.v.tok, it.len - next, A.D);
     }
-    const char* tk = lds[t & 1][0];
-    const char* tv = lds[t & 1][1];
-    const int k0 = t * BK;
+    const char* buf = lds + (W::BUFFERS == 2 ? (t & 1) * 2 * W::BYTES : 0);
+    const char* tk = buf + part * (SUB * 32) * Tile<T, DP>::PITCH;
+    const char* tv = tk + W::BYTES;
+    const int k0 = t * BK + part * (SUB * 32);
     if (k0 <= mine + 31 && mine < it.len) {
       f32x16 s[SUB];
 #pragma unroll
@@ -343,7 +425,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_forward_kernel(AttnAr
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) Mma32<T>::mma(read_rows<T, DP>(tk, u * 32, ks, lane), qf[ks], s[u]);
       }
-      if (k0 + BK - 1 > mine) {  // the tile reaches past some row's own position
+      if (k0 + SUB * 32 - 1 > mine) {  // the tile reaches past some row's own position
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
@@ -385,13 +467,35 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_forward_kernel(AttnAr
             Mma32<T>::mma(M::template read_tr<DP>(tv, u * 32 + g * M::GROUP, dt, lane), p, o[dt]);
         }
     }
+    if constexpr (W::BUFFERS == 1) __syncthreads();
     if (more) {
-      sk.store(lds[(t + 1) & 1][0]);
-      sv.store(lds[(t + 1) & 1][1]);
+      char* next = lds + (W::BUFFERS == 2 ? ((t + 1) & 1) * 2 * W::BYTES : 0);
+      sk.store(next);
+      sv.store(next + W::BYTES);
     }
   }
   const float2 ls = both_halves(l);
   l = ls.x + ls.y;
+  if constexpr (W::SPLIT > 1) {  // bring the waves' sums to the largest maximum of them
+    __shared__ float maxima[W::SPLIT][WAVE], sums[W::SPLIT][WAVE];
+    maxima[part][lane] = m;
+    __syncthreads();
+    float top = m;
+#pragma unroll
+    for (int w = 0; w < W::SPLIT; ++w) top = fmaxf(top, maxima[w][lane]);
+    const float f = m == -INFINITY ? 0.f : exp2_of((m - top) * c);
+    m = top;
+    l *= f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[dt][i] *= f;
+    sums[part][lane] = l;
+    join_waves<W, DT>(o, lds, part, lane);
+    if (part > 0) return;
+#pragma unroll
+    for (int w = 1; w < W::SPLIT; ++w) l += sums[w][lane];
+  }
   const bool in = row < it.len;
   T* out = attn_row<T>(A.o, it, qh, row);
   if (A.shift == nullptr) {
@@ -412,18 +516,19 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_forward_kernel(AttnAr
 
 // ---- backward: queries -------------------------------------------------------------------------------------------
 // dq of 32 queries a wave; also leaves delta (and, for fp16, the largest |do| of a row) for the other kernel.
-template <typename T, int DP>
-__global__ __launch_bounds__(AT_THREADS, 2) void attention_backward_q_kernel(AttnArgs A) {
+template <typename T, int DP, int RW>
+__global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_Q)) void attention_backward_q_kernel(AttnArgs A) {
   using M = Attn<T>;
+  using W = Work<T, DP, RW>;
   constexpr bool HALF = std::is_same<T, f16_t>::value;
-  constexpr int BK = attn_block_keys<T>(), KS = DP / (2 * M::EPL), SUB = BK / 32, G = 32 / M::GROUP, DT = DP / 32;
-  constexpr int BYTES = BK * Tile<T, DP>::PITCH;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][BYTES];
+  constexpr int BK = W::STEP, KS = DP / (2 * M::EPL), SUB = W::SUB, G = 32 / M::GROUP, DT = DP / 32;
+  __shared__ __attribute__((aligned(16))) char lds[W::LDS];
   AttnItem it;
   int kvh, qh;
-  if (!attn_item(A, false, it, kvh, qh)) return;
+  if (!attn_item<W::ROWS>(A, false, it, kvh, qh)) return;
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
-  const int first = it.tile * AT_TILE, mine = first + wave * 32, row = mine + (lane & 31), half = lane >> 5;
+  const int part = wave / RW;  // which of the waves that share rows
+  const int first = it.tile * W::ROWS, mine = first + (wave % RW) * 32, row = mine + (lane & 31), half = lane >> 5;
   if (first >= it.len) {
     if (row < it.limit) zero_row<T, DP>(attn_row<T>(A.dq, it, qh, row), A.D, lane);
     return;
@@ -432,13 +537,14 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_backward_q_kernel(Att
   const T* k = attn_rows<T>(A.k, it, kvh);
   const T* v = attn_rows<T>(A.v, it, kvh);
   uint4 qf[KS], gf[KS];
-  load_own<T, DP>(attn_rows<T>(A.grad_o, it, qh), A.grad_o.tok, row, in, A.D, lane, gf);
+  const int own = row - first, left = it.len - first;
+  load_own<T, DP>(attn_rows<T>(A.grad_o, it, qh) + first * A.grad_o.tok, A.grad_o.tok, own, left, A.D, lane, gf);
   float delta = 0.f, peak = 0.f;
   {
-    load_own<T, DP>(attn_rows<T>(A.o, it, qh), A.o.tok, row, in, A.D, lane, qf);
+    load_own<T, DP>(attn_rows<T>(A.o, it, qh) + first * A.o.tok, A.o.tok, own, left, A.D, lane, qf);
     uint4 rf[KS];
     if constexpr (sizeof(T) == 2)
-      load_own<T, DP>((const T*)A.rest + (it.stat * A.Hq + qh) * A.D, (int64_t)A.Hq * A.D, row, in, A.D, lane, rf);
+      load_own<T, DP>((const T*)A.rest + ((it.stat + first) * A.Hq + qh) * A.D, (int64_t)A.Hq * A.D, own, left, A.D, lane, rf);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       float a[M::EPL], b[M::EPL];
@@ -460,9 +566,9 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_backward_q_kernel(Att
     delta = d.x + d.y;
     peak = fmaxf(p.x, p.y);
   }
-  load_own<T, DP>(attn_rows<T>(A.q, it, qh), A.q.tok, row, in, A.D, lane, qf);
+  load_own<T, DP>(attn_rows<T>(A.q, it, qh) + first * A.q.tok, A.q.tok, own, left, A.D, lane, qf);
   const int64_t stat = (int64_t)qh * A.rows + it.stat + row;
-  if (in && half == 0) {
+  if (in && half == 0 && part == 0) {
     A.delta[stat] = delta;
     if constexpr (HALF) A.peak[stat] = peak;
   }
@@ -477,24 +583,28 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_backward_q_kernel(Att
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dq[dt][i] = 0.f;
-  const int n_tiles = (min(first + AT_TILE, it.len) + BK - 1) / BK;
+  const int n_tiles = (min(first + W::ROWS, it.len) + BK - 1) / BK;
   Staged<T, DP, BK> sk, sv;
-  sk.load(k, A.k.tok, 0, it.len, A.D);
-  sv.load(v, A.v.tok, 0, it.len, A.D);
-  sk.store(lds[0][0]);
-  sv.store(lds[0][1]);
+  sk.init(A.k.tok, A.D);
+  sv.init(A.v.tok, A.D);
+  sk.load(k, A.k.tok, it.len, A.D);
+  sv.load(v, A.v.tok, it.len, A.D);
+  sk.store(lds);
+  sv.store(lds + W::BYTES);
   for (int t = 0; t < n_tiles; ++t) {
     __syncthreads();
     const bool more = t + 1 < n_tiles;
     if (more) {
-      sk.load(k, A.k.tok, (t + 1) * BK, it.len, A.D);
-      sv.load(v, A.v.tok, (t + 1) * BK, it.len, A.D);
+      const int next = (t + 1) * BK;
+      sk.load(k + next * A.k.tok, A.k.tok, it.len - next, A.D);
+      sv.load(v + next * A.v.tok, A.v.tok, it.len - next, A.D);
     }
-    const char* tk = lds[t & 1][0];
-    const char* tv = lds[t & 1][1];
-    const int k0 = t * BK;
+    const char* buf = lds + (W::BUFFERS == 2 ? (t & 1) * 2 * W::BYTES : 0);
+    const char* tk = buf + part * (SUB * 32) * Tile<T, DP>::PITCH;
+    const char* tv = tk + W::BYTES;
+    const int k0 = t * BK + part * (SUB * 32);
     if (k0 <= mine + 31 && mine < it.len) {
-#pragma unroll
+#pragma unroll DP > 96 ? 1 : SUB
       for (int u = 0; u < SUB; ++u) {
         f32x16 s, dp;
 #pragma unroll
@@ -510,9 +620,11 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_backward_q_kernel(Att
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = exp2_of(fmaf(s[i], c, -shift)) * dp[i];
         if (k0 + u * 32 + 31 > mine) {
+          // a sequence's first row has one key and a constant softmax: its dS is 0, not the rounding of dp - delta
+          const int last = row == 0 ? -1 : row;
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (k0 + u * 32 + 8 * (i / 4) + 4 * half + i % 4 > row) s[i] = 0.f;
+            if (k0 + u * 32 + 8 * (i / 4) + 4 * half + i % 4 > last) s[i] = 0.f;
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -523,31 +635,36 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_backward_q_kernel(Att
         }
       }
     }
+    if constexpr (W::BUFFERS == 1) __syncthreads();
     if (more) {
-      sk.store(lds[(t + 1) & 1][0]);
-      sv.store(lds[(t + 1) & 1][1]);
+      char* next = lds + (W::BUFFERS == 2 ? ((t + 1) & 1) * 2 * W::BYTES : 0);
+      sk.store(next);
+      sv.store(next + W::BYTES);
     }
   }
+  join_waves<W, DT>(dq, lds, part, lane);
+  if (part > 0) return;
   T* out = attn_row<T>(A.dq, it, qh, row);
   store_rows<T, DP>(out, nullptr, dq, A.scale * over_sum * exp2_of(-lift), in, A.D, lane);
   if (!in && row < it.limit) zero_row<T, DP>(out, A.D, lane);
 }
 
 // ---- backward: keys and values -----------------------------------------------------------------------------------
-template <typename T, int DP>
-__global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(AttnArgs A) {
+template <typename T, int DP, int RW>
+__global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_KV)) void attention_backward_kv_kernel(AttnArgs A) {
   using M = Attn<T>;
+  using W = Work<T, DP, RW>;
   constexpr bool HALF = std::is_same<T, f16_t>::value;
-  constexpr int BQ = attn_block_keys<T>(), KS = DP / (2 * M::EPL), SUB = BQ / 32, G = 32 / M::GROUP, DT = DP / 32;
-  constexpr int BYTES = BQ * Tile<T, DP>::PITCH;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][BYTES];
+  constexpr int BQ = W::STEP, KS = DP / (2 * M::EPL), SUB = W::SUB, G = 32 / M::GROUP, DT = DP / 32;
+  __shared__ __attribute__((aligned(16))) char lds[W::LDS];
   constexpr int NSTAT = std::is_same<T, bf16_t>::value ? 2 : 3;
-  __shared__ __attribute__((aligned(16))) float stats[2][NSTAT][BQ];
+  __shared__ __attribute__((aligned(16))) float stats[W::BUFFERS][NSTAT][BQ];
   AttnItem it;
   int kvh, qh0;
-  if (!attn_item(A, true, it, kvh, qh0)) return;
+  if (!attn_item<W::ROWS>(A, true, it, kvh, qh0)) return;
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
-  const int first = it.tile * AT_TILE, mine = first + wave * 32, row = mine + (lane & 31), half = lane >> 5;
+  const int part = wave / RW;  // which of the waves that share rows
+  const int first = it.tile * W::ROWS, mine = first + (wave % RW) * 32, row = mine + (lane & 31), half = lane >> 5;
   if (first >= it.len) {
     if (row < it.limit) {
       zero_row<T, DP>(attn_row<T>(A.dk, it, kvh, row), A.D, lane);
@@ -557,8 +674,9 @@ __global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(At
   }
   const bool in = row < it.len;
   uint4 kf[KS], vf[KS];
-  load_own<T, DP>(attn_rows<T>(A.k, it, kvh), A.k.tok, row, in, A.D, lane, kf);
-  load_own<T, DP>(attn_rows<T>(A.v, it, kvh), A.v.tok, row, in, A.D, lane, vf);
+  const int own = row - first, left = it.len - first;
+  load_own<T, DP>(attn_rows<T>(A.k, it, kvh) + first * A.k.tok, A.k.tok, own, left, A.D, lane, kf);
+  load_own<T, DP>(attn_rows<T>(A.v, it, kvh) + first * A.v.tok, A.v.tok, own, left, A.D, lane, vf);
   f32x16 dk[DT], dv[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -567,53 +685,60 @@ __global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(At
   const float c = A.scale * AT_LOG2E;
   const int t0 = first / BQ, per_head = (it.len + BQ - 1) / BQ - t0, n_tiles = per_head * A.group;
   Staged<T, DP, BQ> sq, sg;
-  float stage[NSTAT];
-#pragma unroll
-  for (int i = 0; i < NSTAT; ++i) stage[i] = 0.f;
-  auto load = [&](int t) {
-    const int qh = qh0 + t / per_head, q0 = (t0 + t % per_head) * BQ;
-    sq.load(attn_rows<T>(A.q, it, qh), A.q.tok, q0, it.len, A.D);
-    sg.load(attn_rows<T>(A.grad_o, it, qh), A.grad_o.tok, q0, it.len, A.D);
-    if (threadIdx.x < BQ) {
-      const bool ok = q0 + (int)threadIdx.x < it.len;
-      const int64_t stat = (int64_t)qh * A.rows + it.stat + q0 + threadIdx.x;
-      const float sum = ok ? A.sum[stat] : 1.f;
-      stage[0] = ok ? A.shift[stat] : 0.f;
-      // at 16 bits the sum joins the exponent (its rounding there is far below that of the weights); in fp32 it does not
-      if constexpr (sizeof(T) == 2)
-        stage[0] += log2f(sum);
-      else
-        stage[2] = 1.0f / sum;
-      stage[1] = ok ? A.delta[stat] : 0.f;
-      if constexpr (HALF) stage[2] = ok ? A.peak[stat] : 0.f;
+  float stage[4];
+  // tile t is tile t % per_head of the queries, for query head t / per_head of the group
+  int load_head = qh0, load_tile = t0;
+  auto load = [&]() {
+    const int q0 = load_tile * BQ, rows = it.len - q0;
+    sq.load(attn_rows<T>(A.q, it, load_head) + q0 * A.q.tok, A.q.tok, rows, A.D);
+    sg.load(attn_rows<T>(A.grad_o, it, load_head) + q0 * A.grad_o.tok, A.grad_o.tok, rows, A.D);
+    const int64_t stat = (int64_t)load_head * A.rows + it.stat + q0;
+    const uint32_t mine4 = threadIdx.x < BQ ? threadIdx.x * 4 : NO_ROW;
+    const int n = min(rows, BQ);
+    stage[0] = buffer_load4(row_buffer(A.shift + stat, 1, n, 1), mine4);
+    stage[1] = buffer_load4(row_buffer(A.delta + stat, 1, n, 1), mine4);
+    stage[2] = buffer_load4(row_buffer(A.sum + stat, 1, n, 1), mine4);
+    if constexpr (HALF) stage[3] = buffer_load4(row_buffer(A.peak + stat, 1, n, 1), mine4);
+    if (++load_tile == t0 + per_head) {
+      load_tile = t0;
+      ++load_head;
     }
   };
   auto store = [&](int b) {
-    sq.store(lds[b][0]);
-    sg.store(lds[b][1]);
+    sq.store(lds + b * 2 * W::BYTES);
+    sg.store(lds + b * 2 * W::BYTES + W::BYTES);
     if (threadIdx.x < BQ) {
-#pragma unroll
-      for (int i = 0; i < NSTAT; ++i) stats[b][i][threadIdx.x] = stage[i];
+      const float sum = stage[2] == 0.f ? 1.f : stage[2];  // rows past the end read as zeros
+      // at 16 bits the sum joins the exponent (its rounding there is far below that of the weights); in fp32 it does not
+      stats[b][0][threadIdx.x] = sizeof(T) == 2 ? stage[0] + log2f(sum) : stage[0];
+      stats[b][1][threadIdx.x] = stage[1];
+      if constexpr (HALF) stats[b][2][threadIdx.x] = stage[3];
+      if constexpr (sizeof(T) == 4) stats[b][2][threadIdx.x] = 1.0f / sum;
     }
   };
   // fp16: dS carries a power of two that keeps it out of the subnormals, the one that fits the largest |do| seen so
   // far; when a tile brings a larger one, what has been summed is rescaled (exactly) to the new power.
   int lift = 0;
   bool lifted = false;
-  load(0);
+  sq.init(A.q.tok, A.D);
+  sg.init(A.grad_o.tok, A.D);
+  load();
   store(0);
+  int tile = t0;
   for (int t = 0; t < n_tiles; ++t) {
     __syncthreads();
     const bool more = t + 1 < n_tiles;
-    if (more) load(t + 1);
-    const char* tq = lds[t & 1][0];
-    const char* tg = lds[t & 1][1];
-    const float(*st)[BQ] = stats[t & 1];
-    const int q0 = (t0 + t % per_head) * BQ;
-    if (q0 + BQ > mine && mine < it.len) {
+    if (more) load();
+    const int b = W::BUFFERS == 2 ? t & 1 : 0, skip = part * (SUB * 32);
+    const char* tq = lds + b * 2 * W::BYTES + skip * Tile<T, DP>::PITCH;
+    const char* tg = tq + W::BYTES;
+    const float(*st)[BQ] = stats[b];
+    const int q0 = tile * BQ + skip;
+    if (++tile == t0 + per_head) tile = t0;
+    if (q0 + SUB * 32 > mine && mine < it.len) {
       float raise = 1.f;
       if constexpr (HALF) {
-        const float peak = wave_max(st[2][lane % BQ]);
+        const float peak = wave_max(st[2][skip + lane % (SUB * 32)]);
         if (peak > 0.f && peak < INFINITY) {
           const int want = -ilogbf(peak);
           if (!lifted || want < lift) {
@@ -630,19 +755,19 @@ __global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(At
         }
         raise = exp2_of((float)lift);
       }
-#pragma unroll
+#pragma unroll 1
       for (int u = 0; u < SUB; ++u) {
         if (q0 + u * 32 + 31 < mine) continue;  // all of these queries come before this wave's keys
         f32x16 s, dp;
         float lse[16], over_sum[sizeof(T) == 4 ? 16 : 1];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          const float4 a = *reinterpret_cast<const float4*>(&st[0][u * 32 + 8 * b + 4 * half]);
-          const float4 d = *reinterpret_cast<const float4*>(&st[1][u * 32 + 8 * b + 4 * half]);
+          const float4 a = *reinterpret_cast<const float4*>(&st[0][skip + u * 32 + 8 * b + 4 * half]);
+          const float4 d = *reinterpret_cast<const float4*>(&st[1][skip + u * 32 + 8 * b + 4 * half]);
           lse[4 * b] = a.x, lse[4 * b + 1] = a.y, lse[4 * b + 2] = a.z, lse[4 * b + 3] = a.w;
           dp[4 * b] = -d.x, dp[4 * b + 1] = -d.y, dp[4 * b + 2] = -d.z, dp[4 * b + 3] = -d.w;
           if constexpr (sizeof(T) == 4) {
-            const float4 w = *reinterpret_cast<const float4*>(&st[2][u * 32 + 8 * b + 4 * half]);
+            const float4 w = *reinterpret_cast<const float4*>(&st[2][skip + u * 32 + 8 * b + 4 * half]);
             over_sum[4 * b] = w.x, over_sum[4 * b + 1] = w.y, over_sum[4 * b + 2] = w.z, over_sum[4 * b + 3] = w.w;
           }
         }
@@ -661,8 +786,11 @@ __global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(At
         }
         if (q0 + u * 32 < mine + 31) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (q0 + u * 32 + 8 * (i / 4) + 4 * half + i % 4 < row) s[i] = dp[i] = 0.f;
+          for (int i = 0; i < 16; ++i) {
+            const int query = q0 + u * 32 + 8 * (i / 4) + 4 * half + i % 4;
+            if (query < row) s[i] = dp[i] = 0.f;
+            if (query == 0) dp[i] = 0.f;  // one key, a constant softmax: dS is 0, not the rounding of dp - delta
+          }
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -675,8 +803,20 @@ __global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(At
         }
       }
     }
-    if (more) store((t + 1) & 1);
+    if constexpr (W::BUFFERS == 1) __syncthreads();
+    if (more) store(W::BUFFERS == 2 ? (t + 1) & 1 : 0);
   }
+  if constexpr (HALF && W::SPLIT > 1) {  // the waves' powers of two may differ
+    const float f = exp2_of(-(float)lift);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dk[dt][i] *= f;
+    lift = 0;
+  }
+  join_waves<W, DT>(dk, lds, part, lane);
+  join_waves<W, DT>(dv, lds, part, lane);
+  if (part > 0) return;
   T* out_k = attn_row<T>(A.dk, it, kvh, row);
   T* out_v = attn_row<T>(A.dv, it, kvh, row);
   store_rows<T, DP>(out_k, nullptr, dk, A.scale * exp2_of(-(float)lift), in, A.D, lane);
@@ -688,75 +828,82 @@ __global__ __launch_bounds__(AT_THREADS, 1) void attention_backward_kv_kernel(At
 }
 
 // ---- packed sequences: the list of tiles -------------------------------------------------------------------------
-// One entry per AT_TILE rows of a sequence, entries of a higher tile (more keys to walk) first, and entries that only
-// clear the rows outside every sequence.  The sequences' ends are device data: they are clamped to the packed rows and
-// to each other, and an entry that would not fit in the list is dropped, so that no offsets lead out of bounds.
-constexpr int PLAN_LEVELS = 4096;
+// One entry per tile of a sequence, entries of a higher tile (more of the other side to walk) first, and entries that
+// only clear the rows outside every sequence; one list per tile height, each made by one workgroup.  The sequences'
+// ends are device data: they are clamped to the packed rows and to each other, and an entry that would not fit in the
+// list is dropped, so that no boundaries lead out of bounds.
+constexpr int PLAN_THREADS = 1024;
 
 __device__ inline int2 plan_sequence(const int32_t* cu, int n, int rows) {
   const int a = min(max(cu[n], 0), rows), b = min(max(cu[n + 1], a), rows);
   return make_int2(a, b - a);
 }
 
-__global__ __launch_bounds__(1024) void attention_plan_kernel(const int32_t* __restrict__ cu, int N, int rows,
-                                                              int4* table, int entries) {
-  __shared__ int level[PLAN_LEVELS];  // sequences with exactly that many tiles; then: entries before the level's first
-  __shared__ int carry[1024];
-  const int most = (rows + AT_TILE - 1) / AT_TILE;
-  int fold = 0;  // levels are grouped by 2^fold tiles when there are more than PLAN_LEVELS
-  while ((most >> fold) >= PLAN_LEVELS) ++fold;
-  for (int i = threadIdx.x; i < PLAN_LEVELS; i += 1024) level[i] = 0;
-  for (int i = threadIdx.x; i < entries; i += 1024) table[i] = make_int4(0, 0, 0, 0);
-  __syncthreads();
-  // tiles per level: a sequence of n tiles has one tile at each of 0 .. n - 1
-  for (int n = threadIdx.x; n < N; n += 1024) {
-    const int tiles = (plan_sequence(cu, n, rows).y + AT_TILE - 1) / AT_TILE;
-    for (int t = 0; t < tiles; t += 1 << fold) atomicAdd(&level[t >> fold], min(1 << fold, tiles - t));
+// sum of v over the threads from this one on
+__device__ inline int suffix_sum(int v, int* waves) {
+  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+#pragma unroll
+  for (int d = 1; d < WAVE; d <<= 1) {
+    const int up = __shfl_down(v, d, WAVE);
+    if (lane + d < WAVE) v += up;
   }
   __syncthreads();
-  // entries before each level, the highest first: thread i sums a run of levels from the top
-  constexpr int RUN = PLAN_LEVELS / 1024;
-  int sum = 0;
-  for (int j = 0; j < RUN; ++j) sum += level[PLAN_LEVELS - 1 - (threadIdx.x * RUN + j)];
-  carry[threadIdx.x] = sum;
+  if (lane == 0) waves[wave] = v;
   __syncthreads();
-  for (int d = 1; d < 1024; d <<= 1) {
-    const int add = threadIdx.x >= d ? carry[threadIdx.x - d] : 0;
-    __syncthreads();
-    carry[threadIdx.x] += add;
-    __syncthreads();
+  for (int w = wave + 1; w < PLAN_THREADS / WAVE; ++w) v += waves[w];
+  return v;
+}
+
+__global__ __launch_bounds__(PLAN_THREADS) void attention_plan_kernel(const int32_t* __restrict__ cu, int N, int rows,
+                                                                      int4* tables, int entries0, int entries1) {
+  // a level is a tile's index, or 2^fold of them where there are more levels than threads
+  __shared__ int whole[PLAN_THREADS], partial[PLAN_THREADS], cursor[PLAN_THREADS], waves[PLAN_THREADS / WAVE];
+  __shared__ int total;
+  const int height = AT_TILES[blockIdx.x], entries = blockIdx.x == 0 ? entries0 : entries1;
+  int4* table = tables + (blockIdx.x == 0 ? 0 : entries0);
+  auto tiles_of = [&](int length) { return (length + height - 1) / height; };
+  int fold = 0;
+  while ((tiles_of(rows) >> fold) >= PLAN_THREADS) ++fold;
+  whole[threadIdx.x] = partial[threadIdx.x] = 0;
+  __syncthreads();
+  for (int n = threadIdx.x; n < N; n += PLAN_THREADS) {
+    const int tiles = tiles_of(plan_sequence(cu, n, rows).y);
+    if (tiles > 0) {
+      atomicAdd(&whole[tiles >> fold], 1);  // levels below this one it fills, this one in part
+      if (fold > 0) atomicAdd(&partial[tiles >> fold], tiles & ((1 << fold) - 1));
+    }
   }
-  int before = threadIdx.x > 0 ? carry[threadIdx.x - 1] : 0;
-  const int total = carry[1023];
-  for (int j = 0; j < RUN; ++j) {
-    const int l = PLAN_LEVELS - 1 - (threadIdx.x * RUN + j), here = level[l];
-    level[l] = before;
-    before += here;
-  }
+  __syncthreads();
+  // tiles of a level: 2^fold of every sequence that reaches past it, and what ends in it
+  const int reach = suffix_sum(whole[threadIdx.x], waves) - whole[threadIdx.x];
+  const int here = (reach << fold) + partial[threadIdx.x];
+  const int from_here = suffix_sum(here, waves);
+  cursor[threadIdx.x] = from_here - here;
+  if (threadIdx.x == 0) total = from_here;
   __syncthreads();
   // within a level the order is whatever the counters hand out: it decides when a tile runs, not what it computes
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
-  for (int n = wave; n < N; n += 1024 / WAVE) {
+  for (int n = wave; n < N; n += PLAN_THREADS / WAVE) {
     const int2 s = plan_sequence(cu, n, rows);
-    const int tiles = (s.y + AT_TILE - 1) / AT_TILE;
-    for (int t = lane; t < tiles; t += WAVE) {
-      const int at = atomicAdd(&level[t >> fold], 1);
+    for (int t = lane; t < tiles_of(s.y); t += WAVE) {
+      const int at = atomicAdd(&cursor[t >> fold], 1);
       if ((unsigned)at < (unsigned)entries) table[at] = make_int4(s.x, s.y, t, s.y);
     }
   }
-  // rows before the first and after the last sequence
+  // rows before the first and after the last sequence, then entries without work
   const int head = N > 0 ? plan_sequence(cu, 0, rows).x : 0;
   const int2 last = N > 0 ? plan_sequence(cu, N - 1, rows) : make_int2(0, 0);
-  const int tail = last.x + last.y, head_tiles = (head + AT_TILE - 1) / AT_TILE;
-  const int tail_tiles = (rows - tail + AT_TILE - 1) / AT_TILE;
-  for (int i = threadIdx.x; i < head_tiles + tail_tiles; i += 1024) {
-    const int at = total + i;
-    if ((unsigned)at >= (unsigned)entries) break;
-    table[at] = i < head_tiles ? make_int4(0, 0, i, head) : make_int4(tail, 0, i - head_tiles, rows - tail);
+  const int tail = last.x + last.y, head_tiles = tiles_of(head), clear = head_tiles + tiles_of(rows - tail);
+  for (int at = total + (int)threadIdx.x; at < entries; at += PLAN_THREADS) {
+    if (at < 0) break;
+    const int i = at - total;
+    table[at] = i >= clear       ? make_int4(0, 0, 0, 0)
+                : i < head_tiles ? make_int4(0, 0, i, head)
+                                 : make_int4(tail, 0, i - head_tiles, rows - tail);
   }
 }
 
-int64_t attention_plan_entries(int64_t rows, int N) { return rows / AT_TILE + N + 2; }
+static int64_t plan_entries(int64_t rows, int n_seqs, int which) { return rows / AT_TILES[which] + n_seqs + 2; }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 static int attn_check(const bgx_attention_shape* a, const char* what) {
@@ -767,35 +914,55 @@ static int attn_check(const bgx_attention_shape* a, const char* what) {
   BGX_REQUIRE(a->head_dim >= 1 && a->head_dim <= AT_MAX_D, BGX_E_SHAPE, "%s: head_dim=%d, supported are 1 to %d", what,
               a->head_dim, AT_MAX_D);
   BGX_REQUIRE(a->dtype >= BGX_F32 && a->dtype <= BGX_BF16, BGX_E_DTYPE, "%s: dtype %d", what, a->dtype);
+  BGX_REQUIRE(a->head_dim % (16 / (int)dtype_size(a->dtype)) == 0, BGX_E_SHAPE,
+              "%s: head_dim=%d is not whole 16-byte pieces; pad it with zeros", what, a->head_dim);
   BGX_REQUIRE(a->scale > 0.f && a->scale < INFINITY, BGX_E_ARG, "%s: scale %g must be positive and finite", what, a->scale);
   // tile bounds are formed in 32 bits
-  BGX_REQUIRE(a->rows < (1ll << 31) - 4 * AT_TILE, BGX_E_SHAPE, "%s: %lld rows", what, (long long)a->rows);
+  BGX_REQUIRE(a->rows < (1ll << 31) - 4 * AT_TILES[0], BGX_E_SHAPE, "%s: %lld rows", what, (long long)a->rows);
   if (a->plan_dev == nullptr)
     BGX_REQUIRE(a->n_seqs == 0 ? a->rows == 0 : a->rows % a->n_seqs == 0, BGX_E_ARG,
                 "%s: %lld rows are not %d sequences of one width", what, (long long)a->rows, a->n_seqs);
   return 0;
 }
 
-static int64_t attn_items(const bgx_attention_shape* a) {
-  if (a->plan_dev != nullptr) return attention_plan_entries(a->rows, a->n_seqs);
+// tiles of the given height, over all sequences
+static int64_t attn_items(const bgx_attention_shape* a, int which) {
+  if (a->plan_dev != nullptr) return plan_entries(a->rows, a->n_seqs, which);
   const int64_t S = a->n_seqs ? a->rows / a->n_seqs : 0;
-  return (S + AT_TILE - 1) / AT_TILE * a->n_seqs;
+  return (S + AT_TILES[which] - 1) / AT_TILES[which] * a->n_seqs;
 }
 
 static AttnArgs attn_args(const bgx_attention_shape* a) {
   AttnArgs A{};
-  A.table = (const int4*)a->plan_dev;
   A.lengths = a->lengths_dev;
   A.rows = a->rows;
   A.N = a->n_seqs;
   A.S = a->plan_dev == nullptr && a->n_seqs ? (int)(a->rows / a->n_seqs) : 0;
-  A.tiles = (A.S + AT_TILE - 1) / AT_TILE;
   A.Hq = a->heads;
   A.Hk = a->kv_heads;
   A.group = a->heads / a->kv_heads;
   A.D = a->head_dim;
   A.scale = a->scale;
   return A;
+}
+
+// Which tile height a launch over `heads` heads takes, and its number of workgroups (0: too many).
+static unsigned attn_grid(AttnArgs& A, const bgx_attention_shape* a, int heads, int* which) {
+  *which = attn_items(a, 0) * heads < AT_FEW ? 1 : 0;
+  const int64_t grid = attn_items(a, *which) * heads;
+  if (a->plan_dev != nullptr)
+    A.table = (const int4*)a->plan_dev + (*which ? plan_entries(a->rows, a->n_seqs, 0) : 0);
+  A.tiles = (A.S + AT_TILES[*which] - 1) / AT_TILES[*which];
+  return grid < (1ll << 31) ? (unsigned)grid : 0;
+}
+
+// offsets within a tile are 32-bit
+static int attn_check_rows(const bgx_attention_rows* t, int head_dim, int dtype, const char* what) {
+  BGX_REQUIRE(t != nullptr && t->data != nullptr, BGX_E_ARG, "%s: null operand", what);
+  BGX_REQUIRE(t->tok_stride >= head_dim && t->tok_stride * (int64_t)dtype_size(dtype) <= (1 << 23), BGX_E_SHAPE,
+              "%s: %lld elements between positions, supported are head_dim=%d up to 8 MiB", what,
+              (long long)t->tok_stride, head_dim);
+  return 0;
 }
 
 static AttnView attn_view(const bgx_attention_rows* t) {
@@ -809,42 +976,50 @@ static AttnView attn_view(const bgx_attention_rows* t) {
   return v;
 }
 
-#define BGX_ATTN_WIDTHS(KERNEL, T, D, GRID, S, A)            \
-  do {                                                       \
-    if ((D) <= 32)                                           \
-      KERNEL<T, 32><<<(GRID), AT_THREADS, 0, (S)>>>(A);      \
-    else if ((D) <= 64)                                      \
-      KERNEL<T, 64><<<(GRID), AT_THREADS, 0, (S)>>>(A);      \
-    else if ((D) <= 96)                                      \
-      KERNEL<T, 96><<<(GRID), AT_THREADS, 0, (S)>>>(A);      \
-    else                                                     \
-      KERNEL<T, 128><<<(GRID), AT_THREADS, 0, (S)>>>(A);     \
+#define BGX_ATTN_ROWS(KERNEL, T, DP, WHICH, GRID, S, A)       \
+  do {                                                        \
+    if ((WHICH) == 0)                                         \
+      KERNEL<T, DP, 4><<<(GRID), AT_THREADS, 0, (S)>>>(A);    \
+    else                                                      \
+      KERNEL<T, DP, 1><<<(GRID), AT_THREADS, 0, (S)>>>(A);    \
   } while (0)
-#define BGX_ATTN_LAUNCH(KERNEL, DTYPE, D, GRID, S, A)        \
-  do {                                                       \
-    if ((DTYPE) == BGX_F32)                                  \
-      BGX_ATTN_WIDTHS(KERNEL, float, D, GRID, S, A);         \
-    else if ((DTYPE) == BGX_F16)                             \
-      BGX_ATTN_WIDTHS(KERNEL, f16_t, D, GRID, S, A);         \
-    else                                                     \
-      BGX_ATTN_WIDTHS(KERNEL, bf16_t, D, GRID, S, A);        \
-    BGX_HIP(hipGetLastError());                              \
+#define BGX_ATTN_WIDTHS(KERNEL, T, D, WHICH, GRID, S, A)      \
+  do {                                                        \
+    if ((D) <= 32)                                            \
+      BGX_ATTN_ROWS(KERNEL, T, 32, WHICH, GRID, S, A);        \
+    else if ((D) <= 64)                                       \
+      BGX_ATTN_ROWS(KERNEL, T, 64, WHICH, GRID, S, A);        \
+    else if ((D) <= 96)                                       \
+      BGX_ATTN_ROWS(KERNEL, T, 96, WHICH, GRID, S, A);        \
+    else                                                      \
+      BGX_ATTN_ROWS(KERNEL, T, 128, WHICH, GRID, S, A);       \
+  } while (0)
+#define BGX_ATTN_LAUNCH(KERNEL, DTYPE, D, WHICH, GRID, S, A)  \
+  do {                                                        \
+    if ((DTYPE) == BGX_F32)                                   \
+      BGX_ATTN_WIDTHS(KERNEL, float, D, WHICH, GRID, S, A);   \
+    else if ((DTYPE) == BGX_F16)                              \
+      BGX_ATTN_WIDTHS(KERNEL, f16_t, D, WHICH, GRID, S, A);   \
+    else                                                      \
+      BGX_ATTN_WIDTHS(KERNEL, bf16_t, D, WHICH, GRID, S, A);  \
+    BGX_HIP(hipGetLastError());                               \
   } while (0)
 
 size_t attention_plan_bytes(int64_t rows, int n_seqs) {
   if (rows < 0 || n_seqs < 0) return 0;
-  return (size_t)attention_plan_entries(rows, n_seqs) * sizeof(int4);
+  return (size_t)(plan_entries(rows, n_seqs, 0) + plan_entries(rows, n_seqs, 1)) * sizeof(int4);
 }
 
 int attention_plan_impl(const int32_t* cu, int n_seqs, int64_t rows, void* plan, size_t plan_bytes, void* stream) {
-  BGX_REQUIRE(n_seqs >= 0 && rows >= 0 && rows < (1ll << 31) - 4 * AT_TILE, BGX_E_ARG, "attention plan: n_seqs=%d rows=%lld",
+  BGX_REQUIRE(n_seqs >= 0 && rows >= 0 && rows < (1ll << 31) - 4 * AT_TILES[0], BGX_E_ARG, "attention plan: n_seqs=%d rows=%lld",
               n_seqs, (long long)rows);
   BGX_REQUIRE(cu != nullptr || n_seqs == 0, BGX_E_ARG, "attention plan: null cu_seqlens");
-  const int64_t entries = attention_plan_entries(rows, n_seqs);
-  BGX_REQUIRE(entries < (1ll << 31), BGX_E_SHAPE, "attention plan: %lld entries", (long long)entries);
+  const int64_t tall = plan_entries(rows, n_seqs, 0), flat = plan_entries(rows, n_seqs, 1);
+  BGX_REQUIRE(flat < (1ll << 31), BGX_E_SHAPE, "attention plan: %lld entries", (long long)flat);
   BGX_REQUIRE(plan != nullptr && plan_bytes >= attention_plan_bytes(rows, n_seqs), BGX_E_WORKSPACE,
               "attention plan: %zu bytes, %zu needed", plan_bytes, attention_plan_bytes(rows, n_seqs));
-  attention_plan_kernel<<<1, 1024, 0, (hipStream_t)stream>>>(cu, n_seqs, (int)rows, (int4*)plan, (int)entries);
+  attention_plan_kernel<<<2, PLAN_THREADS, 0, (hipStream_t)stream>>>(cu, n_seqs, (int)rows, (int4*)plan, (int)tall,
+                                                                    (int)flat);
   BGX_HIP(hipGetLastError());
   return 0;
 }
@@ -867,16 +1042,18 @@ int attention_forward_impl(const bgx_attention_shape* a, const bgx_attention_row
                            const bgx_attention_rows* v, const bgx_attention_rows* o, void* saved, void* stream) {
   if (int rc = attn_check(a, "attention")) return rc;
   if (a->rows == 0) return 0;
-  BGX_REQUIRE(q && k && v && o && q->data && k->data && v->data && o->data, BGX_E_ARG, "attention: null operand");
+  for (const bgx_attention_rows* t : {q, k, v, o})
+    if (int rc = attn_check_rows(t, a->head_dim, a->dtype, "attention")) return rc;
   AttnArgs A = attn_args(a);
   A.q = attn_view(q);
   A.k = attn_view(k);
   A.v = attn_view(v);
   A.o = attn_view(o);
   attn_saved(A, a, saved);
-  const int64_t grid = attn_items(a) * a->heads;
-  BGX_REQUIRE(grid < (1ll << 31), BGX_E_SHAPE, "attention: %lld workgroups", (long long)grid);
-  BGX_ATTN_LAUNCH(attention_forward_kernel, a->dtype, a->head_dim, dim3((unsigned)grid), (hipStream_t)stream, A);
+  int which;
+  const unsigned grid = attn_grid(A, a, a->heads, &which);
+  BGX_REQUIRE(grid > 0, BGX_E_SHAPE, "attention: %lld rows of %d heads", (long long)a->rows, a->heads);
+  BGX_ATTN_LAUNCH(attention_forward_kernel, a->dtype, a->head_dim, which, grid, (hipStream_t)stream, A);
   return 0;
 }
 
@@ -891,9 +1068,8 @@ int attention_backward_impl(const bgx_attention_shape* a, const bgx_attention_ro
                             const bgx_attention_rows* dv, void* ws, size_t ws_bytes, void* stream) {
   if (int rc = attn_check(a, "attention backward")) return rc;
   if (a->rows == 0) return 0;
-  const bgx_attention_rows* all[] = {q, k, v, o, grad_o, dq, dk, dv};
-  for (const bgx_attention_rows* t : all)
-    BGX_REQUIRE(t != nullptr && t->data != nullptr, BGX_E_ARG, "attention backward: null operand");
+  for (const bgx_attention_rows* t : {q, k, v, o, grad_o, dq, dk, dv})
+    if (int rc = attn_check_rows(t, a->head_dim, a->dtype, "attention backward")) return rc;
   BGX_REQUIRE(saved != nullptr, BGX_E_ARG, "attention backward: null saved");
   const size_t need = attention_backward_workspace_bytes(a);
   BGX_REQUIRE(ws != nullptr && ws_bytes >= need, BGX_E_WORKSPACE, "attention backward: workspace of %zu bytes, %zu needed",
@@ -910,12 +1086,13 @@ int attention_backward_impl(const bgx_attention_shape* a, const bgx_attention_ro
   attn_saved(A, a, const_cast<void*>(saved));
   A.delta = (float*)ws;
   A.peak = A.delta + a->rows * a->heads;
-  const int64_t items = attn_items(a);
-  BGX_REQUIRE(items * a->heads < (1ll << 31), BGX_E_SHAPE, "attention backward: %lld workgroups",
-              (long long)(items * a->heads));
   hipStream_t s = (hipStream_t)stream;
-  BGX_ATTN_LAUNCH(attention_backward_q_kernel, a->dtype, a->head_dim, dim3((unsigned)(items * a->heads)), s, A);
-  BGX_ATTN_LAUNCH(attention_backward_kv_kernel, a->dtype, a->head_dim, dim3((unsigned)(items * a->kv_heads)), s, A);
+  int which;
+  unsigned grid = attn_grid(A, a, a->heads, &which);
+  BGX_REQUIRE(grid > 0, BGX_E_SHAPE, "attention backward: %lld rows of %d heads", (long long)a->rows, a->heads);
+  BGX_ATTN_LAUNCH(attention_backward_q_kernel, a->dtype, a->head_dim, which, grid, s, A);
+  grid = attn_grid(A, a, a->kv_heads, &which);
+  BGX_ATTN_LAUNCH(attention_backward_kv_kernel, a->dtype, a->head_dim, which, grid, s, A);
   return 0;
 }
 

@@ -161,17 +161,22 @@ Tensor layer_norm(const Tensor& x, const optional<Tensor>& weight_in, const opti
 }
 
 // ---- causal attention -------------------------------------------------------------------------------------------
-Tensor operand(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// elements contiguous, positions ascending, apart, and at most 8 MiB so
+bool direct(const Tensor& t) {
+  const int64_t tok = t.stride(-3), dim = t.size(-1);
+  return (dim == 1 || t.stride(-1) == 1) && (t.size(-3) == 1 || (tok >= dim && tok * t.element_size() <= (1 << 23)));
+}
+Tensor operand(const Tensor& t) { return direct(t) ? t : t.contiguous(); }
 
 bgx_attention_rows rows_of(const Tensor& t) {
-  if (t.dim() == 4) return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
-  return {t.data_ptr(), 0, t.stride(0), t.stride(1)};
+  const int64_t tok = t.size(-3) == 1 ? t.size(-1) : t.stride(-3);  // the stride of a single position means nothing
+  return {t.data_ptr(), t.dim() == 4 ? t.stride(0) : 0, tok, t.stride(-2)};
 }
 
 // a gradient's buffer in the layout of its input, where that has every element once
 Tensor gradient_like(const Tensor& t) {
   Tensor g = at::empty_like(t);
-  return g.size(-1) == 1 || g.stride(-1) == 1 ? g : at::empty(t.sizes(), t.options());
+  return direct(g) ? g : at::empty(t.sizes(), t.options());
 }
 
 bgx_attention_shape shape_of(const Tensor& q, const Tensor& k, const Tensor& plan, const Tensor& lengths, int64_t n_seqs,
@@ -284,6 +289,12 @@ Tensor causal_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   // nothing to attend to: a plain zero of the inputs, which keeps their graph
   if (q.numel() == 0) return (q.sum() + k.sum() + v.sum()) * at::zeros(q.sizes(), q.options());
   const c10::DeviceGuard guard(q.device());
+  // heads of a ragged width are padded with zeros to whole 16-byte pieces: zeros change no score and no sum
+  const int64_t piece = 16 / q.element_size(), pad = (piece - dim % piece) % piece;
+  if (pad) {
+    auto wide = [&](const Tensor& t) { return at::constant_pad_nd(t, {0, pad}); };
+    return causal_attention(wide(q), wide(k), wide(v), cu_in, lengths_in, scale).narrow(-1, 0, dim).contiguous();
+  }
   if (wants_graph({q, k, v})) return CausalAttention::apply(q, k, v, cu_in, lengths_in, scale);
   return attention_forward(operand(q), operand(k), operand(v), cu, lengths, scale, false).out;
 }

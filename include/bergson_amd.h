@@ -546,8 +546,10 @@ int bgx_layernorm_backward(const void* dy_dev, int64_t dy_row_stride,
  *           `rows` rows
  * Rows that belong to no sequence are not read; their outputs and gradients
  * are zero.  Operands: element strides between sequences (batch layout),
- * positions and heads, the head_dim (1..128) elements contiguous, any element
- * alignment; stride 0 broadcasts an input.  scale must be positive.
+ * positions (head_dim up to 8 MiB) and heads, the head_dim elements contiguous,
+ * any element alignment; a stride of 0 between sequences or heads broadcasts an
+ * input.  head_dim is a multiple of 8
+ * (of 4 in fp32) up to 128.  scale must be positive.
  * saved_dev (bgx_attention_saved_bytes; NULL: forward only) receives what the
  * backward pass needs of the forward pass beside out: the softmax statistics,
  * and for 16-bit types what the rounding of out has cut off. */

@@ -134,13 +134,17 @@ def test_c_abi_refusals():
             setattr(s, name, value)
         return C.byref(s)
 
-    rows = C.byref(_lib.AttentionRows(256, 8, 8, 8))
+    rows = C.byref(_lib.AttentionRows(256, 16, 16, 16))
     fwd = lambda s, q=rows: lib.bgx_attention_forward(s, q, rows, rows, rows, None, None)
     assert fwd(None) == -1 and b"null" in lib.bgx_last_error()
     assert fwd(shape(), None) == -1
     assert fwd(shape(), C.byref(_lib.AttentionRows(None, 0, 0, 0))) == -1
     assert fwd(shape(kv_heads=3)) == -3 and fwd(shape(heads=0)) == -3
     assert fwd(shape(head_dim=129)) == -3 and b"129" in lib.bgx_last_error()
+    assert fwd(shape(head_dim=20)) == -3 and b"16-byte" in lib.bgx_last_error()
+    assert fwd(shape(head_dim=6, dtype=0)) == -3
+    assert fwd(shape(), C.byref(_lib.AttentionRows(256, 8, (1 << 22) + 1, 8))) == -3 and b"8 MiB" in lib.bgx_last_error()
+    assert fwd(shape(), C.byref(_lib.AttentionRows(256, 8, -16, 8))) == -3 and fwd(shape(), C.byref(_lib.AttentionRows(256, 8, 15, 8))) == -3
     assert fwd(shape(dtype=5)) == -2
     assert fwd(shape(scale=0.0)) == -1 and fwd(shape(scale=float("nan"))) == -1
     assert fwd(shape(rows=11)) == -1 and b"one width" in lib.bgx_last_error()
@@ -154,7 +158,7 @@ def test_c_abi_refusals():
     # two statistics per head and row; at 16 bits also what the output's rounding cuts off
     assert lib.bgx_attention_saved_bytes(shape()) == 10 * 4 * (2 * 4 + 16 * 2)
     assert lib.bgx_attention_saved_bytes(shape(dtype=0)) == 10 * 4 * 2 * 4
-    assert lib.bgx_attention_plan_bytes(1000, 3) == (1000 // 128 + 3 + 2) * 16
+    assert lib.bgx_attention_plan_bytes(1000, 3) == (1000 // 128 + 3 + 2 + 1000 // 32 + 3 + 2) * 16
     assert lib.bgx_attention_plan(P, 3, 1000, P, 16, None) == -4
     assert lib.bgx_attention_plan(None, 3, 1000, P, 1 << 20, None) == -1
 

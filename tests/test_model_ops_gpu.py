@@ -282,15 +282,11 @@ def test_attention_plan_of_many_sequences(device):
     ends = [0] + torch.tensor(lengths).cumsum(0).tolist()
     cu = torch.tensor(ends, dtype=torch.int32, device=device)
     out = B.causal_attention(q, k, v, cu_seqlens=cu)
-    width = max(lengths)
-    N = len(lengths)
-    idx = (torch.tensor(ends[:-1])[:, None] + torch.arange(width)).clamp_max(T - 1).to(device)
-    lens = torch.tensor(lengths, dtype=torch.int32, device=device)
-    picked = [B.causal_attention(q[idx[a:a + 200]], k[idx[a:a + 200]], v[idx[a:a + 200]], lengths=lens[a:a + 200])
-              for a in range(0, N, 200)]
-    batch = torch.cat(picked)
-    keep = torch.arange(width, device=device) < lens[:, None]
-    assert torch.equal(out[:ends[-1]], batch[keep]) and (out[ends[-1]:] == 0).all()
+    for a, b in zip(ends, ends[1:]):
+        if b > a:
+            ref = attention_reference(q[a:b], k[a:b], v[a:b], 32 ** -0.5, None, torch.bfloat16)
+            assert_within(out[a:b], *ref["o"], f"rows {a}:{b}")
+    assert (out[ends[-1]:] == 0).all()
 
 
 def test_attention_malformed_boundaries_stay_in_bounds(device):
@@ -532,17 +528,11 @@ def test_differentiable_once(device, which):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
 def test_attention_gradients_that_cancel(device, dtype):
-    """Sequences of one token: the softmax is constant, dq and dk vanish; what is left is the fp32 rounding of
-    dp - delta, two sums of D products in different orders."""
+    """Sequences of one token: the softmax is constant, dq and dk are exactly 0 and dv is the sum over the heads."""
     q, k, v, do = _qkv((40,), 4, 2, 64, dtype, 30, device)
     cu = torch.arange(41, dtype=torch.int32, device=device)
     for t in (q, k, v):
         t.requires_grad_()
     dq, dk, dv = torch.autograd.grad(B.causal_attention(q, k, v, cu_seqlens=cu), (q, k, v), do)
-    vq, kq = (t.detach().repeat_interleave(2, 1).double() for t in (v, k))
-    # o is v exactly in fp32 and held with twice the type's bits: half a step of it squared is the type's share
-    half = torch.finfo(dtype).eps / 2
-    e = (2 * 64 * 2.0 ** -24 + (half * half if dtype != torch.float32 else 2.0 ** -24)) * (do.double() * vq).abs().sum(2)
-    assert (dq.double().abs() <= 0.125 * e[..., None] * kq.abs() * 1.01 + 1e-7).all()
-    bound = 0.125 * (e[..., None] * q.detach().double().abs()).unflatten(1, (2, 2)).sum(2)
-    assert (dk.double().abs() <= bound * 1.01 + 1e-7).all()
+    assert (dq == 0).all() and (dk == 0).all()
+    assert torch.equal(dv, do.float().unflatten(1, (2, 2)).sum(2).to(dtype))
