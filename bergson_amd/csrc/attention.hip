@@ -26,8 +26,9 @@ namespace bgx {
 
 constexpr int AT_WAVES = 4;
 constexpr int AT_THREADS = AT_WAVES * WAVE;
-constexpr int AT_TILES[2] = {128, 32};  // rows a workgroup owns (see Work)
-constexpr int AT_FEW = 512;  // fewer workgroups of 128 rows than this: workgroups of 32 rows
+constexpr int AT_TILES[3] = {128, 64, 32};  // rows a workgroup owns (see Work)
+// workgroups of 128 rows: from AT_MANY on they are taken, from AT_SOME on workgroups of 64 rows, below of 32
+constexpr int AT_MANY = 512, AT_SOME = 128;
 constexpr int AT_MAX_D = 128;
 constexpr float AT_LOG2E = 1.4426950408889634f;
 
@@ -178,9 +179,9 @@ struct Staged {
 
 // ---- how a workgroup's waves divide the work ---------------------------------------------------------------------
 // A workgroup owns 32 * RW rows (queries, or keys in the kernel for dk and dv) and walks the other side in tiles of
-// STEP rows.  RW = 4: every wave owns 32 rows and takes each tile whole.  RW = 1: all four waves share 32 rows, each
-// takes a quarter of every tile, and their sums are joined through LDS at the end -- four times the workgroups with
-// a quarter of the walk each, at four times the traffic to LDS: for calls that would not fill the chip otherwise.
+// STEP rows.  RW = 4: every wave owns 32 rows and takes each tile whole.  RW = 2, 1: two or all four waves share 32
+// rows, each takes its part of every tile, and their sums are joined through LDS at the end -- more workgroups with
+// shorter walks, at twice or four times the traffic to LDS: for calls that would not fill the chip otherwise.
 template <typename T, int DP, int RW>
 struct Work {
   static constexpr int ROWS = 32 * RW, SPLIT = AT_WAVES / RW;
@@ -197,10 +198,9 @@ struct Work {
 
 // Sums of the waves that share rows: the others hand theirs to the first through LDS, which adds them in order.
 template <typename W, int DT>
-__device__ inline void join_waves(f32x16 (&acc)[DT], char* lds, int part, int lane) {
+__device__ inline void join_waves(f32x16 (&acc)[DT], char* lds, int part, int group, int lane) {
   if constexpr (W::SPLIT > 1) {
-    static_assert(W::ROWS == 32, "one group of waves");
-    float4* box = reinterpret_cast<float4*>(lds);
+    float4* box = reinterpret_cast<float4*>(lds) + group * (W::SPLIT - 1) * DT * 4 * WAVE;
     __syncthreads();
     if (part > 0) {
 #pragma unroll
@@ -477,12 +477,12 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_Q)) void attent
   const float2 ls = both_halves(l);
   l = ls.x + ls.y;
   if constexpr (W::SPLIT > 1) {  // bring the waves' sums to the largest maximum of them
-    __shared__ float maxima[W::SPLIT][WAVE], sums[W::SPLIT][WAVE];
-    maxima[part][lane] = m;
+    __shared__ float maxima[AT_WAVES][WAVE], sums[AT_WAVES][WAVE];
+    maxima[wave][lane] = m;
     __syncthreads();
     float top = m;
 #pragma unroll
-    for (int w = 0; w < W::SPLIT; ++w) top = fmaxf(top, maxima[w][lane]);
+    for (int w = 0; w < W::SPLIT; ++w) top = fmaxf(top, maxima[w * RW + wave % RW][lane]);
     const float f = m == -INFINITY ? 0.f : exp2_of((m - top) * c);
     m = top;
     l *= f;
@@ -490,11 +490,11 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_Q)) void attent
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[dt][i] *= f;
-    sums[part][lane] = l;
-    join_waves<W, DT>(o, lds, part, lane);
+    sums[wave][lane] = l;
+    join_waves<W, DT>(o, lds, part, wave % RW, lane);
     if (part > 0) return;
 #pragma unroll
-    for (int w = 1; w < W::SPLIT; ++w) l += sums[w][lane];
+    for (int w = 1; w < W::SPLIT; ++w) l += sums[w * RW + wave % RW][lane];
   }
   const bool in = row < it.len;
   T* out = attn_row<T>(A.o, it, qh, row);
@@ -642,7 +642,7 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_Q)) void attent
       sv.store(next + W::BYTES);
     }
   }
-  join_waves<W, DT>(dq, lds, part, lane);
+  join_waves<W, DT>(dq, lds, part, wave % RW, lane);
   if (part > 0) return;
   T* out = attn_row<T>(A.dq, it, qh, row);
   store_rows<T, DP>(out, nullptr, dq, A.scale * over_sum * exp2_of(-lift), in, A.D, lane);
@@ -814,8 +814,8 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_KV)) void atten
       for (int i = 0; i < 16; ++i) dk[dt][i] *= f;
     lift = 0;
   }
-  join_waves<W, DT>(dk, lds, part, lane);
-  join_waves<W, DT>(dv, lds, part, lane);
+  join_waves<W, DT>(dk, lds, part, wave % RW, lane);
+  join_waves<W, DT>(dv, lds, part, wave % RW, lane);
   if (part > 0) return;
   T* out_k = attn_row<T>(A.dk, it, kvh, row);
   T* out_v = attn_row<T>(A.dv, it, kvh, row);
@@ -855,12 +855,13 @@ __device__ inline int suffix_sum(int v, int* waves) {
 }
 
 __global__ __launch_bounds__(PLAN_THREADS) void attention_plan_kernel(const int32_t* __restrict__ cu, int N, int rows,
-                                                                      int4* tables, int entries0, int entries1) {
+                                                                      int4* tables, int entries0, int entries1,
+                                                                      int entries2) {
   // a level is a tile's index, or 2^fold of them where there are more levels than threads
   __shared__ int whole[PLAN_THREADS], partial[PLAN_THREADS], cursor[PLAN_THREADS], waves[PLAN_THREADS / WAVE];
   __shared__ int total;
-  const int height = AT_TILES[blockIdx.x], entries = blockIdx.x == 0 ? entries0 : entries1;
-  int4* table = tables + (blockIdx.x == 0 ? 0 : entries0);
+  const int height = AT_TILES[blockIdx.x], entries = blockIdx.x == 0 ? entries0 : blockIdx.x == 1 ? entries1 : entries2;
+  int4* table = tables + (blockIdx.x == 0 ? 0 : blockIdx.x == 1 ? entries0 : entries0 + entries1);
   auto tiles_of = [&](int length) { return (length + height - 1) / height; };
   int fold = 0;
   while ((tiles_of(rows) >> fold) >= PLAN_THREADS) ++fold;
@@ -948,10 +949,13 @@ static AttnArgs attn_args(const bgx_attention_shape* a) {
 
 // Which tile height a launch over `heads` heads takes, and its number of workgroups (0: too many).
 static unsigned attn_grid(AttnArgs& A, const bgx_attention_shape* a, int heads, int* which) {
-  *which = attn_items(a, 0) * heads < AT_FEW ? 1 : 0;
+  const int64_t tall = attn_items(a, 0) * heads;
+  *which = tall >= AT_MANY ? 0 : tall >= AT_SOME ? 1 : 2;
   const int64_t grid = attn_items(a, *which) * heads;
-  if (a->plan_dev != nullptr)
-    A.table = (const int4*)a->plan_dev + (*which ? plan_entries(a->rows, a->n_seqs, 0) : 0);
+  if (a->plan_dev != nullptr) {
+    A.table = (const int4*)a->plan_dev;
+    for (int i = 0; i < *which; ++i) A.table += plan_entries(a->rows, a->n_seqs, i);
+  }
   A.tiles = (A.S + AT_TILES[*which] - 1) / AT_TILES[*which];
   return grid < (1ll << 31) ? (unsigned)grid : 0;
 }
@@ -980,6 +984,8 @@ static AttnView attn_view(const bgx_attention_rows* t) {
   do {                                                        \
     if ((WHICH) == 0)                                         \
       KERNEL<T, DP, 4><<<(GRID), AT_THREADS, 0, (S)>>>(A);    \
+    else if ((WHICH) == 1)                                    \
+      KERNEL<T, DP, 2><<<(GRID), AT_THREADS, 0, (S)>>>(A);    \
     else                                                      \
       KERNEL<T, DP, 1><<<(GRID), AT_THREADS, 0, (S)>>>(A);    \
   } while (0)
@@ -1007,19 +1013,22 @@ static AttnView attn_view(const bgx_attention_rows* t) {
 
 size_t attention_plan_bytes(int64_t rows, int n_seqs) {
   if (rows < 0 || n_seqs < 0) return 0;
-  return (size_t)(plan_entries(rows, n_seqs, 0) + plan_entries(rows, n_seqs, 1)) * sizeof(int4);
+  size_t entries = 0;
+  for (int i = 0; i < 3; ++i) entries += plan_entries(rows, n_seqs, i);
+  return entries * sizeof(int4);
 }
 
 int attention_plan_impl(const int32_t* cu, int n_seqs, int64_t rows, void* plan, size_t plan_bytes, void* stream) {
   BGX_REQUIRE(n_seqs >= 0 && rows >= 0 && rows < (1ll << 31) - 4 * AT_TILES[0], BGX_E_ARG, "attention plan: n_seqs=%d rows=%lld",
               n_seqs, (long long)rows);
   BGX_REQUIRE(cu != nullptr || n_seqs == 0, BGX_E_ARG, "attention plan: null cu_seqlens");
-  const int64_t tall = plan_entries(rows, n_seqs, 0), flat = plan_entries(rows, n_seqs, 1);
-  BGX_REQUIRE(flat < (1ll << 31), BGX_E_SHAPE, "attention plan: %lld entries", (long long)flat);
+  int64_t n[3], all = 0;
+  for (int i = 0; i < 3; ++i) all += n[i] = plan_entries(rows, n_seqs, i);
+  BGX_REQUIRE(all < (1ll << 31), BGX_E_SHAPE, "attention plan: %lld entries", (long long)all);
   BGX_REQUIRE(plan != nullptr && plan_bytes >= attention_plan_bytes(rows, n_seqs), BGX_E_WORKSPACE,
               "attention plan: %zu bytes, %zu needed", plan_bytes, attention_plan_bytes(rows, n_seqs));
-  attention_plan_kernel<<<2, PLAN_THREADS, 0, (hipStream_t)stream>>>(cu, n_seqs, (int)rows, (int4*)plan, (int)tall,
-                                                                    (int)flat);
+  attention_plan_kernel<<<3, PLAN_THREADS, 0, (hipStream_t)stream>>>(cu, n_seqs, (int)rows, (int4*)plan, (int)n[0],
+                                                                    (int)n[1], (int)n[2]);
   BGX_HIP(hipGetLastError());
   return 0;
 }

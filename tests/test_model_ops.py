@@ -158,7 +158,7 @@ def test_c_abi_refusals():
     # two statistics per head and row; at 16 bits also what the output's rounding cuts off
     assert lib.bgx_attention_saved_bytes(shape()) == 10 * 4 * (2 * 4 + 16 * 2)
     assert lib.bgx_attention_saved_bytes(shape(dtype=0)) == 10 * 4 * 2 * 4
-    assert lib.bgx_attention_plan_bytes(1000, 3) == (1000 // 128 + 3 + 2 + 1000 // 32 + 3 + 2) * 16
+    assert lib.bgx_attention_plan_bytes(1000, 3) == sum(1000 // height + 3 + 2 for height in (128, 64, 32)) * 16
     assert lib.bgx_attention_plan(P, 3, 1000, P, 16, None) == -4
     assert lib.bgx_attention_plan(None, 3, 1000, P, 1 << 20, None) == -1
 
