@@ -151,10 +151,10 @@ __device__ inline float buffer_load4(__amdgpu_buffer_rsrc_t r, uint32_t offset) 
 // current tile's work.  Rows past the end and columns from D on become zeros.  A thread keeps one
 // chunk of columns and takes every RPI-th row: its place in a tile is one 32-bit offset, made once; what changes from
 // tile to tile is a uniform base.
-template <typename T, int DP, int BK>
+template <typename T, int DP, int BK, int THREADS = AT_THREADS>
 struct Staged {
   static constexpr int CH = Tile<T, DP>::PITCH / 16;  // threads per row (with DP = 96 a quarter of them idles)
-  static constexpr int RPI = AT_THREADS / CH, PER = BK / RPI;
+  static constexpr int RPI = THREADS / CH, PER = BK / RPI;
   static_assert(BK % RPI == 0, "whole passes over a tile");
   uint4 v[PER];
   uint32_t offset, pass;
@@ -182,14 +182,14 @@ struct Staged {
 // STEP rows.  RW = 4: every wave owns 32 rows and takes each tile whole.  RW = 2, 1: two or all four waves share 32
 // rows, each takes its part of every tile, and their sums are joined through LDS at the end -- more workgroups with
 // shorter walks, at twice or four times the traffic to LDS: for calls that would not fill the chip otherwise.
-template <typename T, int DP, int RW>
+template <typename T, int DP, int RW, int WAVES = AT_WAVES>
 struct Work {
-  static constexpr int ROWS = 32 * RW, SPLIT = AT_WAVES / RW;
-  static constexpr int SUB = RW == 4 && sizeof(T) == 2 ? 2 : 1;  // blocks of 32 a wave takes of a tile
+  static constexpr int THREADS = WAVES * WAVE, ROWS = 32 * RW, SPLIT = WAVES / RW;
+  static constexpr int SUB = SPLIT == 1 && sizeof(T) == 2 ? 2 : 1;  // blocks of 32 a wave takes of a tile
   static constexpr int STEP = 32 * SUB * SPLIT;
   // waves a SIMD has room for without spilling registers to memory (the compiler's budget: 512 / 2 or 512)
-  static constexpr int WAVES_Q = sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : (RW == 4 || DP <= 64 ? 2 : 1);
-  static constexpr int WAVES_KV = sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : (DP <= 64 ? 2 : 1);
+  static constexpr int PER_SIMD_Q = sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : (RW == 4 || DP <= 64 ? 2 : 1);
+  static constexpr int PER_SIMD_KV = sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : (DP <= 64 || WAVES == 8 ? 2 : 1);
   static constexpr int BYTES = STEP * Tile<T, DP>::PITCH;
   static constexpr int BUFFERS = 4 * BYTES <= 65536 ? 2 : 1;  // two workgroups of a CU fit at 16 bits
   static constexpr int JOIN = (SPLIT - 1) * RW * (DP / 32) * 16 * WAVE * 4;
@@ -369,7 +369,7 @@ __device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ---- forward -----------------------------------------------------------------------------------------------------
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_Q)) void attention_forward_kernel(AttnArgs A) {
+__global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void attention_forward_kernel(AttnArgs A) {
   using M = Attn<T>;
   using W = Work<T, DP, RW>;
   constexpr int BK = W::STEP, KS = DP / (2 * M::EPL), SUB = W::SUB, G = 32 / M::GROUP, DT = DP / 32;
@@ -517,7 +517,7 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_Q)) void attent
 // ---- backward: queries -------------------------------------------------------------------------------------------
 // dq of 32 queries a wave; also leaves delta (and, for fp16, the largest |do| of a row) for the other kernel.
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_Q)) void attention_backward_q_kernel(AttnArgs A) {
+__global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void attention_backward_q_kernel(AttnArgs A) {
   using M = Attn<T>;
   using W = Work<T, DP, RW>;
   constexpr bool HALF = std::is_same<T, f16_t>::value;
@@ -650,13 +650,27 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_Q)) void attent
 }
 
 // ---- backward: keys and values -----------------------------------------------------------------------------------
+// Wide heads at 16 bits with enough keys (RW = 4, DP > 64): dk and dv of 32 keys take half of a wave's registers, and with
+// k, v and a tile on its way in the other half only one wave fits a SIMD, which then waits for every LDS read and every
+// exponential itself (643 TFLOP/s of the four products at 2 x 4096 positions, 32 / 8 heads of 128).  There the
+// workgroup has eight waves, two for the same 32 keys that take the queries of a tile in halves, and k and v are read
+// from LDS as the products need them.
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_KV)) void attention_backward_kv_kernel(AttnArgs A) {
+constexpr int kv_waves() {
+  return RW == 4 && DP > 64 && sizeof(T) == 2 ? 8 : AT_WAVES;
+}
+
+template <typename T, int DP, int RW>
+__global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
+                             (Work<T, DP, RW, kv_waves<T, DP, RW>()>::PER_SIMD_KV)) void attention_backward_kv_kernel(AttnArgs A) {
   using M = Attn<T>;
-  using W = Work<T, DP, RW>;
+  using W = Work<T, DP, RW, kv_waves<T, DP, RW>()>;
+  constexpr bool OWN = W::THREADS > AT_THREADS;  // k and v of the workgroup's keys live in LDS
   constexpr bool HALF = std::is_same<T, f16_t>::value;
   constexpr int BQ = W::STEP, KS = DP / (2 * M::EPL), SUB = W::SUB, G = 32 / M::GROUP, DT = DP / 32;
+  constexpr int KEEP = OWN ? W::ROWS * Tile<T, DP>::PITCH : 0;
   __shared__ __attribute__((aligned(16))) char lds[W::LDS];
+  __shared__ __attribute__((aligned(16))) char keep[OWN ? 2 * KEEP : 16];
   constexpr int NSTAT = std::is_same<T, bf16_t>::value ? 2 : 3;
   __shared__ __attribute__((aligned(16))) float stats[W::BUFFERS][NSTAT][BQ];
   AttnItem it;
@@ -673,10 +687,22 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_KV)) void atten
     return;
   }
   const bool in = row < it.len;
-  uint4 kf[KS], vf[KS];
+  uint4 kf[OWN ? 1 : KS], vf[OWN ? 1 : KS];
   const int own = row - first, left = it.len - first;
-  load_own<T, DP>(attn_rows<T>(A.k, it, kvh) + first * A.k.tok, A.k.tok, own, left, A.D, lane, kf);
-  load_own<T, DP>(attn_rows<T>(A.v, it, kvh) + first * A.v.tok, A.v.tok, own, left, A.D, lane, vf);
+  const T* k = attn_rows<T>(A.k, it, kvh) + first * A.k.tok;
+  const T* v = attn_rows<T>(A.v, it, kvh) + first * A.v.tok;
+  if constexpr (OWN) {
+    Staged<T, DP, W::ROWS, W::THREADS> once;
+    once.init(A.k.tok, A.D);
+    once.load(k, A.k.tok, left, A.D);
+    once.store(keep);
+    once.init(A.v.tok, A.D);
+    once.load(v, A.v.tok, left, A.D);
+    once.store(keep + KEEP);
+  } else {
+    load_own<T, DP>(k, A.k.tok, own, left, A.D, lane, kf);
+    load_own<T, DP>(v, A.v.tok, own, left, A.D, lane, vf);
+  }
   f32x16 dk[DT], dv[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -684,7 +710,7 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_KV)) void atten
     for (int i = 0; i < 16; ++i) dk[dt][i] = dv[dt][i] = 0.f;
   const float c = A.scale * AT_LOG2E;
   const int t0 = first / BQ, per_head = (it.len + BQ - 1) / BQ - t0, n_tiles = per_head * A.group;
-  Staged<T, DP, BQ> sq, sg;
+  Staged<T, DP, BQ, W::THREADS> sq, sg;
   float stage[4];
   // tile t is tile t % per_head of the queries, for query head t / per_head of the group
   int load_head = qh0, load_tile = t0;
@@ -775,8 +801,13 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::WAVES_KV)) void atten
         for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          Mma32<T>::mma(read_rows<T, DP>(tq, u * 32, ks, lane), kf[ks], s);
-          Mma32<T>::mma(read_rows<T, DP>(tg, u * 32, ks, lane), vf[ks], dp);
+          if constexpr (OWN) {
+            Mma32<T>::mma(read_rows<T, DP>(tq, u * 32, ks, lane), read_rows<T, DP>(keep, mine - first, ks, lane), s);
+            Mma32<T>::mma(read_rows<T, DP>(tg, u * 32, ks, lane), read_rows<T, DP>(keep + KEEP, mine - first, ks, lane), dp);
+          } else {
+            Mma32<T>::mma(read_rows<T, DP>(tq, u * 32, ks, lane), kf[ks], s);
+            Mma32<T>::mma(read_rows<T, DP>(tg, u * 32, ks, lane), vf[ks], dp);
+          }
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -951,6 +982,8 @@ static AttnArgs attn_args(const bgx_attention_shape* a) {
 static unsigned attn_grid(AttnArgs& A, const bgx_attention_shape* a, int heads, int* which) {
   const int64_t tall = attn_items(a, 0) * heads;
   *which = tall >= AT_MANY ? 0 : tall >= AT_SOME ? 1 : 2;
+  for (int i = 0; i < 3; ++i)
+    if (switches().attention_rows == AT_TILES[i]) *which = i;
   const int64_t grid = attn_items(a, *which) * heads;
   if (a->plan_dev != nullptr) {
     A.table = (const int4*)a->plan_dev;
@@ -980,14 +1013,27 @@ static AttnView attn_view(const bgx_attention_rows* t) {
   return v;
 }
 
-#define BGX_ATTN_ROWS(KERNEL, T, DP, WHICH, GRID, S, A)       \
-  do {                                                        \
-    if ((WHICH) == 0)                                         \
-      KERNEL<T, DP, 4><<<(GRID), AT_THREADS, 0, (S)>>>(A);    \
-    else if ((WHICH) == 1)                                    \
-      KERNEL<T, DP, 2><<<(GRID), AT_THREADS, 0, (S)>>>(A);    \
-    else                                                      \
-      KERNEL<T, DP, 1><<<(GRID), AT_THREADS, 0, (S)>>>(A);    \
+template <typename T, int DP>
+constexpr int attention_forward_kernel_threads() {
+  return AT_THREADS;
+}
+template <typename T, int DP>
+constexpr int attention_backward_q_kernel_threads() {
+  return AT_THREADS;
+}
+template <typename T, int DP>
+constexpr int attention_backward_kv_kernel_threads() {
+  return kv_waves<T, DP, 4>() * WAVE;
+}
+
+#define BGX_ATTN_ROWS(KERNEL, T, DP, WHICH, GRID, S, A)                    \
+  do {                                                                     \
+    if ((WHICH) == 0)                                                      \
+      KERNEL<T, DP, 4><<<(GRID), KERNEL##_threads<T, DP>(), 0, (S)>>>(A);  \
+    else if ((WHICH) == 1)                                                 \
+      KERNEL<T, DP, 2><<<(GRID), AT_THREADS, 0, (S)>>>(A);                 \
+    else                                                                   \
+      KERNEL<T, DP, 1><<<(GRID), AT_THREADS, 0, (S)>>>(A);                 \
   } while (0)
 #define BGX_ATTN_WIDTHS(KERNEL, T, D, WHICH, GRID, S, A)      \
   do {                                                        \

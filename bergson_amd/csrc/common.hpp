@@ -42,6 +42,7 @@ struct Switches {
   bool scan_stream_off = false;   // BGX_SCAN_STREAM_OFF set
   bool scan_wide_off = false;     // BGX_SCAN_WIDE_OFF set
   bool wgrad_big_off = false;     // BGX_WGRAD_BIG_OFF set: per-sequence weight gradients on 64 x 64 tiles only
+  int attention_rows = 0;         // BGX_ATTENTION_ROWS = 128, 64 or 32: rows per workgroup of the attention kernels, 0 = by size
 };
 const Switches& switches();
 

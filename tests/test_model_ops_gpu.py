@@ -139,11 +139,13 @@ def _check_sequences(q, k, v, do, out, grads, spans, scale, dtype):
         assert (t[~covered] == 0).all()
 
 
+@pytest.mark.parametrize("rows", [128, 64, 32])
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
 @pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (4, 2, 128), (3, 1, 32), (2, 1, 96), (1, 1, 80), (2, 2, 20),
                                                 (1, 1, 7)], ids=str)
 @pytest.mark.parametrize("lengths", [[1], [2, 33], [64, 1, 31, 65], [129, 127, 300]], ids=str)
-def test_attention_packed(device, lengths, heads, kv_heads, dim, dtype):
+def test_attention_packed(device, bgx_env, lengths, heads, kv_heads, dim, dtype, rows):
+    bgx_env("BGX_ATTENTION_ROWS", rows)
     T = sum(lengths)
     q, k, v, do = _qkv((T,), heads, kv_heads, dim, dtype, T + dim, device)
     cu = torch.tensor([0] + lengths).cumsum(0).to(torch.int32).to(device)
@@ -155,11 +157,13 @@ def test_attention_packed(device, lengths, heads, kv_heads, dim, dtype):
     _check_sequences(q, k, v, do, out, grads, list(zip(ends, ends[1:])), dim ** -0.5, dtype)
 
 
+@pytest.mark.parametrize("rows", [128, 64, 32])
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
 @pytest.mark.parametrize("N,S,lengths", [(1, 1, None), (2, 130, None), (3, 200, [200, 0, 77]), (4, 64, [1, 64, 65, -3])],
                          ids=str)
-def test_attention_batch(device, N, S, lengths, dtype):
+def test_attention_batch(device, bgx_env, N, S, lengths, dtype, rows):
     """lengths beyond the width or below zero count as the width and zero."""
+    bgx_env("BGX_ATTENTION_ROWS", rows)
     q, k, v, do = _qkv((N, S), 4, 2, 64, dtype, N * S, device)
     for t in (q, k, v):
         t.requires_grad_()
@@ -170,9 +174,11 @@ def test_attention_batch(device, N, S, lengths, dtype):
     _check_sequences(q, k, v, do, out, grads, spans, 0.21, dtype)
 
 
+@pytest.mark.parametrize("rows", [128, 64, 32])
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
-def test_attention_rows_outside_the_sequences(device, dtype):
+def test_attention_rows_outside_the_sequences(device, bgx_env, dtype, rows):
     """NaN in rows before, after and between nothing reaches the sequences; those rows come out as zeros."""
+    bgx_env("BGX_ATTENTION_ROWS", rows)
     T, cu_list = 400, [40, 100, 100, 260]
     q, k, v, do = _qkv((T,), 2, 1, 64, dtype, 8, device)
     outside = torch.ones(T, dtype=torch.bool, device=device)
@@ -235,9 +241,11 @@ def test_attention_layouts_and_broadcast(device):
     assert torch.equal(got, full.sum(2, keepdim=True))
 
 
+@pytest.mark.parametrize("rows", [128, 64, 32])
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
-def test_attention_far_scores(device, dtype):
+def test_attention_far_scores(device, bgx_env, dtype, rows):
     """Scores hundreds apart, -inf in a key (its weight is 0 wherever it is seen), keys at the type's lowest values."""
+    bgx_env("BGX_ATTENTION_ROWS", rows)
     q, k, v, do = _qkv((140,), 1, 1, 32, dtype, 6, device, gain=6.0)
     cu = torch.tensor([0, 140], dtype=torch.int32, device=device)
     for t in (q, k, v):
@@ -257,8 +265,10 @@ def test_attention_far_scores(device, dtype):
     assert out[:64].isnan().all()     # softmax of nothing but -inf
 
 
-def test_attention_small_gradients_in_fp16(device):
+@pytest.mark.parametrize("rows", [128, 64, 32])
+def test_attention_small_gradients_in_fp16(device, bgx_env, rows):
     """Output gradients near fp16's smallest normal number: dS itself would vanish among the subnormals."""
+    bgx_env("BGX_ATTENTION_ROWS", rows)
     q, k, v, do = _qkv((260,), 2, 1, 64, torch.float16, 12, device)
     do = (do.float() * 2.0 ** -12).half()
     do[:100] *= 2.0 ** -2
@@ -299,6 +309,25 @@ def test_attention_malformed_boundaries_stay_in_bounds(device):
     cu = torch.tensor([0, 300], dtype=torch.int32, device=device)
     torch.cuda.synchronize()
     assert torch.equal(B.causal_attention(q, k, v, cu_seqlens=cu), B.causal_attention(q[None], k[None], v[None])[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("N,heads,kv_heads", [(34, 8, 4), (140, 4, 4)], ids=str)
+def test_attention_sizes_by_rule(device, N, heads, kv_heads, dtype):
+    """Enough sequences and heads that the workgroup sizes follow from the rule: 64 rows in the first case, 128 in the
+    second; heads of 128 and 64."""
+    g = _gen(N)
+    for dim in (128, 64):
+        lengths = torch.randint(0, 160, (N,), generator=g).tolist()
+        T = sum(lengths)
+        q, k, v, do = _qkv((T,), heads, kv_heads, dim, dtype, N + dim, device)
+        cu = torch.tensor([0] + lengths).cumsum(0).to(torch.int32).to(device)
+        for t in (q, k, v):
+            t.requires_grad_()
+        out = B.causal_attention(q, k, v, cu_seqlens=cu)
+        grads = torch.autograd.grad(out, (q, k, v), do)
+        ends = cu.tolist()
+        _check_sequences(q, k, v, do, out, grads, list(zip(ends, ends[1:])), dim ** -0.5, dtype)
 
 
 def test_attention_empty_inputs(device):
@@ -526,9 +555,11 @@ def test_differentiable_once(device, which):
         got[0].float().sum().backward()
 
 
+@pytest.mark.parametrize("rows", [128, 64, 32])
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
-def test_attention_gradients_that_cancel(device, dtype):
+def test_attention_gradients_that_cancel(device, bgx_env, dtype, rows):
     """Sequences of one token: the softmax is constant, dq and dk are exactly 0 and dv is the sum over the heads."""
+    bgx_env("BGX_ATTENTION_ROWS", rows)
     q, k, v, do = _qkv((40,), 4, 2, 64, dtype, 30, device)
     cu = torch.arange(41, dtype=torch.int32, device=device)
     for t in (q, k, v):
