@@ -27,8 +27,6 @@ namespace bgx {
 constexpr int AT_WAVES = 4;
 constexpr int AT_THREADS = AT_WAVES * WAVE;
 constexpr int AT_TILES[3] = {128, 64, 32};  // rows a workgroup owns (see Work)
-// workgroups of 128 rows: from AT_MANY on they are taken, from AT_SOME on workgroups of 64 rows, below of 32
-constexpr int AT_MANY = 512, AT_SOME = 128;
 constexpr int AT_MAX_D = 128;
 constexpr float AT_LOG2E = 1.4426950408889634f;
 
@@ -979,9 +977,21 @@ static AttnArgs attn_args(const bgx_attention_shape* a) {
 }
 
 // Which tile height a launch over `heads` heads takes, and its number of workgroups (0: too many).
-static unsigned attn_grid(AttnArgs& A, const bgx_attention_shape* a, int heads, int* which) {
+// By the number of workgroups that 128 rows each would make.  With few of them the longest walk decides and shorter
+// walks win; with many the traffic to LDS does, and wide heads, whose smaller workgroups run one wave a SIMD, turn
+// earlier.  Measured (us, 128 / 64 / 32 rows): bf16, heads of 64, forward of 1 x 512 positions, 12 heads (48
+// workgroups) 11.7 / 10.3 / 8.4, 2 x 1024 (192) 18.8 / 17.3 / 17.8, 4 x 1024 (384) 21.1 / 18.5 / 27.8, 6 x 1024 (576)
+// 23.3 / 24.6 / 41.4; heads of 128, 8 heads, 1 x 2048 (128) 50.0 / 48.0 / 42.1, 32 heads, 1 x 1024 (256)
+// 29.3 / 33.8 / 52.1; its dq 40.5 / 38.5 / 59.4; dk and dv of 1 x 4096, 8 key/value heads (256) 519 / 470 / 545; fp32, heads
+// of 64, forward of 6 x 1024 (576) 125 / 107 / 121; dk and dv of fp32 heads of 128 spill at 128 rows (2653 / 1201 / 2510).
+enum AttnKernel { ATTN_FORWARD, ATTN_Q, ATTN_KV };
+static unsigned attn_grid(AttnArgs& A, const bgx_attention_shape* a, AttnKernel kernel, int* which) {
+  const int heads = kernel == ATTN_KV ? a->kv_heads : a->heads;
   const int64_t tall = attn_items(a, 0) * heads;
-  *which = tall >= AT_MANY ? 0 : tall >= AT_SOME ? 1 : 2;
+  const bool wide = a->head_dim > 64, full = a->dtype == BGX_F32;
+  const int64_t many = full ? (!wide ? 1024 : kernel == ATTN_KV ? INT64_MAX : 512)
+                            : (!wide ? 512 : kernel == ATTN_FORWARD ? 160 : kernel == ATTN_Q ? 256 : 384);
+  *which = tall >= many ? 0 : tall >= 160 ? 1 : 2;
   for (int i = 0; i < 3; ++i)
     if (switches().attention_rows == AT_TILES[i]) *which = i;
   const int64_t grid = attn_items(a, *which) * heads;
@@ -1106,7 +1116,7 @@ int attention_forward_impl(const bgx_attention_shape* a, const bgx_attention_row
   A.o = attn_view(o);
   attn_saved(A, a, saved);
   int which;
-  const unsigned grid = attn_grid(A, a, a->heads, &which);
+  const unsigned grid = attn_grid(A, a, ATTN_FORWARD, &which);
   BGX_REQUIRE(grid > 0, BGX_E_SHAPE, "attention: %lld rows of %d heads", (long long)a->rows, a->heads);
   BGX_ATTN_LAUNCH(attention_forward_kernel, a->dtype, a->head_dim, which, grid, (hipStream_t)stream, A);
   return 0;
@@ -1143,10 +1153,10 @@ int attention_backward_impl(const bgx_attention_shape* a, const bgx_attention_ro
   A.peak = A.delta + a->rows * a->heads;
   hipStream_t s = (hipStream_t)stream;
   int which;
-  unsigned grid = attn_grid(A, a, a->heads, &which);
+  unsigned grid = attn_grid(A, a, ATTN_Q, &which);
   BGX_REQUIRE(grid > 0, BGX_E_SHAPE, "attention backward: %lld rows of %d heads", (long long)a->rows, a->heads);
   BGX_ATTN_LAUNCH(attention_backward_q_kernel, a->dtype, a->head_dim, which, grid, s, A);
-  grid = attn_grid(A, a, a->kv_heads, &which);
+  grid = attn_grid(A, a, ATTN_KV, &which);
   BGX_ATTN_LAUNCH(attention_backward_kv_kernel, a->dtype, a->head_dim, which, grid, s, A);
   return 0;
 }

@@ -13,6 +13,7 @@
 namespace bgx {
 
 constexpr int DISTILL_MAX_K = 1024;
+constexpr int DEEP = 4;  // chunks a thread has on their way at once
 
 struct DistillArgs {
   const void* logits;
@@ -108,18 +109,10 @@ __global__ __launch_bounds__(THREADS) void distill_forward_kernel(DistillArgs A)
   const float c = LOG2E / A.tau;
   float m = -INFINITY, s = 0.f;
   bool bad = false;
-  const int chunks = (A.V + EPL - 1) / EPL;
-  for (int i = threadIdx.x; i < chunks; i += THREADS) {
-    float v[EPL];
-    Chunk<T>::unpack(load_chunk_tail(z, (int64_t)i * EPL, A.V), v);
-    if ((i + 1) * EPL > A.V) {
-#pragma unroll
-      for (int e = 0; e < EPL; ++e)
-        if (i * EPL + e >= A.V) v[e] = -INFINITY;
-    }
+  auto take = [&](const float* v, auto count) {
     float top = m;
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) {
+    for (int e = 0; e < count; ++e) {
       top = fmaxf(top, v[e]);
       bad |= v[e] != v[e];
     }
@@ -127,10 +120,29 @@ __global__ __launch_bounds__(THREADS) void distill_forward_kernel(DistillArgs A)
       s *= exp2_hw((m - top) * c);
       m = top;
     }
-    if (m != -INFINITY) {
+    const float shift = m == -INFINITY ? 0.f : m * c;  // nothing but -inf so far: weights of 0
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) s += exp2_hw((v[e] - m) * c);
-    }
+    for (int e = 0; e < count; ++e) s += exp2_hw(fmaf(v[e], c, -shift));
+  };
+  const int chunks = A.V / EPL;  // whole ones; the row's last elements go one by one
+  int i = threadIdx.x;
+  for (; i + (DEEP - 1) * THREADS < chunks; i += DEEP * THREADS) {
+    uint4 w[DEEP];
+    float v[DEEP * EPL];
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) w[k] = load_chunk_any(z + (int64_t)(i + k * THREADS) * EPL);
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) Chunk<T>::unpack(w[k], v + k * EPL);
+    take(v, std::integral_constant<int, DEEP * EPL>());
+  }
+  for (; i < chunks; i += THREADS) {
+    float v[EPL];
+    Chunk<T>::unpack(load_chunk_any(z + (int64_t)i * EPL), v);
+    take(v, std::integral_constant<int, EPL>());
+  }
+  if ((int)threadIdx.x < A.V - chunks * EPL) {
+    const float v = Elem<T>::load(z + (int64_t)chunks * EPL + threadIdx.x);
+    take(&v, std::integral_constant<int, 1>());
   }
   const float top = block_max<THREADS>(m, slot);
   s = block_sum<THREADS>(m == -INFINITY ? 0.f : s * exp2_hw((m - top) * c), slot);
@@ -163,22 +175,41 @@ __global__ __launch_bounds__(THREADS) void distill_backward_kernel(DistillArgs A
   const int64_t r = blockIdx.x;
   const float top = A.stats[2 * r], s = A.stats[2 * r + 1];
   T* dz = (T*)A.dlogits + r * A.dstride;
-  const int chunks = (A.V + EPL - 1) / EPL;
+  const int chunks = A.V / EPL, rest = A.V - chunks * EPL;
   if (s < 0.f) {
     for (int i = threadIdx.x; i < chunks; i += THREADS)
-      store_chunk_tail(dz, (int64_t)i * EPL, A.V, make_uint4(0u, 0u, 0u, 0u));
+      store_chunk_any(dz + (int64_t)i * EPL, make_uint4(0u, 0u, 0u, 0u));
+    if ((int)threadIdx.x < rest) store_bits(dz + (int64_t)chunks * EPL + threadIdx.x, 0u);
     return;
   }
   float t_max, t_sum;
   teacher_row<THREADS>(A, r, id, prob, slot, t_max, t_sum);
   const T* z = (const T*)A.logits + r * A.stride;
   const float c = LOG2E / A.tau, g = A.grad[r] * A.tau, scale = g / s;
-  for (int i = threadIdx.x; i < chunks; i += THREADS) {
+  int i = threadIdx.x;
+  for (; i + (DEEP - 1) * THREADS < chunks; i += DEEP * THREADS) {
+    uint4 w[DEEP];
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) w[k] = load_chunk_any(z + (int64_t)(i + k * THREADS) * EPL);
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) {
+      float v[EPL];
+      Chunk<T>::unpack(w[k], v);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) v[e] = exp2_hw((v[e] - top) * c) * scale;
+      store_chunk_any(dz + (int64_t)(i + k * THREADS) * EPL, Chunk<T>::pack(v));
+    }
+  }
+  for (; i < chunks; i += THREADS) {
     float v[EPL];
-    Chunk<T>::unpack(load_chunk_tail(z, (int64_t)i * EPL, A.V), v);
+    Chunk<T>::unpack(load_chunk_any(z + (int64_t)i * EPL), v);
 #pragma unroll
     for (int e = 0; e < EPL; ++e) v[e] = exp2_hw((v[e] - top) * c) * scale;
-    store_chunk_tail(dz, (int64_t)i * EPL, A.V, Chunk<T>::pack(v));
+    store_chunk_any(dz + (int64_t)i * EPL, Chunk<T>::pack(v));
+  }
+  if ((int)threadIdx.x < rest) {
+    const int64_t at = (int64_t)chunks * EPL + threadIdx.x;
+    store_as(dz, at, exp2_hw((Elem<T>::load(z + at) - top) * c) * scale, Elem<T>::code);
   }
   // The teacher's entries again, with their probabilities taken off before the one rounding.  An id that comes
   // twice is written twice with the same value: every writer adds all entries of its id, in the order of k.

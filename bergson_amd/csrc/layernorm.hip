@@ -52,61 +52,95 @@ __device__ inline float2 row_sum2(float2 v, float2 (*slot)[LN_WAVES], int& turn)
   return v;
 }
 
-template <typename T, typename WT, int NE, int WPR>
+// How a row's columns fall to the lanes: chunk c of a lane starts at column (c * WPR * 64 + lane) * EPL.  Where a row is
+// no whole number of chunks (RAGGED), the last one is moved back to end with the row -- every load and store stays one
+// vector access without a branch around it, a column two lanes hold gets the same value from both, and the sums leave
+// out the moved chunk's first `skip` elements.  Lanes past the row's end read the last chunk and count for nothing.
+// Rows shorter than a chunk (TINY) go element by element.
+enum LnMode { LN_WHOLE, LN_RAGGED, LN_TINY };
+
+template <typename T, int NE, int WPR, int MODE>
+struct LnRow {
+  static constexpr int EPL = Chunk<T>::N, NC = NE / EPL;
+  int first, d;
+  __device__ LnRow(int d) : first(WPR == 1 ? threadIdx.x & (WAVE - 1) : threadIdx.x), d(d) {}
+  __device__ int start(int c) const { return (c * WPR * WAVE + first) * EPL; }
+  __device__ bool used(int c) const { return start(c) < d; }
+  __device__ int at(int c) const { return MODE == LN_TINY ? start(c) : min(start(c), d - EPL); }
+  // whether element e of chunk c is this lane's to count
+  __device__ bool counts(int c, int e) const {
+    if constexpr (MODE == LN_WHOLE) return used(c);
+    if constexpr (MODE == LN_TINY) return start(c) + e < d;
+    return used(c) && at(c) + e >= start(c);
+  }
+  template <typename U>
+  __device__ void load(const U* row, int c, float* f) const {  // EPL elements of a type that may be wider than T
+#pragma unroll
+    for (int k = 0; k < EPL; k += Chunk<U>::N) Chunk<U>::unpack(load_raw(row, c, k), f + k);
+  }
+  template <typename U>
+  __device__ uint4 load_raw(const U* row, int c, int k = 0) const {
+    if constexpr (MODE == LN_TINY) return load_chunk_tail(row, min(start(c) + k, d), d);
+    return load_chunk_any(row + at(c) + k);
+  }
+  __device__ void store(T* row, int c, const float* f) const {
+    if (!used(c)) return;
+    if constexpr (MODE == LN_TINY)
+      store_chunk_tail(row, start(c), d, Chunk<T>::pack(f));
+    else
+      store_chunk_any(row + at(c), Chunk<T>::pack(f));
+  }
+  // sum over the chunk's elements that count
+  template <typename F>
+  __device__ float sum(int c, F f) const {
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) s += MODE == LN_WHOLE || counts(c, e) ? f(e) : 0.f;
+    return MODE == LN_WHOLE && !used(c) ? 0.f : s;
+  }
+};
+
+template <typename T, typename WT, int NE, int WPR, int MODE>
 __global__ __launch_bounds__(LN_WAVES* WAVE) void layernorm_forward_kernel(NormArgs A) {
-  constexpr int EPL = Chunk<T>::N, NC = NE / EPL;
+  using Row = LnRow<T, NE, WPR, MODE>;
+  constexpr int EPL = Row::EPL, NC = Row::NC;
   __shared__ float2 slot[2][LN_WAVES];
   int turn = 0;
-  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+  const Row row(A.d);
+  const float over_d = 1.0f / A.d;
   const int64_t step = (int64_t)gridDim.x * (LN_WAVES / WPR);
-  const int first = WPR == 1 ? lane : (int)threadIdx.x;
-  for (int64_t r = (int64_t)blockIdx.x * (LN_WAVES / WPR) + (WPR == 1 ? wave : 0); r < A.rows; r += step) {
+  for (int64_t r = (int64_t)blockIdx.x * (LN_WAVES / WPR) + (WPR == 1 ? threadIdx.x / WAVE : 0); r < A.rows; r += step) {
     const T* xr = (const T*)A.x + r * A.x_stride;
     float x[NE];
-    float2 s = make_float2(0.f, 0.f);
+    float2 s = make_float2(0.f, 0.f), q = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) row.load(xr, c, x + c * EPL);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) s.x += row.sum(c, [&](int e) { return x[c * EPL + e]; });
+    const float mean = row_sum2<WPR>(s, slot, turn).x * over_d;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int col = (c * WPR * WAVE + first) * EPL;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (col < A.d) v = load_chunk_tail(xr, col, A.d);
-      Chunk<T>::unpack(v, x + c * EPL);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) x[c * EPL + e] -= mean;
+      q.x += row.sum(c, [&](int e) { return x[c * EPL + e] * x[c * EPL + e]; });
     }
-#pragma unroll
-    for (int e = 0; e < NE; ++e) s.x += x[e];
-    const float mean = row_sum2<WPR>(s, slot, turn).x / A.d;
-    float2 q = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int e = 0; e < EPL; ++e) {
-        const bool in = (c * WPR * WAVE + first) * EPL + e < A.d;
-        const float dev = in ? x[c * EPL + e] - mean : 0.f;
-        x[c * EPL + e] = dev;
-        q.x = fmaf(dev, dev, q.x);
-      }
-    const float rstd = 1.0f / sqrtf(row_sum2<WPR>(q, slot, turn).x / A.d + A.eps);
+    const float rstd = 1.0f / sqrtf(row_sum2<WPR>(q, slot, turn).x * over_d + A.eps);
     T* yr = (T*)A.y + r * A.y_stride;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int col = (c * WPR * WAVE + first) * EPL;
-      if (col >= A.d) continue;
-      float o[EPL];
+      float w[EPL], b[EPL];
+      row.load((const WT*)A.weight, c, w);
+      if (A.bias != nullptr) {
+        row.load((const WT*)A.bias, c, b);
+      } else {
 #pragma unroll
-      for (int k = 0; k < EPL; k += Chunk<WT>::N) {  // weights of a wider type take two chunks
-        float w[Chunk<WT>::N], b[Chunk<WT>::N];
-        Chunk<WT>::unpack(load_chunk_tail((const WT*)A.weight, col + k, A.d), w);
-        if (A.bias != nullptr) {
-          Chunk<WT>::unpack(load_chunk_tail((const WT*)A.bias, col + k, A.d), b);
-        } else {
-#pragma unroll
-          for (int e = 0; e < Chunk<WT>::N; ++e) b[e] = 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < Chunk<WT>::N; ++e) o[k + e] = fmaf(x[c * EPL + k + e] * rstd, w[e], b[e]);
+        for (int e = 0; e < EPL; ++e) b[e] = 0.f;
       }
-      store_chunk_tail(yr, col, A.d, Chunk<T>::pack(o));
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) b[e] = fmaf(x[c * EPL + e] * rstd, w[e], b[e]);
+      row.store(yr, c, b);
     }
-    if (A.mean != nullptr && first == 0) {
+    if (A.mean != nullptr && row.first == 0) {
       A.mean[r] = mean;
       A.rstd[r] = rstd;
     }
@@ -114,76 +148,76 @@ __global__ __launch_bounds__(LN_WAVES* WAVE) void layernorm_forward_kernel(NormA
 }
 
 // PARAMS: the workgroup also sums dy xh and dy over its rows, column by column in registers (a lane keeps the same
-// columns for every row), adds its waves' sums through LDS in a fixed order and writes one row of partial sums.
-template <typename T, typename WT, int NE, int WPR, bool PARAMS>
+// columns for every row), adds its waves' sums through LDS in a fixed order and writes one row of partial sums.  The
+// next row's x and dy are on their way while a row is worked on.
+template <typename T, typename WT, int NE, int WPR, int MODE, bool PARAMS>
 __global__ __launch_bounds__(LN_WAVES* WAVE) void layernorm_backward_kernel(NormArgs A) {
-  constexpr int EPL = Chunk<T>::N, NC = NE / EPL;
+  using Row = LnRow<T, NE, WPR, MODE>;
+  constexpr int EPL = Row::EPL, NC = Row::NC;
   __shared__ float2 slot[2][LN_WAVES];
   __shared__ float colsum[PARAMS && WPR == 1 ? WAVE * NE : 1];
   int turn = 0;
+  const Row row(A.d);
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+  const float over_d = 1.0f / A.d;
   const int64_t step = (int64_t)gridDim.x * (LN_WAVES / WPR);
-  const int first = WPR == 1 ? lane : (int)threadIdx.x;
   float dw[PARAMS ? NE : 1], db[PARAMS ? NE : 1];
   if constexpr (PARAMS) {
 #pragma unroll
     for (int e = 0; e < NE; ++e) dw[e] = db[e] = 0.f;
   }
-  for (int64_t r = (int64_t)blockIdx.x * (LN_WAVES / WPR) + (WPR == 1 ? wave : 0); r < A.rows; r += step) {
+  uint4 xv[NC], gv[NC];
+  float mean = 0.f, rstd = 0.f;
+  auto fetch = [&](int64_t r) {
     const T* xr = (const T*)A.x + r * A.x_stride;
     const T* gr = (const T*)A.dy + r * A.dy_stride;
-    const float mean = A.mean[r], rstd = A.rstd[r];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      xv[c] = row.load_raw(xr, c);
+      gv[c] = row.load_raw(gr, c);
+    }
+    mean = A.mean[r];
+    rstd = A.rstd[r];
+  };
+  int64_t r = (int64_t)blockIdx.x * (LN_WAVES / WPR) + (WPR == 1 ? wave : 0);
+  if (r < A.rows) fetch(r);
+  for (; r < A.rows; r += step) {
     float x[NE], h[NE];
     float2 s = make_float2(0.f, 0.f);  // sums of h and of h xh
-    uint4 xv[NC], gv[NC];
+    const float m = mean, f = rstd;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int col = (c * WPR * WAVE + first) * EPL;
-      xv[c] = gv[c] = make_uint4(0u, 0u, 0u, 0u);
-      if (col < A.d) {
-        xv[c] = load_chunk_tail(xr, col, A.d);
-        gv[c] = load_chunk_tail(gr, col, A.d);
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int col = (c * WPR * WAVE + first) * EPL;
       Chunk<T>::unpack(xv[c], x + c * EPL);
       Chunk<T>::unpack(gv[c], h + c * EPL);
+    }
+    fetch(r + step < A.rows ? r + step : r);
 #pragma unroll
-      for (int k = 0; k < EPL; k += Chunk<WT>::N) {
-        float w[Chunk<WT>::N];
-        uint4 wv = make_uint4(0u, 0u, 0u, 0u);
-        if (col < A.d) wv = load_chunk_tail((const WT*)A.weight, col + k, A.d);
-        Chunk<WT>::unpack(wv, w);
+    for (int c = 0; c < NC; ++c) {
+      float w[EPL];
+      row.load((const WT*)A.weight, c, w);
 #pragma unroll
-        for (int e = 0; e < Chunk<WT>::N; ++e) {
-          const int i = c * EPL + k + e;
-          const bool in = col + k + e < A.d;
-          const float xh = in ? (x[i] - mean) * rstd : 0.f;
-          if constexpr (PARAMS) {
-            dw[i] = fmaf(h[i], xh, dw[i]);
-            db[i] += h[i];
-          }
-          x[i] = xh;
-          h[i] *= w[e];
-          s.x += h[i];
-          s.y = fmaf(h[i], xh, s.y);
+      for (int e = 0; e < EPL; ++e) {
+        const int i = c * EPL + e;
+        x[i] = (x[i] - m) * f;
+        if constexpr (PARAMS) {  // columns that are another lane's, or none, are left out when the sums are written
+          dw[i] = fmaf(h[i], x[i], dw[i]);
+          db[i] += h[i];
         }
+        h[i] *= w[e];
       }
+      s.x += row.sum(c, [&](int e) { return h[c * EPL + e]; });
+      s.y += row.sum(c, [&](int e) { return h[c * EPL + e] * x[c * EPL + e]; });
     }
     if (A.y == nullptr) continue;
     s = row_sum2<WPR>(s, slot, turn);
-    const float mh = s.x / A.d, mx = s.y / A.d;
+    const float mh = s.x * over_d, mx = s.y * over_d;
     T* dxr = (T*)A.y + r * A.y_stride;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int col = (c * WPR * WAVE + first) * EPL;
-      if (col >= A.d) continue;
       float o[EPL];
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) o[e] = rstd * (h[c * EPL + e] - mh - x[c * EPL + e] * mx);
-      store_chunk_tail(dxr, col, A.d, Chunk<T>::pack(o));
+      for (int e = 0; e < EPL; ++e) o[e] = f * (h[c * EPL + e] - mh - x[c * EPL + e] * mx);
+      row.store(dxr, c, o);
     }
   }
   if constexpr (PARAMS) {
@@ -207,32 +241,34 @@ __global__ __launch_bounds__(LN_WAVES* WAVE) void layernorm_backward_kernel(Norm
       }
       if (WPR > 1 || wave == 0) {
 #pragma unroll
-        for (int e = 0; e < NE; ++e) {
-          const int col = ((e / EPL) * WPR * WAVE + first) * EPL + e % EPL;
-          if (col < A.d) part[(int64_t)which * A.d + col] = acc[e];
-        }
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int e = 0; e < EPL; ++e)
+            if (row.counts(c, e)) part[(int64_t)which * A.d + row.at(c) + e] = acc[c * EPL + e];
       }
     }
   }
 }
 
-// dw[c], db[c] = sum over the n_parts rows of partial sums, in a fixed order: 16 groups of rows per column, joined
+// dw[c], db[c] = sum over the n_parts rows of partial sums, in a fixed order: 64 groups of rows per column, joined
 // through LDS.  grid.y = 0: dw, 1: db.
-__global__ __launch_bounds__(1024) void layernorm_params_kernel(const float* __restrict__ parts, int n_parts, int d,
-                                                                void* dw, void* db, int dtype) {
-  __shared__ float sums[16][64];
-  const int col = blockIdx.x * 64 + (threadIdx.x & 63), group = threadIdx.x >> 6;
+constexpr int LN_COLS = 16, LN_GROUPS = 64;
+__global__ __launch_bounds__(LN_COLS* LN_GROUPS) void layernorm_params_kernel(const float* __restrict__ parts, int n_parts,
+                                                                              int d, void* dw, void* db, int dtype) {
+  __shared__ float sums[LN_GROUPS][LN_COLS + 1];
+  const int lane = threadIdx.x % LN_COLS, group = threadIdx.x / LN_COLS, col = blockIdx.x * LN_COLS + lane;
+  const float* p = parts + (int64_t)blockIdx.y * d + min(col, d - 1);
   float s = 0.f;
-  if (col < d)
-    for (int i = group; i < n_parts; i += 16) s += parts[((int64_t)i * 2 + blockIdx.y) * d + col];
-  sums[group][threadIdx.x & 63] = s;
+#pragma unroll 8
+  for (int i = group; i < n_parts; i += LN_GROUPS) s += p[(int64_t)i * 2 * d];
+  sums[group][lane] = s;
   __syncthreads();
-  if (group == 0 && col < d) {
-#pragma unroll
-    for (int g = 1; g < 16; ++g) s += sums[g][threadIdx.x];
-    void* out = blockIdx.y == 0 ? dw : db;
-    if (out != nullptr) store_as(out, col, s, dtype);
+  for (int half = LN_GROUPS / 2; half > 0; half /= 2) {
+    if (group < half) sums[group][lane] += sums[group + half][lane];
+    __syncthreads();
   }
+  void* out = blockIdx.y == 0 ? dw : db;
+  if (group == 0 && col < d && out != nullptr) store_as(out, col, sums[0][lane], dtype);
 }
 
 static int ln_check(int64_t rows, int d, int dtype, int wdtype) {
@@ -260,22 +296,38 @@ static int ln_grid(int64_t rows, int wpr, int most) {
 
 template <typename T, typename WT>
 static int ln_forward(const NormArgs& A, hipStream_t stream) {
-#define BGX_LN_CALL(NE, WPR)                                                                                   \
-  {                                                                                                            \
-    layernorm_forward_kernel<T, WT, NE, WPR><<<ln_grid(A.rows, WPR, 8192), LN_WAVES * WAVE, 0, stream>>>(A);   \
+#define BGX_LN_LAUNCH(NE, WPR, MODE) \
+  layernorm_forward_kernel<T, WT, NE, WPR, MODE><<<ln_grid(A.rows, WPR, 8192), LN_WAVES * WAVE, 0, stream>>>(A)
+#define BGX_LN_CALL(NE, WPR)                                \
+  {                                                         \
+    if (std::is_same<T, WT>::value && A.d % Chunk<T>::N == 0) \
+      BGX_LN_LAUNCH(NE, WPR, (std::is_same<T, WT>::value ? LN_WHOLE : LN_RAGGED)); \
+    else                                                    \
+      BGX_LN_LAUNCH(NE, WPR, LN_RAGGED);                    \
   }
-  BGX_LN_WIDTHS(A.d, BGX_LN_CALL)
+  if (A.d < Chunk<T>::N) BGX_LN_LAUNCH(8, 1, LN_TINY);
+  else BGX_LN_WIDTHS(A.d, BGX_LN_CALL)
 #undef BGX_LN_CALL
+#undef BGX_LN_LAUNCH
   BGX_HIP(hipGetLastError());
   return 0;
 }
 
 template <typename T, typename WT, bool PARAMS>
 static int ln_backward(const NormArgs& A, int grid, hipStream_t stream) {
-#define BGX_LN_CALL(NE, WPR) \
-  { layernorm_backward_kernel<T, WT, NE, WPR, PARAMS><<<grid, LN_WAVES * WAVE, 0, stream>>>(A); }
-  BGX_LN_WIDTHS(A.d, BGX_LN_CALL)
+#define BGX_LN_LAUNCH(NE, WPR, MODE) \
+  layernorm_backward_kernel<T, WT, NE, WPR, MODE, PARAMS><<<grid, LN_WAVES * WAVE, 0, stream>>>(A)
+#define BGX_LN_CALL(NE, WPR)                                \
+  {                                                         \
+    if (std::is_same<T, WT>::value && A.d % Chunk<T>::N == 0) \
+      BGX_LN_LAUNCH(NE, WPR, (std::is_same<T, WT>::value ? LN_WHOLE : LN_RAGGED)); \
+    else                                                    \
+      BGX_LN_LAUNCH(NE, WPR, LN_RAGGED);                    \
+  }
+  if (A.d < Chunk<T>::N) BGX_LN_LAUNCH(8, 1, LN_TINY);
+  else BGX_LN_WIDTHS(A.d, BGX_LN_CALL)
 #undef BGX_LN_CALL
+#undef BGX_LN_LAUNCH
   BGX_HIP(hipGetLastError());
   return 0;
 }
@@ -361,7 +413,7 @@ int layernorm_backward_impl(const void* dy, int64_t dy_stride, const void* x, in
     if (rc) return rc;
   }
   if (params) {
-    layernorm_params_kernel<<<dim3((d + 63) / 64, 2), 1024, 0, s>>>((const float*)ws, parts, d, dweight, dbias, wdtype);
+    layernorm_params_kernel<<<dim3((d + LN_COLS - 1) / LN_COLS, 2), LN_COLS * LN_GROUPS, 0, s>>>((const float*)ws, parts, d, dweight, dbias, wdtype);
     BGX_HIP(hipGetLastError());
   }
   return 0;

@@ -124,16 +124,28 @@ __device__ inline void store_chunk_tail(T* row, int64_t col, int64_t len, const 
     }
 }
 
-// Sum / maximum over the 64 lanes of a wave; every lane gets the result, formed in the same order on every lane.
+// Sum / maximum over the 64 lanes of a wave; every lane gets the result, formed in the same order on every lane: within
+// 16 lanes by lane permutations that the operand read applies, then across the 16s and the halves.
+template <int CTRL>
+__device__ inline float dpp_of(float v) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+template <typename OP>
+__device__ inline float wave_reduce(float v, OP op) {
+  v = op(v, dpp_of<0xb1>(v));   // lane ^ 1
+  v = op(v, dpp_of<0x4e>(v));   // lane ^ 2
+  v = op(v, dpp_of<0x141>(v));  // mirrored within 8: the other four
+  v = op(v, dpp_of<0x140>(v));  // mirrored within 16: the other eight
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 __device__ inline float wave_sum(float v) {
-#pragma unroll
-  for (int m = 1; m < WAVE; m <<= 1) v += __shfl_xor(v, m, WAVE);
-  return v;
+  return wave_reduce(v, [](float a, float b) { return a + b; });
 }
 __device__ inline float wave_max(float v) {
-#pragma unroll
-  for (int m = 1; m < WAVE; m <<= 1) v = fmaxf(v, __shfl_xor(v, m, WAVE));
-  return v;
+  return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 }  // namespace bgx
