@@ -13,6 +13,7 @@
 namespace bgx {
 
 constexpr int DISTILL_MAX_K = 1024;
+constexpr int DISTILL_FEW = 512;
 constexpr int DEEP = 4;  // chunks a thread has on their way at once
 
 struct DistillArgs {
@@ -108,14 +109,10 @@ __global__ __launch_bounds__(THREADS) void distill_forward_kernel(DistillArgs A)
   const T* z = (const T*)A.logits + r * A.stride;
   const float c = LOG2E / A.tau;
   float m = -INFINITY, s = 0.f;
-  bool bad = false;
   auto take = [&](const float* v, auto count) {
     float top = m;
 #pragma unroll
-    for (int e = 0; e < count; ++e) {
-      top = fmaxf(top, v[e]);
-      bad |= v[e] != v[e];
-    }
+    for (int e = 0; e < count; ++e) top = fmaxf(top, v[e]);  // drops NaN; the sum keeps it
     if (top > m) {
       s *= exp2_hw((m - top) * c);
       m = top;
@@ -145,8 +142,7 @@ __global__ __launch_bounds__(THREADS) void distill_forward_kernel(DistillArgs A)
     take(&v, std::integral_constant<int, 1>());
   }
   const float top = block_max<THREADS>(m, slot);
-  s = block_sum<THREADS>(m == -INFINITY ? 0.f : s * exp2_hw((m - top) * c), slot);
-  if (block_max<THREADS>(bad ? 1.f : 0.f, slot) != 0.f) s = NAN;
+  s = block_sum<THREADS>(m == -INFINITY ? s : s * exp2_hw((m - top) * c), slot);
   const float log_s = logf(s), log_t = logf(t_sum), inv_tau = 1.f / A.tau;
   float loss = 0.f;
   for (int k = threadIdx.x; k < A.K; k += THREADS) {
@@ -172,7 +168,8 @@ __global__ __launch_bounds__(THREADS) void distill_backward_kernel(DistillArgs A
   __shared__ float slot[THREADS / WAVE];
   __shared__ int id[DISTILL_MAX_K];
   __shared__ float prob[DISTILL_MAX_K];
-  const int64_t r = blockIdx.x;
+  // from the last row on: what the forward pass read last may still be in the memory-side cache
+  const int64_t r = A.rows - 1 - blockIdx.x;
   const float top = A.stats[2 * r], s = A.stats[2 * r + 1];
   T* dz = (T*)A.dlogits + r * A.dstride;
   const int chunks = A.V / EPL, rest = A.V - chunks * EPL;
@@ -242,10 +239,16 @@ static int distill_check(const DistillArgs& A, int dtype, const char* what) {
 template <typename T>
 static int distill_launch(const DistillArgs& A, bool backward, hipStream_t s) {
   const dim3 grid((unsigned)A.rows);
-  if (backward)
+  if (A.rows < DISTILL_FEW) {
+    if (backward)
+      distill_backward_kernel<T, 1024><<<grid, 1024, 0, s>>>(A);
+    else
+      distill_forward_kernel<T, 1024><<<grid, 1024, 0, s>>>(A);
+  } else if (backward) {
     distill_backward_kernel<T, 256><<<grid, 256, 0, s>>>(A);
-  else
+  } else {
     distill_forward_kernel<T, 256><<<grid, 256, 0, s>>>(A);
+  }
   BGX_HIP(hipGetLastError());
   return 0;
 }

@@ -168,7 +168,8 @@ __global__ __launch_bounds__(LN_WAVES* WAVE) void layernorm_backward_kernel(Norm
   }
   uint4 xv[NC], gv[NC];
   float mean = 0.f, rstd = 0.f;
-  auto fetch = [&](int64_t r) {
+  auto fetch = [&](int64_t i) {
+    const int64_t r = A.rows - 1 - i;  // from the last row on: the forward pass's last rows may still be cached
     const T* xr = (const T*)A.x + r * A.x_stride;
     const T* gr = (const T*)A.dy + r * A.dy_stride;
 #pragma unroll
@@ -211,7 +212,7 @@ __global__ __launch_bounds__(LN_WAVES* WAVE) void layernorm_backward_kernel(Norm
     if (A.y == nullptr) continue;
     s = row_sum2<WPR>(s, slot, turn);
     const float mh = s.x * over_d, mx = s.y * over_d;
-    T* dxr = (T*)A.y + r * A.y_stride;
+    T* dxr = (T*)A.y + (A.rows - 1 - r) * A.y_stride;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       float o[EPL];
