@@ -424,11 +424,12 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
         for (int ks = 0; ks < KS; ++ks) Mma32<T>::mma(read_rows<T, DP>(tk, u * 32, ks, lane), qf[ks], s[u]);
       }
       if (k0 + SUB * 32 - 1 > mine) {  // the tile reaches past some row's own position
+        const int last = row - k0 - 4 * half;
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (k0 + u * 32 + 8 * (i / 4) + 4 * half + i % 4 > row) s[u][i] = -INFINITY;
+            if (u * 32 + 8 * (i / 4) + i % 4 > last) s[u][i] = -INFINITY;
       }
       float top = m;
 #pragma unroll
@@ -437,10 +438,10 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
       const float2 halves = both_halves(top);
       top = fmaxf(halves.x, halves.y);
-      // a row all of whose scores so far are -inf keeps a maximum of -inf; its weights are 0, not 0 - 0
-      const float shift = top == -INFINITY ? 0.f : top * c;
-      if (__any(top > m)) {
-        const float f = exp2_of(m * c - shift);
+      // The shift of the exponents follows the maximum only when it is 2^8 behind for some row: weights up to 2^8
+      // round like smaller ones, and what has been summed is rescaled a few times a row instead of at most tiles.
+      if (__any((top - m) * c > 8.f)) {
+        const float f = top == -INFINITY ? 0.f : exp2_of((m - top) * c);
         l *= f;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
@@ -448,6 +449,8 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
           for (int i = 0; i < 16; ++i) o[dt][i] *= f;
         m = top;
       }
+      // a row all of whose scores so far are -inf keeps a maximum of -inf; its weights are 0, not 0 - 0
+      const float shift = m == -INFINITY ? 0.f : m * c;
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
@@ -619,10 +622,10 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
         for (int i = 0; i < 16; ++i) s[i] = exp2_of(fmaf(s[i], c, -shift)) * dp[i];
         if (k0 + u * 32 + 31 > mine) {
           // a sequence's first row has one key and a constant softmax: its dS is 0, not the rounding of dp - delta
-          const int last = row == 0 ? -1 : row;
+          const int last = (row == 0 ? -1 : row) - k0 - u * 32 - 4 * half;
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (k0 + u * 32 + 8 * (i / 4) + 4 * half + i % 4 > last) s[i] = 0.f;
+            if (8 * (i / 4) + i % 4 > last) s[i] = 0.f;
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -814,12 +817,12 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
           dp[i] = HALF ? s[i] * raise * dp[i] : s[i] * dp[i];
         }
         if (q0 + u * 32 < mine + 31) {
+          const int first_query = row - q0 - u * 32 - 4 * half;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int query = q0 + u * 32 + 8 * (i / 4) + 4 * half + i % 4;
-            if (query < row) s[i] = dp[i] = 0.f;
-            if (query == 0) dp[i] = 0.f;  // one key, a constant softmax: dS is 0, not the rounding of dp - delta
-          }
+          for (int i = 0; i < 16; ++i)
+            if (8 * (i / 4) + i % 4 < first_query) s[i] = dp[i] = 0.f;
+          // a sequence's first row has one key and a constant softmax: its dS is 0, not the rounding of dp - delta
+          if (q0 + u * 32 == 0 && half == 0) dp[0] = 0.f;
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {

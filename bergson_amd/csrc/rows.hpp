@@ -43,14 +43,20 @@ struct Chunk<bf16_t> {
 template <>
 struct Chunk<f16_t> {
   static constexpr int N = 8;
+  // both at once (v_cvt_pk_f16_f32, to nearest even); converted one by one they would take three instructions
+  __device__ static uint32_t pair(float lo, float hi) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 v = {lo, hi};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));
+  }
   __device__ static void unpack(const uint4& v, float* f) {
     const f16x8 h = __builtin_bit_cast(f16x8, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = (float)h[i];
   }
   __device__ static uint4 pack(const float* f) {
-    return make_uint4(f32x2_to_f16x2_bits(f[0], f[1]), f32x2_to_f16x2_bits(f[2], f[3]),
-                      f32x2_to_f16x2_bits(f[4], f[5]), f32x2_to_f16x2_bits(f[6], f[7]));
+    return make_uint4(pair(f[0], f[1]), pair(f[2], f[3]), pair(f[4], f[5]), pair(f[6], f[7]));
   }
 };
 
