@@ -21,6 +21,7 @@ from .data import (
     load_token_gradients,
     pad_and_tensor,
 )
+from .fused_model import fused_model_ops, sequence_lengths
 from .gradient_collectors import GradientCollector, StreamingGradientCollector, TraceCollector
 from .hessians import DensePreconditioner, invert_psd_matrix, load_preconditioner
 from .gradients import AdafactorNormalizer, AdamNormalizer, GradientProcessor, LayerAdapter, Normalizer
@@ -40,7 +41,7 @@ __all__ = [
     "GradientProcessor", "LayerAdapter", "Normalizer", "InMemoryCollector", "normalize_and_aggregate_grads",
     "normalize_flat_grad", "Scorer", "InversionConfig", "DensePreconditioner", "invert_psd_matrix",
     "load_preconditioner", "load_from_optimizer", "build", "create_processor", "create_scorer", "get_query_grads", "score_dataset",
-    "causal_attention", "layer_norm", "topk_distillation",
+    "causal_attention", "layer_norm", "topk_distillation", "fused_model_ops", "sequence_lengths",
 ]
 
 

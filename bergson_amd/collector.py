@@ -37,8 +37,10 @@ from torch.utils.hooks import RemovableHandle
 
 from . import ops
 from .config import AttentionConfig, IndexConfig
-from .data import compute_num_token_grads, pad_and_tensor
+from .data import compute_num_token_grads, pad_and_tensor, pad_teacher
+from .fused_model import fused_model_ops, sequence_lengths
 from .gradients import AdafactorNormalizer, AdamNormalizer, GradientProcessor, LayerAdapter
+from .model_ops import topk_distillation
 
 
 def create_projection_matrix(identifier: str, m: int, n: int, dtype: torch.dtype, device: torch.device | str,
@@ -783,6 +785,18 @@ class CollectorComputer:
         """For each batch: pad, forward, loss, backward (hooks fire), `collector.process_batch`; then
         `collector.teardown()`.  No host synchronisation happens inside the loop."""
         total_processed = torch.tensor(0, device=self.device)
+        with fused_model_ops(self.model) if self.cfg.fused_model_ops else nullcontext():
+            self._run_batches(total_processed)
+        self.collector.teardown()
+        self.collector.remove_hooks()
+        if dist.is_initialized():
+            dist.all_reduce(total_processed, op=dist.ReduceOp.SUM)
+        if self.rank == 0 and self.cfg.run_path:
+            os.makedirs(self.cfg.partial_run_path, exist_ok=True)
+            torch.save(total_processed, os.path.join(self.cfg.partial_run_path, "total_processed.pt"))
+        self.total_processed = total_processed
+
+    def _run_batches(self, total_processed: Tensor) -> None:
         overlapped = OverlappedSteps(self.model, self.collector, self.cfg) if self.overlap_backward else None
         try:
             for indices in self.batches:
@@ -805,21 +819,36 @@ class CollectorComputer:
             raise
         if overlapped is not None:
             overlapped.close()
-        self.collector.teardown()
-        self.collector.remove_hooks()
-        if dist.is_initialized():
-            dist.all_reduce(total_processed, op=dist.ReduceOp.SUM)
-        if self.rank == 0 and self.cfg.run_path:
-            os.makedirs(self.cfg.partial_run_path, exist_ok=True)
-            torch.save(total_processed, os.path.join(self.cfg.partial_run_path, "total_processed.pt"))
-        self.total_processed = total_processed
 
 
 def forward_loss_factory(cfg: IndexConfig) -> Callable:
     """forward_loss(model, x, y, batch) -> per-sample losses [N] with their autograd graph: the forward half
-    of collector.py:926-985 (cross-entropy branch)."""
-    if cfg.loss_fn != "ce":
-        raise NotImplementedError("only the cross-entropy loss is supported (loss_fn='kl' needs PEFT)")
+    of collector.py:926-985 (cross-entropy branch), or with `loss_fn="topk_kl"` the distillation loss."""
+    if cfg.loss_fn not in ("ce", "topk_kl"):
+        raise NotImplementedError("the cross-entropy loss and 'topk_kl' are supported (loss_fn='kl' needs PEFT)")
+    if cfg.loss_fn == "topk_kl" and cfg.label_smoothing:
+        raise ValueError("label_smoothing belongs to the cross-entropy loss, not to loss_fn='topk_kl'")
+
+    def run_model(model, x: Tensor, batch: dict) -> Tensor:
+        if not cfg.fused_model_ops:
+            return model(x).logits
+        lengths = torch.tensor([len(seq) for seq in batch["input_ids"]], dtype=torch.int32)
+        with sequence_lengths(lengths.to(x.device, non_blocking=True)):
+            return model(x).logits
+
+    def distillation_loss(model, x: Tensor, y: Tensor, batch: dict):
+        ids, teacher = pad_teacher(batch, x.shape[1], x.device)
+        logits = run_model(model, x, batch)
+        valid = F.pad(y[:, 1:] != -100, (0, 1), value=False)
+        losses = topk_distillation(logits, ids, teacher, temperature=cfg.distill_temperature, valid=valid).sum(1)
+        if cfg.loss_reduction == "mean":
+            losses = losses / valid.sum(dim=1, dtype=losses.dtype)
+        if "advantage" in batch:
+            losses = losses * torch.tensor(batch["advantage"], device=losses.device)
+        return losses
+
+    if cfg.loss_fn == "topk_kl":
+        return distillation_loss
 
     def forward_loss(model, x: Tensor, y: Tensor, batch: dict):
         # The reference slices `logits[:, :-1]` and reshapes, which copies the [N, S-1, V] logits (400 MB for a
@@ -827,7 +856,7 @@ def forward_loss_factory(cfg: IndexConfig) -> Callable:
         # The same losses come from the whole [N, S, V] tensor as a view, with the labels shifted left and the
         # last position ignored (-100 is cross_entropy's ignore_index: loss 0, gradient 0 -- what the slice's
         # backward pass fills in).
-        logits = model(x).logits
+        logits = run_model(model, x, batch)
         targets = F.pad(y[:, 1:], (0, 1), value=-100)
         masks = y[:, 1:] != -100
         denoms = masks.sum(dim=1, dtype=model.dtype) if cfg.loss_reduction == "mean" else 1.0

@@ -37,7 +37,10 @@ class IndexConfig:
     projection_target: Literal["per_module", "global"] = "per_module"
     token_batch_size: int = 2048
     max_batch_size: int | None = None
-    loss_fn: Literal["ce", "kl"] = "ce"
+    loss_fn: Literal["ce", "kl", "topk_kl"] = "ce"
+    """"topk_kl": distillation from a teacher's highest logits, in the data's columns `teacher_ids` and
+    `teacher_logits` ([length, K] per document; the entries at position s speak about token s + 1)."""
+    distill_temperature: float = 1.0
     loss_reduction: Literal["mean", "sum"] = "sum"
     label_smoothing: float = 0.0
     split_attention_modules: list[str] = field(default_factory=list)
@@ -48,6 +51,8 @@ class IndexConfig:
     modules: list[str] = field(default_factory=list)
     drop_columns: bool = True
     debug: bool = False
+    fused_model_ops: bool = False
+    """Run the model's layer norms and causal attention on this package's kernels (see fused_model.py)."""
 
     @property
     def partial_run_path(self) -> Path:

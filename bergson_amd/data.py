@@ -360,3 +360,28 @@ def pad_and_tensor(sequences: list[list[int]], labels: list[list[int]] | None = 
     lengths_t = torch.tensor(lengths).to(device, non_blocking=True)
     collection_masks = torch.arange(1, width + 1, device=device).unsqueeze(0) < lengths_t.unsqueeze(1)
     return tokens, labels_t, supervised_next, collection_masks
+
+
+def pad_teacher(batch: dict, width: int, device: torch.device | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(ids int64, logits float32), both [N, width, K], of a batch's columns `teacher_ids` and `teacher_logits`: per
+    document one list of a teacher's highest entries per token, which may differ in number.  What is missing -- short
+    lists, positions past a document's end -- has id -1, which the loss takes for no entry."""
+    columns = []
+    for name in ("teacher_ids", "teacher_logits"):
+        if name not in batch:
+            raise ValueError(f"loss_fn='topk_kl' needs the data's column `{name}`: per document a [length, K] list")
+        columns.append(batch[name])
+    entries = max((len(token) for doc in columns[0] for token in doc), default=0)
+    ids = np.full((len(columns[0]), width, max(entries, 1)), -1, dtype=np.int64)
+    logits = np.zeros(ids.shape, dtype=np.float32)
+    for n, (doc_ids, doc_logits, tokens) in enumerate(zip(*columns, batch["input_ids"])):
+        if len(doc_ids) != len(doc_logits) or len(doc_ids) > len(tokens):
+            raise ValueError(f"document {n} of the batch: {len(doc_ids)} teacher_ids, {len(doc_logits)} teacher_logits, "
+                             f"{len(tokens)} tokens")
+        for s, (token_ids, token_logits) in enumerate(zip(doc_ids, doc_logits)):
+            if len(token_ids) != len(token_logits):
+                raise ValueError(f"document {n} of the batch, position {s}: {len(token_ids)} teacher_ids, "
+                                 f"{len(token_logits)} teacher_logits")
+            ids[n, s, :len(token_ids)] = token_ids
+            logits[n, s, :len(token_ids)] = token_logits
+    return torch.from_numpy(ids).to(device, non_blocking=True), torch.from_numpy(logits).to(device, non_blocking=True)

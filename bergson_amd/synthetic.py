@@ -73,16 +73,20 @@ def random_docs(lengths: list[int], vocab: int = 50304, seed: int = 0) -> list[l
 
 class ListDataset:
     """Minimal stand-in for a `datasets.Dataset` of token ids: `len`, `column_names`, `ds[list_of_indices]`.
-    Optional per-document columns: `labels` (token labels, -100 = not supervised) and `advantage`."""
+    Optional per-document columns: `labels` (token labels, -100 = not supervised), `advantage`, and a teacher's highest
+    entries per token, `teacher_ids` and `teacher_logits`."""
 
     def __init__(self, docs: list[list[int]], *, labels: list[list[int]] | None = None,
-                 advantage: list[float] | None = None):
+                 advantage: list[float] | None = None, teacher_ids: list | None = None,
+                 teacher_logits: list | None = None):
         self.docs = docs
         self.columns = {"input_ids": docs, "length": [len(d) for d in docs]}
         if labels is not None:
             self.columns["labels"] = labels
         if advantage is not None:
             self.columns["advantage"] = advantage
+        if teacher_ids is not None:
+            self.columns["teacher_ids"], self.columns["teacher_logits"] = teacher_ids, teacher_logits
         self.column_names = list(self.columns)
 
     def __len__(self) -> int:
