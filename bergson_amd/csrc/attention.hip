@@ -114,6 +114,16 @@ struct Attn<float> {
   }
 };
 
+// what the rounding of pack() cuts off, as a second operand of its own (16-bit types)
+template <typename T>
+__device__ inline uint4 pack_rest(const f32x16& s, int g, const uint4& rounded) {
+  float f[8];
+  Chunk<T>::unpack(rounded, f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = s[g * 8 + i] - f[i];
+  return Chunk<T>::pack(f);
+}
+
 // operand read by rows: chunk 2 ks + h of row base + lane % 32
 template <typename T, int DP>
 __device__ inline uint4 read_rows(const char* tile, int base, int ks, int lane) {
@@ -185,6 +195,10 @@ struct Work {
   static constexpr int THREADS = WAVES * WAVE, ROWS = 32 * RW, SPLIT = WAVES / RW;
   static constexpr int SUB = SPLIT == 1 && sizeof(T) == 2 ? 2 : 1;  // blocks of 32 a wave takes of a tile
   static constexpr int STEP = 32 * SUB * SPLIT;
+  // Few workgroups leave the matrix units idle, and with few rows the roundings of P and dS do not average out (a
+  // sequence of two rows shows that of its one dS in every gradient): there both go in as two operands, the rounded
+  // value and the rest, which gives them 16 or more bits.
+  static constexpr bool FINE = RW == 1 && sizeof(T) == 2;
   // waves a SIMD has room for without spilling registers to memory (the compiler's budget: 512 / 2 or 512)
   static constexpr int PER_SIMD_Q = sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : (RW == 4 || DP <= 64 ? 2 : 1);
   static constexpr int PER_SIMD_KV = sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : (DP <= 64 || WAVES == 8 ? 2 : 1);
@@ -463,9 +477,14 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           const uint4 p = M::pack(s[u], g);
+          uint4 rest = p;
+          if constexpr (W::FINE) rest = pack_rest<T>(s[u], g, p);
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-            Mma32<T>::mma(M::template read_tr<DP>(tv, u * 32 + g * M::GROUP, dt, lane), p, o[dt]);
+          for (int dt = 0; dt < DT; ++dt) {
+            const uint4 a = M::template read_tr<DP>(tv, u * 32 + g * M::GROUP, dt, lane);
+            Mma32<T>::mma(a, p, o[dt]);
+            if constexpr (W::FINE) Mma32<T>::mma(a, rest, o[dt]);
+          }
         }
     }
     if constexpr (W::BUFFERS == 1) __syncthreads();
@@ -630,9 +649,14 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           const uint4 ds = M::pack(s, g);
+          uint4 rest = ds;
+          if constexpr (W::FINE) rest = pack_rest<T>(s, g, ds);
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-            Mma32<T>::mma(M::template read_tr<DP>(tk, u * 32 + g * M::GROUP, dt, lane), ds, dq[dt]);
+          for (int dt = 0; dt < DT; ++dt) {
+            const uint4 a = M::template read_tr<DP>(tk, u * 32 + g * M::GROUP, dt, lane);
+            Mma32<T>::mma(a, ds, dq[dt]);
+            if constexpr (W::FINE) Mma32<T>::mma(a, rest, dq[dt]);
+          }
         }
       }
     }
@@ -827,10 +851,21 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           const uint4 p = M::pack(s, g), ds = M::pack(dp, g);
+          uint4 p_rest = p, ds_rest = ds;
+          if constexpr (W::FINE) {
+            p_rest = pack_rest<T>(s, g, p);
+            ds_rest = pack_rest<T>(dp, g, ds);
+          }
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
-            Mma32<T>::mma(M::template read_tr<DP>(tg, u * 32 + g * M::GROUP, dt, lane), p, dv[dt]);
-            Mma32<T>::mma(M::template read_tr<DP>(tq, u * 32 + g * M::GROUP, dt, lane), ds, dk[dt]);
+            const uint4 a = M::template read_tr<DP>(tg, u * 32 + g * M::GROUP, dt, lane);
+            const uint4 b = M::template read_tr<DP>(tq, u * 32 + g * M::GROUP, dt, lane);
+            Mma32<T>::mma(a, p, dv[dt]);
+            Mma32<T>::mma(b, ds, dk[dt]);
+            if constexpr (W::FINE) {
+              Mma32<T>::mma(a, p_rest, dv[dt]);
+              Mma32<T>::mma(b, ds_rest, dk[dt]);
+            }
           }
         }
       }

@@ -24,6 +24,9 @@ struct NormArgs {
   float* mean;
   float* rstd;
   float* parts;         // backward: [workgroups][2][d] partial sums of dw, db
+  void* dweight;        // backward of a single workgroup: its sums are the gradients
+  void* dbias;
+  int wdtype;
   int64_t rows;
   int64_t x_stride, dy_stride, y_stride;
   int d;
@@ -245,7 +248,14 @@ __global__ __launch_bounds__(LN_WAVES* WAVE) void layernorm_backward_kernel(Norm
         for (int c = 0; c < NC; ++c)
 #pragma unroll
           for (int e = 0; e < EPL; ++e)
-            if (row.counts(c, e)) part[(int64_t)which * A.d + row.at(c) + e] = acc[c * EPL + e];
+            if (row.counts(c, e)) {
+              const int col = row.at(c) + e;
+              void* out = which == 0 ? A.dweight : A.dbias;
+              if (gridDim.x > 1)
+                part[(int64_t)which * A.d + col] = acc[c * EPL + e];
+              else if (out != nullptr)
+                store_as(out, col, acc[c * EPL + e], A.wdtype);
+            }
       }
     }
   }
@@ -362,9 +372,13 @@ int layernorm_forward_impl(const void* x, int64_t x_stride, const void* weight, 
 
 static int ln_wpr(int d) { return d <= 2048 ? 1 : 4; }
 
+// Workgroups that sum dw and db.  Up to 16 rows one does them all and writes the gradients itself: its loop over the
+// rows takes less than a second launch.
+static int ln_parts(int64_t rows, int d) { return rows <= 16 ? 1 : ln_grid(rows, ln_wpr(d), LN_PARTS_MAX); }
+
 size_t layernorm_backward_workspace_bytes(int64_t rows, int d) {
-  if (rows <= 0 || d <= 0 || d > LN_MAX_D) return 0;
-  return (size_t)ln_grid(rows, ln_wpr(d), LN_PARTS_MAX) * 2 * d * sizeof(float);
+  if (rows <= 16 || d <= 0 || d > LN_MAX_D) return 0;
+  return (size_t)ln_parts(rows, d) * 2 * d * sizeof(float);
 }
 
 int layernorm_backward_impl(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* weight,
@@ -382,7 +396,7 @@ int layernorm_backward_impl(const void* dy, int64_t dy_stride, const void* x, in
     BGX_REQUIRE(need == 0 || (ws != nullptr && ws_bytes >= need), BGX_E_WORKSPACE,
                 "layer norm backward: workspace of %zu bytes, %zu needed", ws_bytes, need);
   }
-  const int parts = params ? ln_grid(rows, ln_wpr(d), LN_PARTS_MAX) : 0;
+  const int parts = !params || rows == 0 ? 0 : ln_parts(rows, d);
   if (rows > 0) {
     NormArgs A{};
     A.x = x;
@@ -392,6 +406,9 @@ int layernorm_backward_impl(const void* dy, int64_t dy_stride, const void* x, in
     A.mean = const_cast<float*>(mean);
     A.rstd = const_cast<float*>(rstd);
     A.parts = (float*)ws;
+    A.dweight = dweight;
+    A.dbias = dbias;
+    A.wdtype = wdtype;
     A.rows = rows;
     A.x_stride = x_stride;
     A.dy_stride = dy_stride;
@@ -413,7 +430,7 @@ int layernorm_backward_impl(const void* dy, int64_t dy_stride, const void* x, in
 #undef BGX_LN_BACKWARD
     if (rc) return rc;
   }
-  if (params) {
+  if (params && parts != 1) {
     layernorm_params_kernel<<<dim3((d + LN_COLS - 1) / LN_COLS, 2), LN_COLS * LN_GROUPS, 0, s>>>((const float*)ws, parts, d, dweight, dbias, wdtype);
     BGX_HIP(hipGetLastError());
   }

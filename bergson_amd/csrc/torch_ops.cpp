@@ -123,7 +123,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     size_t nbytes = 0;
     if (want_w || want_b) {
       nbytes = bgx_layernorm_backward_workspace_bytes(n, (int32_t)d);
-      ws = at::empty({(int64_t)nbytes}, rows.options().dtype(at::kByte));
+      if (nbytes) ws = at::empty({(int64_t)nbytes}, rows.options().dtype(at::kByte));
     }
     const float* mean = stats.data_ptr<float>();
     check(bgx_layernorm_backward(ptr(dy), row_stride(dy), ptr(rows), row_stride(rows), ptr(weight),

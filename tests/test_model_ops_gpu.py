@@ -558,7 +558,8 @@ def test_differentiable_once(device, which):
 @pytest.mark.parametrize("rows", [128, 64, 32])
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
 def test_attention_gradients_that_cancel(device, bgx_env, dtype, rows):
-    """Sequences of one token: the softmax is constant, dq and dk are exactly 0 and dv is the sum over the heads."""
+    """Sequences of one token: the softmax is constant, dq and dk are exactly 0 and dv is the sum over the heads,
+    times a weight of 1."""
     bgx_env("BGX_ATTENTION_ROWS", rows)
     q, k, v, do = _qkv((40,), 4, 2, 64, dtype, 30, device)
     cu = torch.arange(41, dtype=torch.int32, device=device)
@@ -566,4 +567,9 @@ def test_attention_gradients_that_cancel(device, bgx_env, dtype, rows):
         t.requires_grad_()
     dq, dk, dv = torch.autograd.grad(B.causal_attention(q, k, v, cu_seqlens=cu), (q, k, v), do)
     assert (dq == 0).all() and (dk == 0).all()
-    assert torch.equal(dv, do.float().unflatten(1, (2, 2)).sum(2).to(dtype))
+    # the weight is 2^(s c - fl(s c)): off from 1 by the rounding of s c (c = scale log2 e) and of the exponential
+    wide = [t.detach().double().cpu() for t in (q, k.repeat_interleave(2, 1), do)]
+    score = (wide[0] * wide[1]).sum(2, keepdim=True).abs() * 0.125 * 1.4427
+    off = ((score + 4) * 2.0 ** -24 * wide[2].abs()).unflatten(1, (2, 2)).sum(2)
+    want = wide[2].unflatten(1, (2, 2)).sum(2)
+    assert_within(dv, want, off + torch.finfo(dtype).eps / 2 * (want.abs() + off), "dv")
