@@ -162,7 +162,7 @@ __global__ __launch_bounds__(THREADS) void distill_forward_kernel(DistillArgs A)
   }
 }
 
-template <typename T, int THREADS>
+template <typename T, int THREADS, bool STREAM>
 __global__ __launch_bounds__(THREADS) void distill_backward_kernel(DistillArgs A) {
   constexpr int EPL = Chunk<T>::N;
   __shared__ float slot[THREADS / WAVE];
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(THREADS) void distill_backward_kernel(DistillArgs A
       Chunk<T>::unpack(w[k], v);
 #pragma unroll
       for (int e = 0; e < EPL; ++e) v[e] = exp2_hw((v[e] - top) * c) * scale;
-      store_chunk_any(dz + (int64_t)(i + k * THREADS) * EPL, Chunk<T>::pack(v));
+      store_chunk<STREAM>(dz + (int64_t)(i + k * THREADS) * EPL, Chunk<T>::pack(v));
     }
   }
   for (; i < chunks; i += THREADS) {
@@ -241,11 +241,13 @@ static int distill_launch(const DistillArgs& A, bool backward, hipStream_t s) {
   const dim3 grid((unsigned)A.rows);
   if (A.rows < DISTILL_FEW) {
     if (backward)
-      distill_backward_kernel<T, 1024><<<grid, 1024, 0, s>>>(A);
+      distill_backward_kernel<T, 1024, false><<<grid, 1024, 0, s>>>(A);
     else
       distill_forward_kernel<T, 1024><<<grid, 1024, 0, s>>>(A);
+  } else if (backward && A.rows * A.V * (int64_t)sizeof(T) >= STREAM_BYTES) {
+    distill_backward_kernel<T, 256, true><<<grid, 256, 0, s>>>(A);
   } else if (backward) {
-    distill_backward_kernel<T, 256><<<grid, 256, 0, s>>>(A);
+    distill_backward_kernel<T, 256, false><<<grid, 256, 0, s>>>(A);
   } else {
     distill_forward_kernel<T, 256><<<grid, 256, 0, s>>>(A);
   }

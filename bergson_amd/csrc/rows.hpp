@@ -80,6 +80,21 @@ __device__ inline void store_chunk_any(T* p, const uint4& v) {
   *(global_ptr)(uintptr_t)p = raw4{v.x, v.y, v.z, v.w};
 }
 
+// The same, STREAM: past the caches.  For results of this many bytes or more: they do not fit the memory-side cache
+// (256 MB) beside what they were made from, whoever reads them next reads memory anyway, and lines that linger there
+// are written back under the next kernel's reads (measured on 4096 x 50304 bf16 logits: the forward pass after a
+// backward pass 102 -> 80 us, the backward pass itself 157 us either way).
+constexpr int64_t STREAM_BYTES = 128ll << 20;
+template <bool STREAM, typename T>
+__device__ inline void store_chunk(T* p, const uint4& v) {
+  if constexpr (STREAM) {
+    typedef __attribute__((address_space(1))) raw4_any<T>* global_ptr;
+    __builtin_nontemporal_store((raw4_any<T>)raw4{v.x, v.y, v.z, v.w}, (global_ptr)(uintptr_t)p);
+  } else {
+    store_chunk_any(p, v);
+  }
+}
+
 template <typename T>
 __device__ inline uint32_t load_bits(const T* p) {
   if constexpr (sizeof(T) == 4)
