@@ -53,6 +53,7 @@ class AttentionShape(C.Structure):
 
     _fields_ = [
         ("plan_dev", C.c_void_p),
+        ("cu_seqlens_dev", C.c_void_p),
         ("lengths_dev", C.c_void_p),
         ("rows", C.c_int64),
         ("n_seqs", C.c_int32),

@@ -46,6 +46,7 @@ struct AttnArgs {
   float* delta;           // [Hq][rows]
   float* peak;            // [Hq][rows]: largest |do| of the row (fp16 only)
   const int4* table;      // packed: {first row, length, tile, limit} per tile of rows, heaviest first
+  const int32_t* bounds;  // packed without a table: the sequences' boundaries
   const int32_t* lengths; // batch layout: [N] or NULL
   int64_t rows;           // N * S, or the packed rows
   int N, S, tiles;        // tiles: per sequence (batch layout) or entries (packed)
@@ -264,13 +265,64 @@ __device__ inline void spread_heads(int u, int streams, int group, int& stream, 
   }
 }
 
+// Boundaries of sequence n as any of its users takes them: clamped to the rows and to each other.
+__device__ inline int2 sequence_span(const int32_t* cu, int n, int rows) {
+  const int a = min(max(cu[n], 0), rows), b = min(max(cu[n + 1], a), rows);
+  return make_int2(a, b - a);
+}
+
+// Entry `entry` of the list of tiles, found by every wave from the boundaries themselves, one sequence a lane (at most
+// 64): sequences in order, a sequence's heaviest tile first, then what lies outside the sequences.
+constexpr int FIND_MAX = WAVE;
+template <int ROWS>
+__device__ inline bool find_item(const AttnArgs& A, bool keys, int entry, AttnItem& it) {
+  const int lane = threadIdx.x & (WAVE - 1), rows = (int)A.rows;
+  int2 span = make_int2(0, 0);
+  if (lane < A.N) span = sequence_span(A.bounds, lane, rows);
+  const int tiles = (span.y + ROWS - 1) / ROWS;
+  int upto = tiles;  // tiles of this and the earlier sequences
+#pragma unroll
+  for (int d = 1; d < WAVE; d <<= 1) {
+    const int below = __shfl_up(upto, d, WAVE);
+    if (lane >= d) upto += below;
+  }
+  const int total = __builtin_amdgcn_readlane(upto, WAVE - 1);
+  it.seq = 0;
+  if (entry < total) {
+    const int n = __popcll(__ballot(upto <= entry));
+    const int here = __builtin_amdgcn_readlane(tiles, n), at = entry - (__builtin_amdgcn_readlane(upto, n) - here);
+    it.row0 = it.stat = __builtin_amdgcn_readlane(span.x, n);
+    it.len = it.limit = __builtin_amdgcn_readlane(span.y, n);
+    it.tile = keys ? at : here - 1 - at;
+    return true;
+  }
+  const int first = A.N > 0 ? __builtin_amdgcn_readlane(span.x, 0) : 0;
+  const int last = A.N > 0 ? __builtin_amdgcn_readlane(span.x + span.y, A.N - 1) : 0;
+  const int head = (first + ROWS - 1) / ROWS;
+  it.len = 0;
+  it.tile = entry - total;
+  if (it.tile < head) {
+    it.row0 = it.stat = 0;
+    it.limit = first;
+  } else {
+    it.tile -= head;
+    it.row0 = it.stat = last;
+    it.limit = rows - last;
+  }
+  return it.tile * ROWS < it.limit;
+}
+
 // keys: the workgroup owns key rows (all query heads of one key/value head, first tile heaviest) instead of query rows
 // (one query head, last tile heaviest).
 template <int ROWS>
 __device__ inline bool attn_item(const AttnArgs& A, bool keys, AttnItem& it, int& kv_head, int& q_head) {
   const int group = keys ? 1 : A.group;
   int g;
-  if (A.table != nullptr) {
+  if (A.bounds != nullptr) {
+    const int per = A.Hk * group;
+    if (!find_item<ROWS>(A, keys, blockIdx.x / per, it)) return false;
+    spread_heads(blockIdx.x % per, A.Hk, group, kv_head, g);
+  } else if (A.table != nullptr) {
     const int per = A.Hk * group;
     const int4 e = A.table[blockIdx.x / per];
     if (e.w <= 0) return false;
@@ -901,11 +953,6 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
 // list is dropped, so that no boundaries lead out of bounds.
 constexpr int PLAN_THREADS = 1024;
 
-__device__ inline int2 plan_sequence(const int32_t* cu, int n, int rows) {
-  const int a = min(max(cu[n], 0), rows), b = min(max(cu[n + 1], a), rows);
-  return make_int2(a, b - a);
-}
-
 // sum of v over the threads from this one on
 __device__ inline int suffix_sum(int v, int* waves) {
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
@@ -917,8 +964,10 @@ __device__ inline int suffix_sum(int v, int* waves) {
   __syncthreads();
   if (lane == 0) waves[wave] = v;
   __syncthreads();
-  for (int w = wave + 1; w < PLAN_THREADS / WAVE; ++w) v += waves[w];
-  return v;
+  int later = lane > wave && lane < PLAN_THREADS / WAVE ? waves[lane] : 0;  // the waves after this one
+#pragma unroll
+  for (int d = 1; d < PLAN_THREADS / WAVE; d <<= 1) later += __shfl_xor(later, d, WAVE);
+  return v + __shfl(later, 0, WAVE);
 }
 
 __global__ __launch_bounds__(PLAN_THREADS) void attention_plan_kernel(const int32_t* __restrict__ cu, int N, int rows,
@@ -935,7 +984,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void attention_plan_kernel(const int3
   whole[threadIdx.x] = partial[threadIdx.x] = 0;
   __syncthreads();
   for (int n = threadIdx.x; n < N; n += PLAN_THREADS) {
-    const int tiles = tiles_of(plan_sequence(cu, n, rows).y);
+    const int tiles = tiles_of(sequence_span(cu, n, rows).y);
     if (tiles > 0) {
       atomicAdd(&whole[tiles >> fold], 1);  // levels below this one it fills, this one in part
       if (fold > 0) atomicAdd(&partial[tiles >> fold], tiles & ((1 << fold) - 1));
@@ -952,15 +1001,15 @@ __global__ __launch_bounds__(PLAN_THREADS) void attention_plan_kernel(const int3
   // within a level the order is whatever the counters hand out: it decides when a tile runs, not what it computes
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
   for (int n = wave; n < N; n += PLAN_THREADS / WAVE) {
-    const int2 s = plan_sequence(cu, n, rows);
+    const int2 s = sequence_span(cu, n, rows);
     for (int t = lane; t < tiles_of(s.y); t += WAVE) {
       const int at = atomicAdd(&cursor[t >> fold], 1);
       if ((unsigned)at < (unsigned)entries) table[at] = make_int4(s.x, s.y, t, s.y);
     }
   }
   // rows before the first and after the last sequence, then entries without work
-  const int head = N > 0 ? plan_sequence(cu, 0, rows).x : 0;
-  const int2 last = N > 0 ? plan_sequence(cu, N - 1, rows) : make_int2(0, 0);
+  const int head = N > 0 ? sequence_span(cu, 0, rows).x : 0;
+  const int2 last = N > 0 ? sequence_span(cu, N - 1, rows) : make_int2(0, 0);
   const int tail = last.x + last.y, head_tiles = tiles_of(head), clear = head_tiles + tiles_of(rows - tail);
   for (int at = total + (int)threadIdx.x; at < entries; at += PLAN_THREADS) {
     if (at < 0) break;
@@ -987,7 +1036,9 @@ static int attn_check(const bgx_attention_shape* a, const char* what) {
   BGX_REQUIRE(a->scale > 0.f && a->scale < INFINITY, BGX_E_ARG, "%s: scale %g must be positive and finite", what, a->scale);
   // tile bounds are formed in 32 bits
   BGX_REQUIRE(a->rows < (1ll << 31) - 4 * AT_TILES[0], BGX_E_SHAPE, "%s: %lld rows", what, (long long)a->rows);
-  if (a->plan_dev == nullptr)
+  BGX_REQUIRE(a->cu_seqlens_dev == nullptr || (a->plan_dev == nullptr && a->n_seqs <= FIND_MAX), BGX_E_ARG,
+              "%s: boundaries of %d sequences; up to %d go without a plan", what, a->n_seqs, FIND_MAX);
+  if (a->plan_dev == nullptr && a->cu_seqlens_dev == nullptr)
     BGX_REQUIRE(a->n_seqs == 0 ? a->rows == 0 : a->rows % a->n_seqs == 0, BGX_E_ARG,
                 "%s: %lld rows are not %d sequences of one width", what, (long long)a->rows, a->n_seqs);
   return 0;
@@ -995,17 +1046,18 @@ static int attn_check(const bgx_attention_shape* a, const char* what) {
 
 // tiles of the given height, over all sequences
 static int64_t attn_items(const bgx_attention_shape* a, int which) {
-  if (a->plan_dev != nullptr) return plan_entries(a->rows, a->n_seqs, which);
+  if (a->plan_dev != nullptr || a->cu_seqlens_dev != nullptr) return plan_entries(a->rows, a->n_seqs, which);
   const int64_t S = a->n_seqs ? a->rows / a->n_seqs : 0;
   return (S + AT_TILES[which] - 1) / AT_TILES[which] * a->n_seqs;
 }
 
 static AttnArgs attn_args(const bgx_attention_shape* a) {
   AttnArgs A{};
+  A.bounds = a->cu_seqlens_dev;
   A.lengths = a->lengths_dev;
   A.rows = a->rows;
   A.N = a->n_seqs;
-  A.S = a->plan_dev == nullptr && a->n_seqs ? (int)(a->rows / a->n_seqs) : 0;
+  A.S = a->plan_dev == nullptr && a->cu_seqlens_dev == nullptr && a->n_seqs ? (int)(a->rows / a->n_seqs) : 0;
   A.Hq = a->heads;
   A.Hk = a->kv_heads;
   A.group = a->heads / a->kv_heads;

@@ -543,7 +543,8 @@ int bgx_layernorm_backward(const void* dy_dev, int64_t dy_row_stride,
  * reads key/value head h / (heads / kv_heads).  Two layouts:
  *   batch   (plan_dev NULL): n_seqs sequences of rows / n_seqs positions each;
  *           lengths_dev [n_seqs] int32 or NULL cuts each to its first rows
- *   packed  (plan_dev from bgx_attention_plan): sequences back to back in
+ *   packed  (plan_dev from bgx_attention_plan, or cu_seqlens_dev itself for at
+ *           most 64 sequences; the other is NULL): sequences back to back in
  *           `rows` rows
  * Rows that belong to no sequence are not read; their outputs and gradients
  * are zero.  Operands: element strides between sequences (batch layout),
@@ -556,6 +557,7 @@ int bgx_layernorm_backward(const void* dy_dev, int64_t dy_row_stride,
  * and for 16-bit types what the rounding of out has cut off. */
 typedef struct bgx_attention_shape {
   const void* plan_dev;
+  const int32_t* cu_seqlens_dev;
   const int32_t* lengths_dev;
   int64_t rows;
   int32_t n_seqs;
@@ -576,7 +578,10 @@ typedef struct bgx_attention_rows {
 /* bgx_attention_plan turns the sequences' boundaries cu_seqlens_dev
  * [n_seqs + 1] int32 (device data, ascending, within 0..rows) into the list of
  * tiles the kernels walk, longest first: bgx_attention_plan_bytes(rows, n_seqs)
- * bytes, valid for every call with these boundaries.  Boundaries that are not
+ * bytes, valid for every call with these boundaries.  A call that is given
+ * cu_seqlens_dev instead needs no plan: every workgroup finds its tile itself,
+ * in the order of the sequences -- for one sequence, or when the call is too
+ * small for the order to matter.  Boundaries that are not
  * ascending or lie outside 0..rows are clamped: which rows then count is
  * unspecified, no access leaves the operands. */
 size_t bgx_attention_plan_bytes(int64_t rows, int32_t n_seqs);

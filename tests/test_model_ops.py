@@ -99,9 +99,9 @@ def test_topk_distillation_refusals():
 
 
 def test_struct_layouts_match_the_header():
-    # two pointers, int64, five int32, one float
-    assert C.sizeof(_lib.AttentionShape) == 2 * 8 + 8 + 5 * 4 + 4
-    assert _lib.AttentionShape.rows.offset == 16 and _lib.AttentionShape.scale.offset == 44
+    # three pointers, int64, five int32, one float
+    assert C.sizeof(_lib.AttentionShape) == 3 * 8 + 8 + 5 * 4 + 4
+    assert _lib.AttentionShape.rows.offset == 24 and _lib.AttentionShape.scale.offset == 52
     assert C.sizeof(_lib.AttentionRows) == 4 * 8
 
 
@@ -130,7 +130,7 @@ def test_c_abi_refusals():
     assert lib.bgx_layernorm_backward_workspace_bytes(4, 1 << 20) == 0
 
     def shape(**kw):
-        s = _lib.AttentionShape(None, None, 10, 2, 4, 2, 16, 2, 0.25)
+        s = _lib.AttentionShape(None, None, None, 10, 2, 4, 2, 16, 2, 0.25)
         for name, value in kw.items():
             setattr(s, name, value)
         return C.byref(s)
@@ -151,6 +151,8 @@ def test_c_abi_refusals():
     assert fwd(shape(rows=11)) == -1 and b"one width" in lib.bgx_last_error()
     assert fwd(shape(rows=1 << 31)) == -3
     assert fwd(shape(rows=0, n_seqs=0)) == 0
+    assert fwd(shape(cu_seqlens_dev=256, n_seqs=65)) == -1 and b"65 sequences" in lib.bgx_last_error()
+    assert fwd(shape(cu_seqlens_dev=256, plan_dev=256)) == -1
     bwd = lambda s, saved=P, ws=P, nbytes=1 << 20: lib.bgx_attention_backward(
         s, rows, rows, rows, rows, saved, rows, rows, rows, rows, ws, nbytes, None)
     assert bwd(shape(), saved=None) == -1 and b"saved" in lib.bgx_last_error()

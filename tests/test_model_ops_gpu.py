@@ -311,6 +311,40 @@ def test_attention_malformed_boundaries_stay_in_bounds(device):
     assert torch.equal(B.causal_attention(q, k, v, cu_seqlens=cu), B.causal_attention(q[None], k[None], v[None])[0])
 
 
+@pytest.mark.parametrize("rows", [128, 64, 32])
+@pytest.mark.parametrize("cu", [[0, 150], [20, 150, 150, 300], [0] * 40 + [300], [300, 300], [0], [0, 7, 14, 200, 299]],
+                         ids=lambda c: f"{len(c) - 1}:{c[0]}-{c[-1]}")
+def test_attention_plan_or_none(device, bgx_env, cu, rows):
+    """The C ABI with a plan and with the boundaries themselves: the same bits, forward and backward, whatever lies
+    outside the sequences; and again after 64 sequences, where only the plan is taken."""
+    from bergson_amd import _lib
+
+    bgx_env("BGX_ATTENTION_ROWS", rows)
+    lib, P = _lib.load(), lambda t: t.data_ptr()
+    q, k, v, do = _qkv((300,), 2, 1, 64, torch.bfloat16, 5, device)
+    bounds = torch.tensor(cu, dtype=torch.int32, device=device)
+    nbytes = lib.bgx_attention_plan_bytes(300, len(cu) - 1)
+    plan = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    stream = torch.cuda.current_stream().cuda_stream
+    _lib.check(lib.bgx_attention_plan(P(bounds), len(cu) - 1, 300, P(plan), nbytes, stream), "plan")
+    results = []
+    for with_plan in (True, False):
+        shape = _lib.AttentionShape(P(plan) if with_plan else None, None if with_plan else P(bounds), None, 300, len(cu) - 1,
+                                    2, 1, 64, _lib.BGX_BF16, 0.125)
+        rows_of = lambda t: _lib.AttentionRows(P(t), 0, t.stride(0), t.stride(1))
+        out = [torch.full_like(t, float("nan")) for t in (q, q, k, v)]
+        saved = torch.empty(lib.bgx_attention_saved_bytes(shape), dtype=torch.uint8, device=device)
+        ws = torch.empty(lib.bgx_attention_backward_workspace_bytes(shape), dtype=torch.uint8, device=device)
+        args = [rows_of(t) for t in (q, k, v)]
+        _lib.check(lib.bgx_attention_forward(shape, *args, rows_of(out[0]), P(saved), stream), "forward")
+        _lib.check(lib.bgx_attention_backward(shape, *args, rows_of(out[0]), P(saved), rows_of(do),
+                                              *(rows_of(t) for t in out[1:]), P(ws), ws.numel(), stream), "backward")
+        results.append(out)
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    _check_sequences(q, k, v, do, results[0][0], results[0][1:], list(zip(cu, cu[1:])), 0.125, torch.bfloat16)
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
 @pytest.mark.parametrize("N,heads,kv_heads", [(34, 8, 4), (140, 4, 4)], ids=str)
 def test_attention_sizes_by_rule(device, N, heads, kv_heads, dtype):
