@@ -45,6 +45,8 @@ struct AttnArgs {
   void* rest;             // [rows][Hq][D], 16-bit types: o minus its rounded value, rounded
   float* delta;           // [Hq][rows]
   float* peak;            // [Hq][rows]: largest |do| of the row (fp16 only)
+  float* part_k;          // [rows][Hq][D]: dk and dv of every query head by itself (attention_backward_join_kernel),
+  float* part_v;          // NULL where a workgroup sums over the heads that share its keys
   const int4* table;      // packed: {first row, length, tile, limit} per tile of rows, heaviest first
   const int32_t* bounds;  // packed without a table: the sequences' boundaries
   const int32_t* lengths; // batch layout: [N] or NULL
@@ -312,11 +314,11 @@ __device__ inline bool find_item(const AttnArgs& A, bool keys, int entry, AttnIt
   return it.tile * ROWS < it.limit;
 }
 
-// keys: the workgroup owns key rows (all query heads of one key/value head, first tile heaviest) instead of query rows
-// (one query head, last tile heaviest).
+// keys: the workgroup owns key rows (of one key/value head for all its query heads, or for one of them; first tile
+// heaviest) instead of query rows (one query head, last tile heaviest).
 template <int ROWS>
 __device__ inline bool attn_item(const AttnArgs& A, bool keys, AttnItem& it, int& kv_head, int& q_head) {
-  const int group = keys ? 1 : A.group;
+  const int group = keys && A.part_k == nullptr ? 1 : A.group;
   int g;
   if (A.bounds != nullptr) {
     const int per = A.Hk * group;
@@ -417,11 +419,12 @@ __device__ inline T* attn_row(const AttnView& v, const AttnItem& it, int head, i
   return const_cast<T*>(attn_rows<T>(v, it, head)) + row * v.tok;
 }
 
-// first-operand fragments of one row kept in registers: row `row` of `rows` from `base` (zeros past the end)
-template <typename T, int DP>
+// first-operand fragments of one row kept in registers: row `row` of the workgroup's ROWS from `base`, of which `rows`
+// exist (zeros past the end).  A buffer spans the workgroup's rows, never the sequence: its size is a 32-bit number.
+template <typename T, int DP, int ROWS>
 __device__ inline void load_own(const T* base, int64_t tok, int row, int rows, int D, int lane, uint4 (&f)[DP / (2 * Attn<T>::EPL)]) {
   constexpr int EPL = Attn<T>::EPL;
-  const __amdgpu_buffer_rsrc_t r = row_buffer(base, tok, rows, D);
+  const __amdgpu_buffer_rsrc_t r = row_buffer(base, tok, min(rows, ROWS), D);
 #pragma unroll
   for (int ks = 0; ks < DP / (2 * EPL); ++ks) {
     const int col = (2 * ks + (lane >> 5)) * EPL;
@@ -452,7 +455,7 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
   const T* k = attn_rows<T>(A.k, it, kvh);
   const T* v = attn_rows<T>(A.v, it, kvh);
   uint4 qf[KS];
-  load_own<T, DP>(q + first * A.q.tok, A.q.tok, row - first, it.len - first, A.D, lane, qf);
+  load_own<T, DP, W::ROWS>(q + first * A.q.tok, A.q.tok, row - first, it.len - first, A.D, lane, qf);
   f32x16 o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -610,13 +613,13 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
   const T* v = attn_rows<T>(A.v, it, kvh);
   uint4 qf[KS], gf[KS];
   const int own = row - first, left = it.len - first;
-  load_own<T, DP>(attn_rows<T>(A.grad_o, it, qh) + first * A.grad_o.tok, A.grad_o.tok, own, left, A.D, lane, gf);
+  load_own<T, DP, W::ROWS>(attn_rows<T>(A.grad_o, it, qh) + first * A.grad_o.tok, A.grad_o.tok, own, left, A.D, lane, gf);
   float delta = 0.f, peak = 0.f;
   {
-    load_own<T, DP>(attn_rows<T>(A.o, it, qh) + first * A.o.tok, A.o.tok, own, left, A.D, lane, qf);
+    load_own<T, DP, W::ROWS>(attn_rows<T>(A.o, it, qh) + first * A.o.tok, A.o.tok, own, left, A.D, lane, qf);
     uint4 rf[KS];
     if constexpr (sizeof(T) == 2)
-      load_own<T, DP>((const T*)A.rest + ((it.stat + first) * A.Hq + qh) * A.D, (int64_t)A.Hq * A.D, own, left, A.D, lane, rf);
+      load_own<T, DP, W::ROWS>((const T*)A.rest + ((it.stat + first) * A.Hq + qh) * A.D, (int64_t)A.Hq * A.D, own, left, A.D, lane, rf);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       float a[M::EPL], b[M::EPL];
@@ -638,7 +641,7 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
     delta = d.x + d.y;
     peak = fmaxf(p.x, p.y);
   }
-  load_own<T, DP>(attn_rows<T>(A.q, it, qh) + first * A.q.tok, A.q.tok, own, left, A.D, lane, qf);
+  load_own<T, DP, W::ROWS>(attn_rows<T>(A.q, it, qh) + first * A.q.tok, A.q.tok, own, left, A.D, lane, qf);
   const int64_t stat = (int64_t)qh * A.rows + it.stat + row;
   if (in && half == 0 && part == 0) {
     A.delta[stat] = delta;
@@ -756,11 +759,19 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
   const int part = wave / RW;  // which of the waves that share rows
   const int first = it.tile * W::ROWS, mine = first + (wave % RW) * 32, row = mine + (lane & 31), half = lane >> 5;
-  if (first >= it.len) {
-    if (row < it.limit) {
+  const bool alone = A.part_k != nullptr;  // one query head of the group
+  const int64_t part_row = ((it.stat + row) * A.Hq + qh0) * A.D;
+  auto clear = [&]() {
+    if (alone) {
+      zero_row<float, DP>(A.part_k + part_row, A.D, lane);
+      zero_row<float, DP>(A.part_v + part_row, A.D, lane);
+    } else {
       zero_row<T, DP>(attn_row<T>(A.dk, it, kvh, row), A.D, lane);
       zero_row<T, DP>(attn_row<T>(A.dv, it, kvh, row), A.D, lane);
     }
+  };
+  if (first >= it.len) {
+    if (row < it.limit) clear();
     return;
   }
   const bool in = row < it.len;
@@ -777,8 +788,8 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
     once.load(v, A.v.tok, left, A.D);
     once.store(keep + KEEP);
   } else {
-    load_own<T, DP>(k, A.k.tok, own, left, A.D, lane, kf);
-    load_own<T, DP>(v, A.v.tok, own, left, A.D, lane, vf);
+    load_own<T, DP, W::ROWS>(k, A.k.tok, own, left, A.D, lane, kf);
+    load_own<T, DP, W::ROWS>(v, A.v.tok, own, left, A.D, lane, vf);
   }
   f32x16 dk[DT], dv[DT];
 #pragma unroll
@@ -786,7 +797,7 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
 #pragma unroll
     for (int i = 0; i < 16; ++i) dk[dt][i] = dv[dt][i] = 0.f;
   const float c = A.scale * AT_LOG2E;
-  const int t0 = first / BQ, per_head = (it.len + BQ - 1) / BQ - t0, n_tiles = per_head * A.group;
+  const int t0 = first / BQ, per_head = (it.len + BQ - 1) / BQ - t0, n_tiles = alone ? per_head : per_head * A.group;
   Staged<T, DP, BQ, W::THREADS> sq, sg;
   float stage[4];
   // tile t is tile t % per_head of the queries, for query head t / per_head of the group
@@ -936,14 +947,42 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
   join_waves<W, DT>(dk, lds, part, wave % RW, lane);
   join_waves<W, DT>(dv, lds, part, wave % RW, lane);
   if (part > 0) return;
-  T* out_k = attn_row<T>(A.dk, it, kvh, row);
-  T* out_v = attn_row<T>(A.dv, it, kvh, row);
-  store_rows<T, DP>(out_k, nullptr, dk, A.scale * exp2_of(-(float)lift), in, A.D, lane);
-  store_rows<T, DP>(out_v, nullptr, dv, 1.0f, in, A.D, lane);
-  if (!in && row < it.limit) {
-    zero_row<T, DP>(out_k, A.D, lane);
-    zero_row<T, DP>(out_v, A.D, lane);
+  const float scale = A.scale * exp2_of(-(float)lift);
+  if (alone) {
+    store_rows<float, DP>(A.part_k + part_row, nullptr, dk, scale, in, A.D, lane);
+    store_rows<float, DP>(A.part_v + part_row, nullptr, dv, 1.0f, in, A.D, lane);
+  } else {
+    store_rows<T, DP>(attn_row<T>(A.dk, it, kvh, row), nullptr, dk, scale, in, A.D, lane);
+    store_rows<T, DP>(attn_row<T>(A.dv, it, kvh, row), nullptr, dv, 1.0f, in, A.D, lane);
   }
+  if (!in && row < it.limit) clear();
+}
+
+// dk and dv of every key/value head: the sums over its query heads in their order, rounded once.  One thread per 16
+// bytes of the fp32 parts; grid.y = 0: dk, 1: dv.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_backward_join_kernel(AttnArgs A) {
+  const int pieces = A.D / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= A.rows * A.Hk * pieces) return;
+  const int d = (int)(i % pieces) * 4, head = (int)(i / pieces % A.Hk);
+  const int64_t row = i / pieces / A.Hk;
+  const float* part = (blockIdx.y == 0 ? A.part_k : A.part_v) + (row * A.Hq + (int64_t)head * A.group) * A.D + d;
+  float4 s = *reinterpret_cast<const float4*>(part);
+  for (int g = 1; g < A.group; ++g) {
+    const float4 v = *reinterpret_cast<const float4*>(part + (int64_t)g * A.D);
+    s.x += v.x;
+    s.y += v.y;
+    s.z += v.z;
+    s.w += v.w;
+  }
+  const AttnView& view = blockIdx.y == 0 ? A.dk : A.dv;
+  const int64_t seq = A.S > 0 ? row / A.S : 0, at = A.S > 0 ? row % A.S : row;
+  T* out = (T*)const_cast<void*>(view.p) + seq * view.seq + at * view.tok + head * view.head + d;
+  store_as(out, 0, s.x, Elem<T>::code);
+  store_as(out, 1, s.y, Elem<T>::code);
+  store_as(out, 2, s.z, Elem<T>::code);
+  store_as(out, 3, s.w, Elem<T>::code);
 }
 
 // ---- packed sequences: the list of tiles -------------------------------------------------------------------------
@@ -1072,18 +1111,20 @@ static AttnArgs attn_args(const bgx_attention_shape* a) {
 // earlier.  Measured (us, 128 / 64 / 32 rows): bf16, heads of 64, forward of 1 x 512 positions, 12 heads (48
 // workgroups) 11.7 / 10.3 / 8.4, 2 x 1024 (192) 18.8 / 17.3 / 17.8, 4 x 1024 (384) 21.1 / 18.5 / 27.8, 6 x 1024 (576)
 // 23.3 / 24.6 / 41.4; heads of 128, 8 heads, 1 x 2048 (128) 50.0 / 48.0 / 42.1, 32 heads, 1 x 1024 (256)
-// 29.3 / 33.8 / 52.1; its dq 40.5 / 38.5 / 59.4; dk and dv of 1 x 4096, 8 key/value heads (256) 519 / 470 / 545; fp32, heads
-// of 64, forward of 6 x 1024 (576) 125 / 107 / 121; dk and dv of fp32 heads of 128 spill at 128 rows (2653 / 1201 / 2510).
+// 29.3 / 33.8 / 52.1; dk and dv of 8 x 256, 16 heads (256) 17.2 / 23.2 / 40.9, 2 x 1024, 12 heads (192) 40.8 / 37.8 / 50.2;
+// fp32, heads of 64, forward of 6 x 1024 (576) 125 / 107 / 121.  dk and dv of wide fp32 heads need more registers than there
+// are with 128 rows (2 x 2048, 8 key/value heads: 2653 / 1201 / 2510) and have no such variant.
 enum AttnKernel { ATTN_FORWARD, ATTN_Q, ATTN_KV };
 static unsigned attn_grid(AttnArgs& A, const bgx_attention_shape* a, AttnKernel kernel, int* which) {
-  const int heads = kernel == ATTN_KV ? a->kv_heads : a->heads;
+  const int heads = kernel == ATTN_KV && A.part_k == nullptr ? a->kv_heads : a->heads;
   const int64_t tall = attn_items(a, 0) * heads;
   const bool wide = a->head_dim > 64, full = a->dtype == BGX_F32;
   const int64_t many = full ? (!wide ? 1024 : kernel == ATTN_KV ? INT64_MAX : 512)
-                            : (!wide ? 512 : kernel == ATTN_FORWARD ? 160 : kernel == ATTN_Q ? 256 : 384);
+                            : (!wide ? 512 : kernel == ATTN_FORWARD ? 160 : 256);
   *which = tall >= many ? 0 : tall >= 160 ? 1 : 2;
   for (int i = 0; i < 3; ++i)
     if (switches().attention_rows == AT_TILES[i]) *which = i;
+  if (kernel == ATTN_KV && wide && full && *which == 0) *which = 1;
   const int64_t grid = attn_items(a, *which) * heads;
   if (a->plan_dev != nullptr) {
     A.table = (const int4*)a->plan_dev;
@@ -1113,23 +1154,36 @@ static AttnView attn_view(const bgx_attention_rows* t) {
   return v;
 }
 
+// the tallest variant of each kernel and its threads
+template <typename T, int DP>
+constexpr int attention_forward_kernel_tall() {
+  return 4;
+}
 template <typename T, int DP>
 constexpr int attention_forward_kernel_threads() {
   return AT_THREADS;
+}
+template <typename T, int DP>
+constexpr int attention_backward_q_kernel_tall() {
+  return 4;
 }
 template <typename T, int DP>
 constexpr int attention_backward_q_kernel_threads() {
   return AT_THREADS;
 }
 template <typename T, int DP>
+constexpr int attention_backward_kv_kernel_tall() {
+  return sizeof(T) == 4 && DP > 64 ? 2 : 4;
+}
+template <typename T, int DP>
 constexpr int attention_backward_kv_kernel_threads() {
-  return kv_waves<T, DP, 4>() * WAVE;
+  return kv_waves<T, DP, attention_backward_kv_kernel_tall<T, DP>()>() * WAVE;
 }
 
 #define BGX_ATTN_ROWS(KERNEL, T, DP, WHICH, GRID, S, A)                    \
   do {                                                                     \
     if ((WHICH) == 0)                                                      \
-      KERNEL<T, DP, 4><<<(GRID), KERNEL##_threads<T, DP>(), 0, (S)>>>(A);  \
+      KERNEL<T, DP, KERNEL##_tall<T, DP>()><<<(GRID), KERNEL##_threads<T, DP>(), 0, (S)>>>(A); \
     else if ((WHICH) == 1)                                                 \
       KERNEL<T, DP, 2><<<(GRID), AT_THREADS, 0, (S)>>>(A);                 \
     else                                                                   \
@@ -1212,9 +1266,24 @@ int attention_forward_impl(const bgx_attention_shape* a, const bgx_attention_row
   return 0;
 }
 
+// Where few key/value heads and rows leave too few workgroups that walk all query heads of a group one after the
+// other, every query head gets workgroups of its own and the heads' parts are added by a kernel behind: 8 bytes of
+// parts per query element, written and read once.
+constexpr int64_t ATTN_PARTS_MAX = 512ll << 20;
+static int64_t attn_part_bytes(const bgx_attention_shape* a) {
+  if (a->kv_heads < 1 || a->heads <= a->kv_heads || attn_items(a, 0) * a->kv_heads >= 384) return 0;
+  const int64_t bytes = a->rows * a->heads * a->head_dim * (int64_t)sizeof(float) * 2;
+  return bytes <= ATTN_PARTS_MAX ? bytes : 0;
+}
+
+static int64_t attn_stat_bytes(const bgx_attention_shape* a) {
+  const int64_t n = a->rows * a->heads * (int64_t)sizeof(float) * (a->dtype == BGX_F16 ? 2 : 1);
+  return (n + 15) / 16 * 16;
+}
+
 size_t attention_backward_workspace_bytes(const bgx_attention_shape* a) {
   if (a == nullptr || a->rows <= 0 || a->heads <= 0) return 0;
-  return (size_t)a->rows * a->heads * sizeof(float) * (a->dtype == BGX_F16 ? 2 : 1);
+  return (size_t)(attn_stat_bytes(a) + attn_part_bytes(a));
 }
 
 int attention_backward_impl(const bgx_attention_shape* a, const bgx_attention_rows* q, const bgx_attention_rows* k,
@@ -1241,13 +1310,30 @@ int attention_backward_impl(const bgx_attention_shape* a, const bgx_attention_ro
   attn_saved(A, a, const_cast<void*>(saved));
   A.delta = (float*)ws;
   A.peak = A.delta + a->rows * a->heads;
+  BGX_REQUIRE((uintptr_t)ws % 16 == 0, BGX_E_ALIGN, "attention backward: workspace not aligned to 16 bytes");
   hipStream_t s = (hipStream_t)stream;
   int which;
   unsigned grid = attn_grid(A, a, ATTN_Q, &which);
   BGX_REQUIRE(grid > 0, BGX_E_SHAPE, "attention backward: %lld rows of %d heads", (long long)a->rows, a->heads);
   BGX_ATTN_LAUNCH(attention_backward_q_kernel, a->dtype, a->head_dim, which, grid, s, A);
+  const int64_t parts = attn_part_bytes(a);
+  if (parts > 0) {
+    A.part_k = (float*)((char*)ws + attn_stat_bytes(a));
+    A.part_v = A.part_k + parts / 2 / (int64_t)sizeof(float);
+  }
   grid = attn_grid(A, a, ATTN_KV, &which);
+  BGX_REQUIRE(grid > 0, BGX_E_SHAPE, "attention backward: %lld rows of %d heads", (long long)a->rows, a->heads);
   BGX_ATTN_LAUNCH(attention_backward_kv_kernel, a->dtype, a->head_dim, which, grid, s, A);
+  if (parts > 0) {
+    const dim3 join((unsigned)((a->rows * a->kv_heads * (a->head_dim / 4) + 255) / 256), 2);
+    if (a->dtype == BGX_F32)
+      attention_backward_join_kernel<float><<<join, 256, 0, s>>>(A);
+    else if (a->dtype == BGX_F16)
+      attention_backward_join_kernel<f16_t><<<join, 256, 0, s>>>(A);
+    else
+      attention_backward_join_kernel<bf16_t><<<join, 256, 0, s>>>(A);
+    BGX_HIP(hipGetLastError());
+  }
   return 0;
 }
 

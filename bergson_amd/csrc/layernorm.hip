@@ -152,11 +152,13 @@ __global__ __launch_bounds__(LN_WAVES* WAVE) void layernorm_forward_kernel(NormA
 
 // PARAMS: the workgroup also sums dy xh and dy over its rows, column by column in registers (a lane keeps the same
 // columns for every row), adds its waves' sums through LDS in a fixed order and writes one row of partial sums.  The
-// next row's x and dy are on their way while a row is worked on.
+// next row's x and dy are on their way while a row is worked on (AHEAD; with 64 elements a lane there are no registers
+// for it).
 template <typename T, typename WT, int NE, int WPR, int MODE, bool PARAMS>
 __global__ __launch_bounds__(LN_WAVES* WAVE) void layernorm_backward_kernel(NormArgs A) {
   using Row = LnRow<T, NE, WPR, MODE>;
   constexpr int EPL = Row::EPL, NC = Row::NC;
+  constexpr bool AHEAD = NE < 64;
   __shared__ float2 slot[2][LN_WAVES];
   __shared__ float colsum[PARAMS && WPR == 1 ? WAVE * NE : 1];
   int turn = 0;
@@ -184,8 +186,9 @@ __global__ __launch_bounds__(LN_WAVES* WAVE) void layernorm_backward_kernel(Norm
     rstd = A.rstd[r];
   };
   int64_t r = (int64_t)blockIdx.x * (LN_WAVES / WPR) + (WPR == 1 ? wave : 0);
-  if (r < A.rows) fetch(r);
+  if (AHEAD && r < A.rows) fetch(r);
   for (; r < A.rows; r += step) {
+    if constexpr (!AHEAD) fetch(r);
     float x[NE], h[NE];
     float2 s = make_float2(0.f, 0.f);  // sums of h and of h xh
     const float m = mean, f = rstd;
@@ -194,7 +197,7 @@ __global__ __launch_bounds__(LN_WAVES* WAVE) void layernorm_backward_kernel(Norm
       Chunk<T>::unpack(xv[c], x + c * EPL);
       Chunk<T>::unpack(gv[c], h + c * EPL);
     }
-    fetch(r + step < A.rows ? r + step : r);
+    if constexpr (AHEAD) fetch(r + step < A.rows ? r + step : r);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       float w[EPL];

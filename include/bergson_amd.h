@@ -514,7 +514,8 @@ int bgx_gram_accumulate(const void* rows_dev, int32_t dtype, int64_t row_stride,
  * (bergson/collector/collector.py:926-985 runs the model's forward pass, a
  * loss and its backward pass): the norms, the attention, the loss.  All sums
  * and statistics are fp32.  The entry points allocate nothing, keep nothing
- * between calls and may be captured into a HIP graph.
+ * between calls and may be captured into a HIP graph.  Outputs overlap neither
+ * inputs nor each other.
  *
  * bgx_layernorm_forward: y[r] = (x[r] - mean) * rstd * weight + bias over rows
  *   of d <= 16384 elements; rows start at any element (strides in elements,

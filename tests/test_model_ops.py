@@ -157,7 +157,12 @@ def test_c_abi_refusals():
         s, rows, rows, rows, rows, saved, rows, rows, rows, rows, ws, nbytes, None)
     assert bwd(shape(), saved=None) == -1 and b"saved" in lib.bgx_last_error()
     assert bwd(shape(), ws=None) == -4 and bwd(shape(), nbytes=16) == -4
-    assert lib.bgx_attention_backward_workspace_bytes(shape()) == 10 * 4 * 4
+    # delta per head and row, and with shared heads and few workgroups fp32 parts of dk and dv per query head
+    assert lib.bgx_attention_backward_workspace_bytes(shape()) == 10 * 4 * 4 + 2 * 10 * 4 * 16 * 4
+    assert lib.bgx_attention_backward_workspace_bytes(shape(kv_heads=4)) == 10 * 4 * 4
+    assert lib.bgx_attention_backward_workspace_bytes(shape(kv_heads=4, dtype=1)) == 2 * 10 * 4 * 4
+    assert lib.bgx_attention_backward_workspace_bytes(shape(rows=2 * 128 * 96)) == 2 * 128 * 96 * 4 * 4
+    assert bwd(shape(), ws=C.c_void_p(264)) == -5
     # two statistics per head and row; at 16 bits also what the output's rounding cuts off
     assert lib.bgx_attention_saved_bytes(shape()) == 10 * 4 * (2 * 4 + 16 * 2)
     assert lib.bgx_attention_saved_bytes(shape(dtype=0)) == 10 * 4 * 2 * 4

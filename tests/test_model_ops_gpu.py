@@ -283,6 +283,26 @@ def test_attention_small_gradients_in_fp16(device, bgx_env, rows):
     _check_sequences(q, k, v, do, B.causal_attention(q, k, v, cu_seqlens=cu), grads, [(0, 260)], 0.125, torch.float16)
 
 
+@pytest.mark.parametrize("rows", [128, 32])
+def test_attention_offsets_past_32_bits(device, bgx_env, rows):
+    """Positions 2 MiB apart: the sequence spans more than 4 GiB of each operand, a tile far less."""
+    bgx_env("BGX_ATTENTION_ROWS", rows)
+    T, far = 2600, 1 << 20
+    store = [torch.empty(T * far, dtype=torch.bfloat16, device=device) for _ in range(3)]
+    views = [torch.as_strided(t, (T, 1, 64), (far, 64, 1)) for t in store]
+    plain = _qkv((T,), 1, 1, 64, torch.bfloat16, 3, device)
+    for view, t in zip(views, plain):
+        view.copy_(t)
+        view.requires_grad_()
+    cu = torch.tensor([0, T], dtype=torch.int32, device=device)
+    out = B.causal_attention(*views, cu_seqlens=cu)
+    leaves = [t.clone().requires_grad_() for t in plain[:3]]
+    want = B.causal_attention(*leaves, cu_seqlens=cu)
+    assert torch.equal(out, want)
+    for a, b in zip(torch.autograd.grad(out, views, plain[3]), torch.autograd.grad(want, leaves, plain[3])):
+        assert torch.equal(a, b)
+
+
 def test_attention_plan_of_many_sequences(device):
     """More sequences than the planning workgroup has threads, empty ones among them, long ones at the end."""
     g = _gen(2)
@@ -346,10 +366,10 @@ def test_attention_plan_or_none(device, bgx_env, cu, rows):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
-@pytest.mark.parametrize("N,heads,kv_heads", [(34, 8, 4), (140, 4, 4)], ids=str)
+@pytest.mark.parametrize("N,heads,kv_heads", [(34, 8, 4), (140, 8, 4)], ids=str)
 def test_attention_sizes_by_rule(device, N, heads, kv_heads, dtype):
     """Enough sequences and heads that the workgroup sizes follow from the rule: 64 rows in the first case, 128 in the
-    second; heads of 128 and 64."""
+    second, where a workgroup also sums dk and dv over the heads that share its keys; heads of 128 and 64."""
     g = _gen(N)
     for dim in (128, 64):
         lengths = torch.randint(0, 160, (N,), generator=g).tolist()
