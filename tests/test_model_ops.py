@@ -118,14 +118,15 @@ def test_c_abi_refusals():
     assert norm(xs=7) == -1 and b"stride" in lib.bgx_last_error()
     assert norm(mean=P) == -1
     assert norm(rows=0, x=None) == 0
-    back = lambda ws=P, nbytes=1 << 20, dx=P, dw=P, rows=20, d=8, mean=P: lib.bgx_layernorm_backward(
+    back = lambda ws=P, nbytes=1 << 20, dx=P, dw=P, rows=5000, d=8, mean=P: lib.bgx_layernorm_backward(
         P, 8, P, 8, P, 2, mean, P, rows, d, 2, dx, 8, dw, None, ws, nbytes, None)
     assert back(ws=None, nbytes=0) == -4 and b"workspace" in lib.bgx_last_error()
     assert back(nbytes=8) == -4
     assert back(mean=None) == -1
     assert back(dx=None, dw=None) == 0     # nothing asked for
-    assert lib.bgx_layernorm_backward_workspace_bytes(20, 8) == 5 * 2 * 8 * 4    # four rows a workgroup
-    assert lib.bgx_layernorm_backward_workspace_bytes(16, 8) == 0                # one workgroup: no partial sums
+    assert lib.bgx_layernorm_backward_workspace_bytes(5000, 8) == 512 * 2 * 8 * 4   # a row of partial sums a workgroup
+    assert lib.bgx_layernorm_backward_workspace_bytes(20, 7) == 5 * 2 * 7 * 4       # four rows a workgroup
+    assert lib.bgx_layernorm_backward_workspace_bytes(1024, 8) == 0                 # few rows: no partial sums
     assert lib.bgx_layernorm_backward_workspace_bytes(0, 8) == 0
     assert lib.bgx_layernorm_backward_workspace_bytes(4, 1 << 20) == 0
 

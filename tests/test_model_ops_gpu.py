@@ -31,7 +31,7 @@ def _norm_case(rows, d, dtype, w_dtype, seed, device):
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
 @pytest.mark.parametrize("rows,d", [(1, 1), (1, 768), (3, 7), (5, 64), (37, 129), (66, 511), (9, 512), (4, 513),
                                     (130, 1001), (7, 2047), (6, 2049), (5, 4096), (3, 5001), (2, 8193), (2, 16384),
-                                    (2100, 40)], ids=str)
+                                    (2100, 40), (4097, 40), (4500, 1001), (4100, 2050), (4099, 5), (1024, 16), (1025, 16)], ids=str)
 def test_layer_norm(device, rows, d, dtype):
     x, w, b, dy = _norm_case(rows, d, dtype, dtype, rows * 31 + d, device)
     for t in (x, w, b):
@@ -47,9 +47,9 @@ def test_layer_norm(device, rows, d, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=ids_of)
-@pytest.mark.parametrize("d", [96, 1500, 5000])
-def test_layer_norm_fp32_weights(device, dtype, d):
-    x, w, b, dy = _norm_case(21, d, dtype, torch.float32, d, device)
+@pytest.mark.parametrize("rows,d", [(21, 96), (21, 1500), (21, 5000), (1100, 97)])
+def test_layer_norm_fp32_weights(device, dtype, rows, d):
+    x, w, b, dy = _norm_case(rows, d, dtype, torch.float32, d, device)
     for t in (x, w, b):
         t.requires_grad_()
     y = B.layer_norm(x, w, b, 1e-3)
@@ -59,9 +59,10 @@ def test_layer_norm_fp32_weights(device, dtype, d):
         assert_within(got, *ref[name], name)
 
 
-def test_layer_norm_subsets_of_gradients(device):
+@pytest.mark.parametrize("rows", [70, 1100])
+def test_layer_norm_subsets_of_gradients(device, rows):
     """Frozen weights (a collection run), no bias, frozen input: each gradient equals the one of the full call."""
-    x, w, b, dy = _norm_case(70, 300, torch.bfloat16, torch.bfloat16, 5, device)
+    x, w, b, dy = _norm_case(rows, 300, torch.bfloat16, torch.bfloat16, 5, device)
     full = [t.clone().requires_grad_() for t in (x, w, b)]
     want = torch.autograd.grad(B.layer_norm(*full), full, dy)
     for need in ((True, False, False), (False, True, False), (False, False, True), (False, True, True), (True, True, False)):
