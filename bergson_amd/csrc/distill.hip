@@ -8,6 +8,10 @@
 // end), the backward pass reads them once and writes their gradient; the K entries are a few hundred bytes.  The
 // forward pass keeps a row's maximum and sum of exponentials apart rather than as one logarithm: a gradient then
 // carries the rounding of z - max, not that of a logarithm of the size of the logits.  All sums in fp32.
+//
+// Measured on 4096 x 50304 bf16 logits, 64 entries: forward 76 us after a backward pass, 70 us alone (0.41 GB: 5.4 and
+// 5.9 TB/s), backward 152 us (0.82 GB: 5.4 TB/s).  One workgroup per row: of 256 threads, or of 1024 below DISTILL_FEW rows,
+// where a row's walk is the whole time (3 x 50257 fp32: forward 8.2 -> 6.5 us, backward 8.6 -> 7.4).
 #include "rows.hpp"
 
 namespace bgx {
