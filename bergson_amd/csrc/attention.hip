@@ -157,11 +157,12 @@ __device__ inline __amdgpu_buffer_rsrc_t row_buffer(const T* base, int64_t tok, 
   const int bytes = rows > 0 ? (int)(((rows - 1) * tok + D) * (int64_t)sizeof(T)) : 0;
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, bytes, 0x00020000);
 }
-constexpr uint32_t NO_ROW = 0x7ffffff0u;  // an offset past every buffer
+constexpr uint32_t NO_ROW = 0x7ffffff0u;  // an offset past every buffer, also with a tile's passes added
 
-__device__ inline uint4 buffer_load16(__amdgpu_buffer_rsrc_t r, uint32_t offset, uint32_t pass) {
+// The whole offset goes through the lane's register: the bounds check is defined for that part only.
+__device__ inline uint4 buffer_load16(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
   typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
-  const raw4 v = __builtin_bit_cast(raw4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)offset, (int)pass, 0));
+  const raw4 v = __builtin_bit_cast(raw4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)offset, 0, 0));
   return make_uint4(v.x, v.y, v.z, v.w);
 }
 __device__ inline float buffer_load4(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
@@ -188,7 +189,7 @@ struct Staged {
   __device__ void load(const T* base, int64_t tok, int rows, int D) {
     const __amdgpu_buffer_rsrc_t r = row_buffer(base, tok, min(rows, BK), D);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) v[i] = buffer_load16(r, offset, i * pass);
+    for (int i = 0; i < PER; ++i) v[i] = buffer_load16(r, offset + i * pass);
   }
   __device__ void store(char* tile) const {
     if (DP == 96 && (int)threadIdx.x % CH >= Tile<T, DP>::CHUNKS) return;
@@ -438,7 +439,7 @@ __device__ inline void load_own(const T* base, int64_t tok, int row, int rows, i
 #pragma unroll
   for (int ks = 0; ks < DP / (2 * EPL); ++ks) {
     const int col = (2 * ks + (lane >> 5)) * EPL;
-    f[ks] = buffer_load16(r, col < D && row < rows ? (uint32_t)(row * (int)tok + col) * (uint32_t)sizeof(T) : NO_ROW, 0);
+    f[ks] = buffer_load16(r, col < D && row < rows ? (uint32_t)(row * (int)tok + col) * (uint32_t)sizeof(T) : NO_ROW);
   }
 }
 

@@ -2,8 +2,8 @@
 // include/bergson_amd.h, without the interpreter in either pass.
 //
 // A Python autograd function of the same calls took 114 us for a forward and backward pass of a small layer norm on
-// an MI355X host (70 us with the engine on the caller's thread), this takes about a third: the backward pass runs on
-// the engine's own thread, where every step of a Python function competes for the interpreter.
+// an MI355X host, this takes 64, of which 40 are the engine's own (x * 2 and its gradient): the backward pass runs on
+// the engine's thread, where every step of a Python function competes for the interpreter.
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
