@@ -27,6 +27,7 @@
 // without overlapping fully: 24 documents of 16 to 2048 positions, 16 heads, fp16: forward 84 us (0.55 PFLOP/s), dq 113 us
 // (0.62), dk and dv 167 us (0.56).  Tiles of 32 or 128 keys instead of 64, four waves a SIMD instead of three, and raised
 // wave priority around the products did not change the forward pass there (86, 93, 87, 84 us).
+#include <cfloat>
 #include <initializer_list>
 
 #include "mma32.hpp"
@@ -530,7 +531,8 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
         m = top;
       }
       // a row all of whose scores so far are -inf keeps a maximum of -inf; its weights are 0, not 0 - 0
-      const float shift = m == -INFINITY ? 0.f : m * c;
+      // (and where the factor takes the type's lowest value past the numbers, its weights become 0, not inf - inf)
+      const float shift = m == -INFINITY ? 0.f : fmaxf(m * c, -FLT_MAX);
 #pragma unroll
       for (int u = 0; u < SUB; ++u)
 #pragma unroll
@@ -659,10 +661,16 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
     if constexpr (HALF) A.peak[stat] = peak;
   }
   // dS is P times something of the size of do: with small gradients it would fall among fp16's subnormals.  The
-  // row's power of two is taken out of it (in the exponent of P, at no cost) and put back on dq.
+  // row's power of two is taken out of it (in the exponent of P, at no cost) and put back on dq.  So is the one that
+  // brings the weights, which are not divided by their sum here and reach 2^8 (the shift may lag that far), below 1:
+  // dS then stays within 4 sum_d |v_d|.
   float lift = 0.f;
-  if constexpr (HALF) lift = peak > 0.f && peak < INFINITY ? -(float)ilogbf(peak) : 0.f;
-  const float shift = in ? A.shift[stat] - lift : 0.f, over_sum = in ? 1.0f / A.sum[stat] : 0.f;
+  const float sum = in ? A.sum[stat] : 1.f;
+  if constexpr (HALF) {
+    lift = peak > 0.f && peak < INFINITY ? -(float)ilogbf(peak) : 0.f;
+    lift -= sum < 256.f ? (float)(ilogbf(sum) + 1) : 8.f;
+  }
+  const float shift = in ? A.shift[stat] - lift : 0.f, over_sum = in ? 1.0f / sum : 0.f;
   const float c = A.scale * AT_LOG2E;
   f32x16 dq[DT];
 #pragma unroll

@@ -121,9 +121,10 @@ __global__ __launch_bounds__(THREADS) void distill_forward_kernel(DistillArgs A)
       s *= exp2_hw((m - top) * c);
       m = top;
     }
-    const float shift = m == -INFINITY ? 0.f : m * c;  // nothing but -inf so far: weights of 0
+    // nothing but -inf so far: weights of 0.  The difference first: m c may leave the numbers where m does not.
+    const float shift = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int e = 0; e < count; ++e) s += exp2_hw(fmaf(v[e], c, -shift));
+    for (int e = 0; e < count; ++e) s += exp2_hw((v[e] - shift) * c);
   };
   const int chunks = A.V / EPL;  // whole ones; the row's last elements go one by one
   int i = threadIdx.x;
@@ -172,6 +173,7 @@ __global__ __launch_bounds__(THREADS) void distill_backward_kernel(DistillArgs A
   __shared__ float slot[THREADS / WAVE];
   __shared__ int id[DISTILL_MAX_K];
   __shared__ float prob[DISTILL_MAX_K];
+  __shared__ int head[DISTILL_MAX_K], next[DISTILL_MAX_K];  // entries by the low bits of their ids, in lists
   // from the last row on: what the forward pass read last may still be in the memory-side cache
   const int64_t r = A.rows - 1 - blockIdx.x;
   const float top = A.stats[2 * r], s = A.stats[2 * r + 1];
@@ -183,8 +185,12 @@ __global__ __launch_bounds__(THREADS) void distill_backward_kernel(DistillArgs A
     if ((int)threadIdx.x < rest) store_bits(dz + (int64_t)chunks * EPL + threadIdx.x, 0u);
     return;
   }
+  const int mask = (1 << (32 - __clz(A.K - 1))) - 1;  // as many lists as entries, rounded up to a power of two
+  for (int k = threadIdx.x; k <= mask; k += THREADS) head[k] = -1;
   float t_max, t_sum;
   teacher_row<THREADS>(A, r, id, prob, slot, t_max, t_sum);
+  for (int k = threadIdx.x; k < A.K; k += THREADS)
+    if (id[k] >= 0) next[k] = atomicExch(&head[id[k] & mask], k);
   const T* z = (const T*)A.logits + r * A.stride;
   const float c = LOG2E / A.tau, g = A.grad[r] * A.tau, scale = g / s;
   int i = threadIdx.x;
@@ -213,13 +219,29 @@ __global__ __launch_bounds__(THREADS) void distill_backward_kernel(DistillArgs A
     store_as(dz, at, exp2_hw((Elem<T>::load(z + at) - top) * c) * scale, Elem<T>::code);
   }
   // The teacher's entries again, with their probabilities taken off before the one rounding.  An id that comes
-  // twice is written twice with the same value: every writer adds all entries of its id, in the order of k.
+  // twice is written twice with the same value: every writer adds all entries of its id, in the order of k.  They
+  // are found in its list, whose own order is that of the atomics: the next one up from the last, while they are few.
+  // (Looking at all K for each: 4096 x 50304 with 1024 entries 609 us, this way 295; 173 with 64.)  The row's
+  // stores are waited for: these overwrite some of them from other waves.
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   __syncthreads();
   for (int k = threadIdx.x; k < A.K; k += THREADS) {
     if (id[k] < 0) continue;
+    int same = 0;
+    for (int j = head[id[k] & mask]; j >= 0; j = next[j]) same += id[j] == id[k];
     float p = 0.f;
-    for (int j = 0; j < A.K; ++j)
-      if (id[j] == id[k]) p += exp2_hw((prob[j] - t_max) * c);
+    if (same <= 8) {
+      for (int n = 0, last = -1; n < same; ++n) {
+        int least = DISTILL_MAX_K;
+        for (int j = head[id[k] & mask]; j >= 0; j = next[j])
+          if (id[j] == id[k] && j > last) least = min(least, j);
+        p += exp2_hw((prob[least] - t_max) * c);
+        last = least;
+      }
+    } else {
+      for (int j = 0; j < A.K; ++j)
+        if (id[j] == id[k]) p += exp2_hw((prob[j] - t_max) * c);
+    }
     const float q = exp2_hw((Elem<T>::load(z + id[k]) - top) * c) / s;
     store_as(dz, id[k], g * (q - p / t_sum), Elem<T>::code);
   }

@@ -180,7 +180,7 @@ Tensor gradient_like(const Tensor& t) {
 }
 
 // Packed calls of one sequence, or of at most 64 and too few tiles for their order to matter, need no plan: a launch
-// less (short documents, 48 of up to 96 tokens with 12 heads: 13 us with it).
+// less (48 documents of up to 96 tokens, 12 heads: 13 us with it, 7.3 without).
 bool needs_plan(const Tensor& q, int64_t n_seqs) {
   return n_seqs > 1 && (n_seqs > 64 || (q.size(0) / 128 + n_seqs) * q.size(1) > 1024);
 }

@@ -5,7 +5,8 @@ They are what runs between the hooked Linear modules of a collection step (the r
 bergson/collector/collector.py:926-985).  The arithmetic is the library's (include/bergson_amd.h); argument checks,
 allocation and the autograd nodes are native too (csrc/torch_ops.cpp).  Everything is enqueued on torch's current
 stream of the tensors' device, allocates through torch only (so that a graph capture owns its memory), keeps nothing
-between calls and can be captured; gradients are not differentiable again.
+between calls and can be captured (a backward pass as torch has it: into leaves that no graph built before the
+capture still holds); gradients are not differentiable again.
 """
 from __future__ import annotations
 

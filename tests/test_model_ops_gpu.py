@@ -1,6 +1,8 @@
 """Layer norm, causal attention and top-k distillation against their definitions in 64 bits, elementwise within the
 bounds derived in model_reference.py; plus what must hold exactly: rows outside every sequence, masked tokens,
 repeated runs, other layouts of the same values, captured graphs."""
+import math
+
 import pytest
 import torch
 
@@ -267,6 +269,19 @@ def test_attention_far_scores(device, bgx_env, dtype, rows):
 
 
 @pytest.mark.parametrize("rows", [128, 64, 32])
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+def test_attention_lowest_scores(device, bgx_env, dtype, rows):
+    """Scores at the type's lowest value, which the exponents' factor takes past the numbers: the rows that see others
+    beside them give those a weight of 0."""
+    bgx_env("BGX_ATTENTION_ROWS", rows)
+    q, k, v, _ = _qkv((140,), 1, 1, 32, dtype, 6, device)
+    q[..., 0], k[:64, :, 0] = 1.0, torch.finfo(dtype).min
+    out = B.causal_attention(q, k, v, cu_seqlens=torch.tensor([0, 140], dtype=torch.int32, device=device), scale=1.0)
+    ref = attention_reference(q[64:], k[64:], v[64:], 1.0, None, dtype)
+    assert_within(out[64:], *ref["o"], "rows that see more than the lowest value")
+
+
+@pytest.mark.parametrize("rows", [128, 64, 32])
 def test_attention_small_gradients_in_fp16(device, bgx_env, rows):
     """Output gradients near fp16's smallest normal number: dS itself would vanish among the subnormals."""
     bgx_env("BGX_ATTENTION_ROWS", rows)
@@ -282,6 +297,23 @@ def test_attention_small_gradients_in_fp16(device, bgx_env, rows):
         # scaled by a power of two: the same up to the rounding of the results among the subnormals
         assert (small.double() - large.double() * 2.0 ** -12).abs().max() <= 2.0 ** -25 + 2.0 ** -11 * small.abs().max()
     _check_sequences(q, k, v, do, B.causal_attention(q, k, v, cu_seqlens=cu), grads, [(0, 260)], 0.125, torch.float16)
+
+
+@pytest.mark.parametrize("rows", [128, 64, 32])
+def test_attention_large_values_in_fp16(device, bgx_env, rows):
+    """Values near 2^8 and weights far above those of a row's first tile: dS of weights that are not yet divided by
+    their sum would leave fp16's range."""
+    bgx_env("BGX_ATTENTION_ROWS", rows)
+    q, k, v, do = _qkv((260,), 2, 1, 64, torch.float16, 13, device, gain=1.0)
+    q, k, v = q * 0.1, k * 0.1, v * 64
+    q[..., 0], k[:, :, 0] = 1.0, 0.0
+    k[130:, :, 0] = 5.0   # 2^7.2 times the weight
+    cu = torch.tensor([0, 260], dtype=torch.int32, device=device)
+    for t in (q, k, v):
+        t.requires_grad_()
+    out = B.causal_attention(q, k, v, cu_seqlens=cu, scale=1.0)
+    grads = torch.autograd.grad(out, (q, k, v), do)
+    _check_sequences(q, k, v, do, out, grads, [(0, 260)], 1.0, torch.float16)
 
 
 @pytest.mark.parametrize("rows", [128, 32])
@@ -447,6 +479,24 @@ def test_distillation_entries(device, dtype):
     assert (loss[[3, 5, 6]] == 0).all() and (dz[[3, 5, 6]] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("K,distinct", [(600, 1), (600, 40), (600, 500), (9, 2), (1024, 1000)], ids=str)
+def test_distillation_repeated_entries(device, dtype, K, distinct):
+    """Ids that come a few times, many times, all the same: their probabilities add up, with the same bits every time."""
+    z, _, _, grad = _distill_case(3, 2000, 1, dtype, 4, device)
+    g = _gen(K + distinct)
+    ids = (torch.randint(0, distinct, (3, K), generator=g) * 1024 % 2000).to(device)   # the low bits alike, too
+    t = torch.randn(3, K, generator=g).to(device)
+    z.requires_grad_()
+    loss = B.topk_distillation(z, ids, t)
+    dz, = torch.autograd.grad(loss, z, grad)
+    ref = distill_reference(z, ids, t, 1.0, None, grad, dtype)
+    assert_within(loss, *ref["loss"], "loss")
+    assert_within(dz, *ref["dz"], "dz")
+    again, = torch.autograd.grad(B.topk_distillation(z, ids, t), z, grad)
+    assert torch.equal(dz, again)
+
+
 def test_distillation_infinite_logits(device):
     """A vocabulary masked with -inf: those entries have no mass and no gradient; a teacher entry among them makes its
     token's loss infinite and leaves the others alone.  NaN stays in its token."""
@@ -465,6 +515,29 @@ def test_distillation_infinite_logits(device):
     ref = distill_reference(z[rows].clamp_min(-1e4), ids[rows], t[rows], 1.0, None, grad[rows], torch.float32)
     assert_within(loss[rows], *ref["loss"], "loss")
     assert_within(dz[rows], *ref["dz"], "dz")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+def test_distillation_lowest_logits(device, dtype):
+    """A vocabulary masked with the type's lowest value, in part and as a whole: what whole threads see of it leaves the
+    numbers when it is scaled."""
+    z = torch.full((3, 5001), torch.finfo(dtype).min, dtype=dtype, device=device)
+    z[0, 17], z[0, 3000], z[1, 17] = 1.0, 2.0, 1.0
+    ids, t = torch.tensor([[17, 3000], [17, -1], [17, 3000]], device=device), torch.ones(3, 2, device=device)
+    grad = torch.ones(3, device=device)
+    z.requires_grad_()
+    loss = B.topk_distillation(z, ids, t)
+    dz, = torch.autograd.grad(loss, z, grad)
+    ref = distill_reference(z, ids, t, 1.0, None, None, dtype)
+    assert_within(loss, *ref["loss"], "loss")
+    q = torch.zeros(3, 5001, dtype=torch.float64)
+    q[0, 17], q[0, 3000], q[1, 17], q[2] = 1 / (1 + math.e), math.e / (1 + math.e), 1.0, 1 / 5001
+    p = torch.zeros_like(q)
+    p[0, 17] = p[0, 3000] = p[2, 17] = p[2, 3000] = 0.5
+    p[1, 17] = 1.0
+    # q to (V / 256 + 48) u, the difference to 4 u of both, the rounding to the type
+    bound = (68 * 2.0 ** -24) * q + 2.0 ** -22 * (q + p) + torch.finfo(dtype).eps / 2 * (q - p).abs() + torch.finfo(dtype).tiny
+    assert_within(dz, q - p, bound, "dz")
 
 
 def test_distillation_layouts(device):
