@@ -626,17 +626,26 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
   const T* v = attn_rows<T>(A.v, it, kvh);
   uint4 qf[KS], gf[KS];
   const int own = row - first, left = it.len - first;
+  const int64_t stat = (int64_t)qh * A.rows + it.stat + row;
+  // everything the walk starts with is on its way before the first value is used
   load_own<T, DP, W::ROWS>(attn_rows<T>(A.grad_o, it, qh) + first * A.grad_o.tok, A.grad_o.tok, own, left, A.D, lane, gf);
+  const float kept_shift = in ? A.shift[stat] : 0.f, sum = in ? A.sum[stat] : 1.f;
+  Staged<T, DP, BK> sk, sv;
+  sk.init(A.k.tok, A.D);
+  sv.init(A.v.tok, A.D);
   float delta = 0.f, peak = 0.f;
   {
-    load_own<T, DP, W::ROWS>(attn_rows<T>(A.o, it, qh) + first * A.o.tok, A.o.tok, own, left, A.D, lane, qf);
-    uint4 rf[KS];
+    uint4 of[KS], rf[KS];
+    load_own<T, DP, W::ROWS>(attn_rows<T>(A.o, it, qh) + first * A.o.tok, A.o.tok, own, left, A.D, lane, of);
     if constexpr (sizeof(T) == 2)
       load_own<T, DP, W::ROWS>((const T*)A.rest + ((it.stat + first) * A.Hq + qh) * A.D, (int64_t)A.Hq * A.D, own, left, A.D, lane, rf);
+    load_own<T, DP, W::ROWS>(attn_rows<T>(A.q, it, qh) + first * A.q.tok, A.q.tok, own, left, A.D, lane, qf);
+    sk.load(k, A.k.tok, it.len, A.D);
+    sv.load(v, A.v.tok, it.len, A.D);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       float a[M::EPL], b[M::EPL];
-      Chunk<T>::unpack(qf[ks], a);
+      Chunk<T>::unpack(of[ks], a);
       Chunk<T>::unpack(gf[ks], b);
       if constexpr (sizeof(T) == 2) {  // delta stands against dp in fp32: it needs o unrounded
         float r[M::EPL];
@@ -654,8 +663,6 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
     delta = d.x + d.y;
     peak = fmaxf(p.x, p.y);
   }
-  load_own<T, DP, W::ROWS>(attn_rows<T>(A.q, it, qh) + first * A.q.tok, A.q.tok, own, left, A.D, lane, qf);
-  const int64_t stat = (int64_t)qh * A.rows + it.stat + row;
   if (in && half == 0 && part == 0) {
     A.delta[stat] = delta;
     if constexpr (HALF) A.peak[stat] = peak;
@@ -665,12 +672,11 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
   // brings the weights, which are not divided by their sum here and reach 2^8 (the shift may lag that far), below 1:
   // dS then stays within 4 sum_d |v_d|.
   float lift = 0.f;
-  const float sum = in ? A.sum[stat] : 1.f;
   if constexpr (HALF) {
     lift = peak > 0.f && peak < INFINITY ? -(float)ilogbf(peak) : 0.f;
     lift -= sum < 256.f ? (float)(ilogbf(sum) + 1) : 8.f;
   }
-  const float shift = in ? A.shift[stat] - lift : 0.f, over_sum = in ? 1.0f / sum : 0.f;
+  const float shift = kept_shift - lift, over_sum = 1.0f / sum;
   const float c = A.scale * AT_LOG2E;
   f32x16 dq[DT];
 #pragma unroll
@@ -678,11 +684,6 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
 #pragma unroll
     for (int i = 0; i < 16; ++i) dq[dt][i] = 0.f;
   const int n_tiles = (min(first + W::ROWS, it.len) + BK - 1) / BK;
-  Staged<T, DP, BK> sk, sv;
-  sk.init(A.k.tok, A.D);
-  sv.init(A.v.tok, A.D);
-  sk.load(k, A.k.tok, it.len, A.D);
-  sv.load(v, A.v.tok, it.len, A.D);
   sk.store(lds);
   sv.store(lds + W::BYTES);
   for (int t = 0; t < n_tiles; ++t) {
