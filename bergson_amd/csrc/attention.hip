@@ -23,10 +23,14 @@
 // products.  At heads of 128 the products win: forward 315 us for 2 x 4096 positions, 32 query on 8 key/value heads
 // (0.27 TFLOP of the causal half: 0.87 PFLOP/s), 2.2-2.3 ms for 1 x 16384 (0.96-1.0), dq 465 us (three products: 0.89), dk and dv
 // 667 us (four: 0.82), where a large library product reaches 1.11.  At heads of 64 a block has half the products for the
-// same vector work, and LDS reads (dk, dv), vector instructions and matrix instructions each take 30-50 % of the time
-// without overlapping fully: 24 documents of 16 to 2048 positions, 16 heads, fp16: forward 84 us (0.55 PFLOP/s), dq 113 us
-// (0.62), dk and dv 167 us (0.56).  Tiles of 32 or 128 keys instead of 64, four waves a SIMD instead of three, and raised
-// wave priority around the products did not change the forward pass there (86, 93, 87, 84 us).
+// same vector work, which then takes longer than they do; long walks still overlap the two: 2 x 16384 positions, 16 heads,
+// fp16: forward 1.24 ms (0.88 PFLOP/s), dq, dk and dv 4.15 ms (seven products: 0.93).  Short walks do not hide what comes
+// before and after them: 24 documents of 16 to 2048 positions (nine tiles a workgroup) take 84 us forward (0.55 PFLOP/s),
+// 111 for dq (0.62), 167 for dk and dv (0.56), and without the walks, loading and storing the rows alone (4 to 5 TB/s), 28, 40
+// and 44.  There tiles of 32 or 128 keys instead of 64, four waves a SIMD instead of three, and raised wave priority around the
+// products were no faster (forward 86, 93, 87, 84 us), nor long and short walks in turn instead of longest first (105),
+// results turned through LDS to whole rows (84) or stored past the caches (97); eight waves for 64 rows
+// made 4 x 1024 positions of 12 heads 23 us forward instead of 19.
 #include <cfloat>
 #include <initializer_list>
 

@@ -2,6 +2,7 @@
 bounds derived in model_reference.py; plus what must hold exactly: rows outside every sequence, masked tokens,
 repeated runs, other layouts of the same values, captured graphs."""
 import math
+import threading
 
 import pytest
 import torch
@@ -634,6 +635,66 @@ def test_on_another_stream(device, which):
     torch.cuda.synchronize()
     for res in results:
         assert all(torch.equal(a, b) for a, b in zip(res, want))
+
+
+def test_two_graphs_of_the_same_calls(device):
+    """Two captured graphs of all three operators, replayed in turn: neither holds anything of the other."""
+    calls = _calls(device)
+    results = []
+    for factor in (1.0, 0.5):
+        args = {n: ([(t.float() * factor).to(t.dtype).requires_grad_() for t in leaves], grad)
+                for n, (_, leaves, grad) in calls.items()}
+
+        def step():
+            out = []
+            for n, (leaves, grad) in args.items():
+                y = calls[n][0](*leaves)
+                out += [y.detach(), *torch.autograd.grad(y, leaves, grad)]
+            return out
+
+        want = [t.clone() for t in step()]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = step()
+        results.append((graph, captured, want, args))
+    for _ in range(3):
+        for graph, _, _, _ in results:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, captured, want, _ in results:
+            assert all(torch.equal(a, b) for a, b in zip(captured, want))
+            for t in captured:
+                t.zero_()
+
+
+def test_calls_from_several_threads(device):
+    """Forward and backward passes of all operators from four threads, each on a stream of its own."""
+    calls = _calls(device)
+    run = lambda leaves: [r for n, (fn, _, grad) in calls.items()
+                          for y in [fn(*leaves[n])] for r in (y.detach(), *torch.autograd.grad(y, leaves[n], grad))]
+    fresh = lambda: {n: [t.detach().clone().requires_grad_() for t in leaves] for n, (_, leaves, _) in calls.items()}
+    want, got = run(fresh()), {}
+    inputs = [fresh() for _ in range(4)]
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i] = run(inputs[i])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want))
 
 
 def test_gradients_against_differences(device):
