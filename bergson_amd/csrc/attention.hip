@@ -20,9 +20,9 @@
 // the rests, see Work).  delta is formed from o as it was before its rounding: dp - delta cancels.
 //
 // What bounds them: a 32 x 32 block of scores costs a wave 16 exponentials a lane beside 2 (forward), 3 (dq) or 4 (dk, dv)
-// products.  At heads of 128 the products win: forward 315 us for 2 x 4096 positions, 32 query on 8 key/value heads
-// (0.27 TFLOP of the causal half: 0.87 PFLOP/s), 2.2-2.3 ms for 1 x 16384 (0.96-1.0), dq 465 us (three products: 0.89), dk and dv
-// 667 us (four: 0.82), where a large library product reaches 1.11.  At heads of 64 a block has half the products for the
+// products.  At heads of 128 the products win: forward 303 us for 2 x 4096 positions, 32 query on 8 key/value heads
+// (0.27 TFLOP of the causal half: 0.91 PFLOP/s), 2.2 ms for 1 x 16384 (1.0), dq 440 us (three products: 0.94), dk and dv
+// 642 us (four: 0.86), where a large library product reaches 1.11.  At heads of 64 a block has half the products for the
 // same vector work, which then takes longer than they do; long walks still overlap the two: 2 x 16384 positions, 16 heads,
 // fp16: forward 1.24 ms (0.88 PFLOP/s), dq, dk and dv 4.15 ms (seven products: 0.93).  Short walks do not hide what comes
 // before and after them: 24 documents of 16 to 2048 positions (nine tiles a workgroup) take 84 us forward (0.55 PFLOP/s),
