@@ -451,10 +451,12 @@ __device__ inline void load_own(const T* base, int64_t tok, int row, int rows, i
 __device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ---- forward -----------------------------------------------------------------------------------------------------
-template <typename T, int DP, int RW>
+// BRIEF: P (here) and dS (in the backward kernels) as two operands whatever RW is (see attn_brief).
+template <typename T, int DP, int RW, bool BRIEF = false>
 __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void attention_forward_kernel(AttnArgs A) {
   using M = Attn<T>;
   using W = Work<T, DP, RW>;
+  constexpr bool FINE = W::FINE || BRIEF;
   constexpr int BK = W::STEP, KS = DP / (2 * M::EPL), SUB = W::SUB, G = 32 / M::GROUP, DT = DP / 32;
   __shared__ __attribute__((aligned(16))) char lds[W::LDS];
   AttnItem it;
@@ -550,12 +552,12 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
         for (int g = 0; g < G; ++g) {
           const uint4 p = M::pack(s[u], g);
           uint4 rest = p;
-          if constexpr (W::FINE) rest = pack_rest<T>(s[u], g, p);
+          if constexpr (FINE) rest = pack_rest<T>(s[u], g, p);
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
             const uint4 a = M::template read_tr<DP>(tv, u * 32 + g * M::GROUP, dt, lane);
             Mma32<T>::mma(a, p, o[dt]);
-            if constexpr (W::FINE) Mma32<T>::mma(a, rest, o[dt]);
+            if constexpr (FINE) Mma32<T>::mma(a, rest, o[dt]);
           }
         }
     }
@@ -608,10 +610,11 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
 
 // ---- backward: queries -------------------------------------------------------------------------------------------
 // dq of 32 queries a wave; also leaves delta (and, for fp16, the largest |do| of a row) for the other kernel.
-template <typename T, int DP, int RW>
+template <typename T, int DP, int RW, bool BRIEF = false>
 __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void attention_backward_q_kernel(AttnArgs A) {
   using M = Attn<T>;
   using W = Work<T, DP, RW>;
+  constexpr bool FINE = W::FINE || BRIEF;
   constexpr bool HALF = std::is_same<T, f16_t>::value;
   constexpr int BK = W::STEP, KS = DP / (2 * M::EPL), SUB = W::SUB, G = 32 / M::GROUP, DT = DP / 32;
   __shared__ __attribute__((aligned(16))) char lds[W::LDS];
@@ -729,12 +732,12 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
         for (int g = 0; g < G; ++g) {
           const uint4 ds = M::pack(s, g);
           uint4 rest = ds;
-          if constexpr (W::FINE) rest = pack_rest<T>(s, g, ds);
+          if constexpr (FINE) rest = pack_rest<T>(s, g, ds);
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
             const uint4 a = M::template read_tr<DP>(tk, u * 32 + g * M::GROUP, dt, lane);
             Mma32<T>::mma(a, ds, dq[dt]);
-            if constexpr (W::FINE) Mma32<T>::mma(a, rest, dq[dt]);
+            if constexpr (FINE) Mma32<T>::mma(a, rest, dq[dt]);
           }
         }
       }
@@ -764,11 +767,12 @@ constexpr int kv_waves() {
   return RW == 4 && DP > 64 && sizeof(T) == 2 ? 8 : AT_WAVES;
 }
 
-template <typename T, int DP, int RW>
+template <typename T, int DP, int RW, bool BRIEF = false>
 __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
                              (Work<T, DP, RW, kv_waves<T, DP, RW>()>::PER_SIMD_KV)) void attention_backward_kv_kernel(AttnArgs A) {
   using M = Attn<T>;
   using W = Work<T, DP, RW, kv_waves<T, DP, RW>()>;
+  constexpr bool FINE = W::FINE || BRIEF;       // dS as two operands
   constexpr bool OWN = W::THREADS > AT_THREADS;  // k and v of the workgroup's keys live in LDS
   constexpr bool HALF = std::is_same<T, f16_t>::value;
   constexpr int BQ = W::STEP, KS = DP / (2 * M::EPL), SUB = W::SUB, G = 32 / M::GROUP, DT = DP / 32;
@@ -939,20 +943,16 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
         for (int g = 0; g < G; ++g) {
           const uint4 p = M::pack(s, g), ds = M::pack(dp, g);
           uint4 p_rest = p, ds_rest = ds;
-          if constexpr (W::FINE) {
-            p_rest = pack_rest<T>(s, g, p);
-            ds_rest = pack_rest<T>(dp, g, ds);
-          }
+          if constexpr (W::FINE) p_rest = pack_rest<T>(s, g, p);
+          if constexpr (FINE) ds_rest = pack_rest<T>(dp, g, ds);
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
             const uint4 a = M::template read_tr<DP>(tg, u * 32 + g * M::GROUP, dt, lane);
             const uint4 b = M::template read_tr<DP>(tq, u * 32 + g * M::GROUP, dt, lane);
             Mma32<T>::mma(a, p, dv[dt]);
             Mma32<T>::mma(b, ds, dk[dt]);
-            if constexpr (W::FINE) {
-              Mma32<T>::mma(a, p_rest, dv[dt]);
-              Mma32<T>::mma(b, ds_rest, dk[dt]);
-            }
+            if constexpr (W::FINE) Mma32<T>::mma(a, p_rest, dv[dt]);
+            if constexpr (FINE) Mma32<T>::mma(b, ds_rest, dk[dt]);
           }
         }
       }
@@ -1138,6 +1138,15 @@ static AttnArgs attn_args(const bgx_attention_shape* a) {
 // 29.3 / 33.8 / 52.1; dk and dv of 8 x 256, 16 heads (256) 17.2 / 23.2 / 40.9, 2 x 1024, 12 heads (192) 40.8 / 37.8 / 50.2;
 // fp32, heads of 64, forward of 6 x 1024 (576) 125 / 107 / 121.  dk and dv of wide fp32 heads need more registers than there
 // are with 128 rows (2 x 2048, 8 key/value heads: 2653 / 1201 / 2510) and have no such variant.
+// 16-bit sequences of up to 64 rows on average take workgroups of 128 rows however many there are, unless they take 32
+// (forward and backward of sequences of 64 / 32 / 8 positions, 4096 in all, 8 heads of 128, 128 against 64 rows: 59 and 65, 71 and
+// 94, 211 and 299 us; 12 heads of 64: the same).  Where gradients are wanted, P in the forward pass and dS go in as two
+// operands (Work): dq and dk of 2 to 8 positions are 1.5 to 1.6 times as far off as their own rounding without that, 1.0 times
+// with it (3 to 8 % of the time); of 64 and more 1.45 times.
+static bool attn_brief(const bgx_attention_shape* a) {
+  return a->dtype != BGX_F32 && a->rows <= 64 * (int64_t)a->n_seqs;
+}
+
 enum AttnKernel { ATTN_FORWARD, ATTN_Q, ATTN_KV };
 static unsigned attn_grid(AttnArgs& A, const bgx_attention_shape* a, AttnKernel kernel, int* which) {
   const int heads = kernel == ATTN_KV && A.part_k == nullptr ? a->kv_heads : a->heads;
@@ -1146,6 +1155,7 @@ static unsigned attn_grid(AttnArgs& A, const bgx_attention_shape* a, AttnKernel 
   const int64_t many = full ? (!wide ? 1024 : kernel == ATTN_KV ? INT64_MAX : 512)
                             : (!wide ? 512 : kernel == ATTN_FORWARD ? 160 : 256);
   *which = tall >= many ? 0 : tall >= 160 ? 1 : 2;
+  if (*which == 1 && attn_brief(a)) *which = 0;
   for (int i = 0; i < 3; ++i)
     if (switches().attention_rows == AT_TILES[i]) *which = i;
   if (kernel == ATTN_KV && wide && full && *which == 0) *which = 1;
@@ -1178,6 +1188,21 @@ static AttnView attn_view(const bgx_attention_rows* t) {
   return v;
 }
 
+// 128 rows, BRIEF
+template <typename T, int DP>
+static void attention_forward_kernel_brief(unsigned grid, hipStream_t s, const AttnArgs& A) {
+  if constexpr (sizeof(T) == 2) attention_forward_kernel<T, DP, 4, true><<<grid, AT_THREADS, 0, s>>>(A);
+}
+template <typename T, int DP>
+static void attention_backward_q_kernel_brief(unsigned grid, hipStream_t s, const AttnArgs& A) {
+  if constexpr (sizeof(T) == 2) attention_backward_q_kernel<T, DP, 4, true><<<grid, AT_THREADS, 0, s>>>(A);
+}
+template <typename T, int DP>
+static void attention_backward_kv_kernel_brief(unsigned grid, hipStream_t s, const AttnArgs& A) {
+  if constexpr (sizeof(T) == 2)
+    attention_backward_kv_kernel<T, DP, 4, true><<<grid, kv_waves<T, DP, 4>() * WAVE, 0, s>>>(A);
+}
+
 // the tallest variant of each kernel and its threads
 template <typename T, int DP>
 constexpr int attention_forward_kernel_tall() {
@@ -1206,7 +1231,9 @@ constexpr int attention_backward_kv_kernel_threads() {
 
 #define BGX_ATTN_ROWS(KERNEL, T, DP, WHICH, GRID, S, A)                    \
   do {                                                                     \
-    if ((WHICH) == 0)                                                      \
+    if ((WHICH) == 0 && brief)                                             \
+      KERNEL##_brief<T, DP>((GRID), (S), A);                               \
+    else if ((WHICH) == 0)                                                 \
       KERNEL<T, DP, KERNEL##_tall<T, DP>()><<<(GRID), KERNEL##_threads<T, DP>(), 0, (S)>>>(A); \
     else if ((WHICH) == 1)                                                 \
       KERNEL<T, DP, 2><<<(GRID), AT_THREADS, 0, (S)>>>(A);                 \
@@ -1284,6 +1311,7 @@ int attention_forward_impl(const bgx_attention_shape* a, const bgx_attention_row
   A.o = attn_view(o);
   attn_saved(A, a, saved);
   int which;
+  const bool brief = saved != nullptr && attn_brief(a);  // its gain is the gradients'
   const unsigned grid = attn_grid(A, a, ATTN_FORWARD, &which);
   BGX_REQUIRE(grid > 0, BGX_E_SHAPE, "attention: %lld rows of %d heads", (long long)a->rows, a->heads);
   BGX_ATTN_LAUNCH(attention_forward_kernel, a->dtype, a->head_dim, which, grid, (hipStream_t)stream, A);
@@ -1337,6 +1365,7 @@ int attention_backward_impl(const bgx_attention_shape* a, const bgx_attention_ro
   BGX_REQUIRE((uintptr_t)ws % 16 == 0, BGX_E_ALIGN, "attention backward: workspace not aligned to 16 bytes");
   hipStream_t s = (hipStream_t)stream;
   int which;
+  const bool brief = attn_brief(a);
   unsigned grid = attn_grid(A, a, ATTN_Q, &which);
   BGX_REQUIRE(grid > 0, BGX_E_SHAPE, "attention backward: %lld rows of %d heads", (long long)a->rows, a->heads);
   BGX_ATTN_LAUNCH(attention_backward_q_kernel, a->dtype, a->head_dim, which, grid, s, A);

@@ -337,6 +337,26 @@ def test_attention_offsets_past_32_bits(device, bgx_env, rows):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=ids_of)
+@pytest.mark.parametrize("length,dim", [(2, 64), (3, 128), (4, 32), (8, 64)], ids=str)
+def test_attention_gradients_of_short_sequences(device, length, dim, dtype):
+    """dq and dk of many short sequences are as near as their own rounding: what the kernel's operands lose (dS to 2^-21
+    of its value as two of them, the fp32 sums less) is 2^-8 of that rounding, and moves a value across a rounding
+    boundary so rarely that a twentieth covers both."""
+    n, scale = 80, dim ** -0.5
+    q, k, v, do = _qkv((n * length,), 8, 4, dim, dtype, length, device, gain=1.0)
+    cu = torch.arange(0, n * length + 1, length, dtype=torch.int32, device=device)
+    for t in (q, k, v):
+        t.requires_grad_()
+    grads = torch.autograd.grad(B.causal_attention(q, k, v, cu_seqlens=cu), (q, k), do)
+    refs = [attention_reference(*(t.detach()[a:a + length] for t in (q, k, v)), scale, do[a:a + length], dtype)
+            for a in range(0, n * length, length)]
+    for got, name in zip(grads, ("dq", "dk")):
+        want = torch.cat([r[name][0] for r in refs])
+        rounding = (want.to(dtype).double() - want).norm()
+        assert (got.cpu().double() - want).norm() <= 1.05 * rounding, name
+
+
 def test_attention_plan_of_many_sequences(device):
     """More sequences than the planning workgroup has threads, empty ones among them, long ones at the end."""
     g = _gen(2)
