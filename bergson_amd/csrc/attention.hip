@@ -16,21 +16,21 @@
 //
 // Scores, softmax statistics, probabilities' sums and all accumulators are fp32.  For 16-bit inputs P and dS are
 // rounded to the inputs' type as operands of the matrix instructions (the products of 16-bit operands are what runs
-// at the card's rate; each rounding is relative to the value, and their sum over a row averages out; small calls keep
-// the rests, see Work).  delta is formed from o as it was before its rounding: dp - delta cancels.
+// at the card's rate; each rounding is relative to the value, and their sum over a row averages out; small calls and
+// the gradients of short sequences keep the rests, see Work and attn_brief).  delta is formed from o as it was before its rounding: dp - delta cancels.
 //
-// What bounds them: a 32 x 32 block of scores costs a wave 16 exponentials a lane beside 2 (forward), 3 (dq) or 4 (dk, dv)
-// products.  At heads of 128 the products win: forward 303 us for 2 x 4096 positions, 32 query on 8 key/value heads
-// (0.27 TFLOP of the causal half: 0.91 PFLOP/s), 2.2 ms for 1 x 16384 (1.0), dq 440 us (three products: 0.94), dk and dv
-// 642 us (four: 0.86), where a large library product reaches 1.11.  At heads of 64 a block has half the products for the
-// same vector work, which then takes longer than they do; long walks still overlap the two: 2 x 16384 positions, 16 heads,
-// fp16: forward 1.24 ms (0.88 PFLOP/s), dq, dk and dv 4.15 ms (seven products: 0.93).  Short walks do not hide what comes
-// before and after them: 24 documents of 16 to 2048 positions (nine tiles a workgroup) take 84 us forward (0.55 PFLOP/s),
-// 111 for dq (0.62), 167 for dk and dv (0.56), and without the walks, loading and storing the rows alone (4 to 5 TB/s), 28, 40
-// and 44.  There tiles of 32 or 128 keys instead of 64, four waves a SIMD instead of three, and raised wave priority around the
-// products were no faster (forward 86, 93, 87, 84 us), nor long and short walks in turn instead of longest first (105),
-// results turned through LDS to whole rows (84) or stored past the caches (97); eight waves for 64 rows
-// made 4 x 1024 positions of 12 heads 23 us forward instead of 19.
+// What bounds them: a 32 x 32 block of scores costs a wave 16 exponentials a lane beside 2 (forward), 3 (dq) or 4 (dk,
+// dv) products.  At heads of 128 the products win: forward 303 us for 2 x 4096 positions, 32 query on 8 key/value heads
+// (0.27 TFLOP of the causal half: 0.91 PFLOP/s), 2.2 ms for 1 x 16384 (1.0), dq 440 us (three products: 0.94), dk and
+// dv 642 us (four: 0.86), where a large library product reaches 1.11.  At heads of 64 a block has half the products for
+// the same vector work, which then takes longer than they do; long walks still overlap the two: 2 x 16384 positions, 16
+// heads, fp16: forward 1.24 ms (0.88 PFLOP/s), dq, dk and dv 4.15 ms (seven products: 0.93).  Short walks do not hide
+// what comes before and after them: 24 documents of 16 to 2048 positions (nine tiles a workgroup) take 84 us forward
+// (0.55 PFLOP/s), 111 for dq (0.62), 167 for dk and dv (0.56), and without the walks, loading and storing the rows
+// alone (4 to 5 TB/s), 28, 40 and 44.  There tiles of 32 or 128 keys instead of 64, four waves a SIMD instead of three,
+// and raised wave priority around the products were no faster (forward 86, 93, 87, 84 us), nor long and short walks in
+// turn instead of longest first (105), results turned through LDS to whole rows (84) or stored past the caches (97);
+// eight waves for 64 rows made 4 x 1024 positions of 12 heads 23 us forward instead of 19.
 #include <cfloat>
 #include <initializer_list>
 
@@ -1139,10 +1139,10 @@ static AttnArgs attn_args(const bgx_attention_shape* a) {
 // fp32, heads of 64, forward of 6 x 1024 (576) 125 / 107 / 121.  dk and dv of wide fp32 heads need more registers than there
 // are with 128 rows (2 x 2048, 8 key/value heads: 2653 / 1201 / 2510) and have no such variant.
 // 16-bit sequences of up to 64 rows on average take workgroups of 128 rows however many there are, unless they take 32
-// (forward and backward of sequences of 64 / 32 / 8 positions, 4096 in all, 8 heads of 128, 128 against 64 rows: 59 and 65, 71 and
-// 94, 211 and 299 us; 12 heads of 64: the same).  Where gradients are wanted, P in the forward pass and dS go in as two
-// operands (Work): dq and dk of 2 to 8 positions are 1.5 to 1.6 times as far off as their own rounding without that, 1.0 times
-// with it (3 to 8 % of the time); of 64 and more 1.45 times.
+// (forward and backward of sequences of 64 / 32 / 8 positions, 4096 in all, 8 heads of 128, 128 against 64 rows:
+// 59 and 65, 71 and 94, 211 and 299 us; 12 heads of 64: the same).  Where gradients are wanted, P in the forward pass
+// and dS go in as two operands (Work): dq and dk of 2 to 8 positions are 1.5 to 1.6 times as far off as their own
+// rounding without that, 1.0 times with it (3 to 8 % of the time); of 64 and more 1.45 times.
 static bool attn_brief(const bgx_attention_shape* a) {
   return a->dtype != BGX_F32 && a->rows <= 64 * (int64_t)a->n_seqs;
 }

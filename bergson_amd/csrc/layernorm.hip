@@ -512,7 +512,8 @@ int layernorm_backward_impl(const void* dy, int64_t dy_stride, const void* x, in
     if (rc) return rc;
   }
   if (params && !few) {
-    layernorm_params_kernel<<<dim3((d + LN_COLS - 1) / LN_COLS, 2), LN_COLS * LN_GROUPS, 0, s>>>((const float*)ws, parts, d, dweight, dbias, wdtype);
+    layernorm_params_kernel<<<dim3((d + LN_COLS - 1) / LN_COLS, 2), LN_COLS * LN_GROUPS, 0, s>>>(
+        (const float*)ws, parts, d, dweight, dbias, wdtype);
     BGX_HIP(hipGetLastError());
   }
   return 0;
