@@ -17,7 +17,8 @@
 // Scores, softmax statistics, probabilities' sums and all accumulators are fp32.  For 16-bit inputs P and dS are
 // rounded to the inputs' type as operands of the matrix instructions (the products of 16-bit operands are what runs
 // at the card's rate; each rounding is relative to the value, and their sum over a row averages out; small calls and
-// the gradients of short sequences keep the rests, see Work and attn_brief).  delta is formed from o as it was before its rounding: dp - delta cancels.
+// the gradients of short sequences keep the rests, see Work and attn_brief).  delta is formed from o as it was before its
+// rounding: dp - delta cancels.
 //
 // What bounds them: a 32 x 32 block of scores costs a wave 16 exponentials a lane beside 2 (forward), 3 (dq) or 4 (dk,
 // dv) products.  At heads of 128 the products win: forward 303 us for 2 x 4096 positions, 32 query on 8 key/value heads
