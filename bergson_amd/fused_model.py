@@ -7,7 +7,8 @@ sees the same modules with inputs and output gradients that differ by rounding.
 
 Right-padded batches need no attention mask here: attention is causal, and with `sequence_lengths(lengths)` around a
 forward pass the padding is not computed at all (its attention output is 0).  A mask that says anything else than
-"causal" is refused.
+"causal" is refused, and so is an attention that takes anything beside queries, keys and values (sparse selections,
+biases on the scores, sinks, windows).
 """
 from __future__ import annotations
 
@@ -22,6 +23,10 @@ from torch import Tensor
 from .model_ops import causal_attention, layer_norm
 
 IMPLEMENTATION = "bergson_amd"
+# Keywords transformers hands through to attention that change none of its values: positions (the embeddings are in q and
+# k by then, and packed positions are refused with their mask) and what a model is asked to return or count.
+_WITHOUT_EFFECT = {"position_ids", "cache_position", "use_cache", "output_hidden_states", "output_router_logits",
+                   "return_dict", "logits_to_keep", "num_items_in_batch"}
 _current = threading.local()
 
 
@@ -54,16 +59,22 @@ def _mask(*args, attention_mask=None, mask_function=None, q_length=None, kv_leng
 
 def _attention(module: nn.Module, query: Tensor, key: Tensor, value: Tensor, attention_mask: Tensor | None,
                scaling: float | None = None, dropout: float = 0.0, **kwargs):
-    """transformers' attention interface: [N, heads, S, D] in, [N, S, heads, D] out, no weights."""
+    """transformers' attention interface: [N, heads, S, D] in, [N, S, heads, D] out, no weights.  A keyword that is not
+    known to leave the values alone is refused."""
     if attention_mask is not None:
         raise ValueError("fused attention takes no attention mask")
     if dropout:
         raise ValueError(f"fused attention has no dropout (got {dropout})")
-    for name in ("sliding_window", "softcap", "s_aux"):
-        if kwargs.get(name) is not None:
-            raise ValueError(f"fused attention does not know {name}={kwargs[name]}")
-    if kwargs.get("is_causal", getattr(module, "is_causal", True)) is False:
+    causal = kwargs.pop("is_causal", None)
+    if (getattr(module, "is_causal", True) if causal is None else causal) is False:
         raise ValueError("fused attention is causal")
+    if kwargs.pop("output_attentions", None):
+        raise ValueError("fused attention has no weights to return (output_attentions)")
+    # a window, sinks, a selection of keys, a bias on the scores ...: dropped, any of them would be a wrong result
+    for name, given in kwargs.items():
+        if given is not None and name not in _WITHOUT_EFFECT:
+            raise ValueError(f"fused attention does not know {name}=" + (f"a tensor {tuple(given.shape)}" if
+                             isinstance(given, Tensor) else repr(given)) + ": this model's attention is another one")
     if query.shape[2] != key.shape[2]:
         raise ValueError(f"fused attention has no key/value cache: {query.shape[2]} queries against {key.shape[2]} keys")
     lengths = getattr(_current, "lengths", None)

@@ -87,3 +87,50 @@ def test_loss_settings():
     with pytest.raises(ValueError, match="label_smoothing"):
         forward_loss_factory(B.IndexConfig(loss_fn="topk_kl", label_smoothing=0.1))
     assert B.IndexConfig().fused_model_ops is False and B.IndexConfig().loss_fn == "ce"
+
+
+def test_keywords_of_other_attentions_are_refused():
+    """What changes an attention's values and is not known here is refused; what does not is let through (the kernels'
+    own refusal of CPU tensors comes behind)."""
+    q = torch.zeros(2, 4, 5, 16)
+    mod = nn.Module()
+    for name, value in (("indices", torch.zeros(2, 5, 3)), ("block_indices", torch.zeros(2, 1, 5, 1)),
+                        ("position_bias", torch.zeros(1, 4, 5, 5)), ("sliding_window", 4), ("softcap", 30.0),
+                        ("s_aux", torch.zeros(4)), ("cu_seq_lens_q", torch.zeros(3)), ("head_mask", torch.ones(4)),
+                        ("an_option_of_tomorrow", False), ("output_attentions", True)):
+        with pytest.raises(ValueError, match=name):
+            fused_model._attention(mod, q, q, q, None, **{name: value})
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        fused_model._attention(mod, q, q, q, None, position_ids=torch.zeros(2, 5), use_cache=True, sliding_window=None,
+                               output_attentions=False, output_router_logits=True, is_causal=None)
+
+
+def test_causality_the_module_decides():
+    """is_causal=None leaves it to the module, like a call without it."""
+    q = torch.zeros(2, 4, 5, 16)
+    mod = nn.Module()
+    mod.is_causal = False
+    for kw in ({}, {"is_causal": None}):
+        with pytest.raises(ValueError, match="causal"):
+            fused_model._attention(mod, q, q, q, None, **kw)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        fused_model._attention(mod, q, q, q, None, is_causal=True)
+
+
+def test_keywords_through_a_model_are_refused(monkeypatch):
+    """What a model's call, or its layers, hand down to the attention function by keyword (here a choice of keys):
+    refused, where it was dropped and every key attended to."""
+    import torch.nn.functional as F
+
+    def attention(q, k, v, lengths=None, scale=None):
+        q, k, v = (t.transpose(1, 2) for t in (q, k, v))
+        return F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=scale, enable_gqa=True).transpose(1, 2)
+
+    monkeypatch.setattr(fused_model, "causal_attention", attention)
+    model = make_llama(torch.float32, "cpu", layers=1, d=32, heads=4, kv_heads=2, mlp=64, vocab=50)
+    x = torch.randint(0, 50, (2, 6))
+    want = model(x).logits
+    with B.fused_model_ops(model):
+        assert torch.allclose(model(x, num_items_in_batch=2).logits, want, atol=1e-5)
+        with pytest.raises(ValueError, match="indices"):
+            model(x, indices=torch.zeros(2, 6, 2, dtype=torch.int64))
