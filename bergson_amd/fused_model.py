@@ -101,6 +101,13 @@ def _register() -> None:
     AttentionMaskInterface.register(IMPLEMENTATION, _mask)
 
 
+def _attention_settings(model: nn.Module) -> list[tuple[object, str]]:
+    """(configuration, attention implementation) of the model and of every part that has its own, outer ones first."""
+    configs = {id(c): c for c in (getattr(m, "config", None) for m in model.modules())
+               if getattr(c, "_attn_implementation", None) is not None}
+    return [(c, c._attn_implementation) for c in configs.values()]
+
+
 @contextmanager
 def fused_model_ops(model: nn.Module):
     """Layer norms and causal attention of `model` through `layer_norm` and `causal_attention` within the context.
@@ -109,7 +116,8 @@ def fused_model_ops(model: nn.Module):
     its layer norms change.  Not for two threads at once on one model."""
     norms = [m for m in model.modules() if _fusable(m)]
     swap = callable(getattr(model, "set_attn_implementation", None))
-    before = model.config._attn_implementation if swap else None
+    # parts of a composite model have configurations of their own, which the outer one's setting overwrites
+    before = _attention_settings(model) if swap else []
     try:
         for m in norms:
             m.forward = functools.partial(_norm_forward, m)
@@ -121,4 +129,6 @@ def fused_model_ops(model: nn.Module):
         for m in norms:
             vars(m).pop("forward", None)
         if swap:
-            model.set_attn_implementation(before)
+            model.set_attn_implementation(before[0][1])
+            for config, implementation in before:
+                config._attn_implementation = implementation

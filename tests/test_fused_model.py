@@ -134,3 +134,35 @@ def test_keywords_through_a_model_are_refused(monkeypatch):
         assert torch.allclose(model(x, num_items_in_batch=2).logits, want, atol=1e-5)
         with pytest.raises(ValueError, match="indices"):
             model(x, indices=torch.zeros(2, 6, 2, dtype=torch.int64))
+
+
+class _Part(nn.Module):
+    def __init__(self, implementation, takes=True):
+        super().__init__()
+        self.config = type("Config", (), {"_attn_implementation": implementation})()
+        self.takes = takes
+
+
+class _Whole(_Part):
+    """Two parts with configurations of their own under one that, like transformers' composite models, sets them all --
+    those that take it."""
+
+    def __init__(self, *parts, takes=True):
+        super().__init__("sdpa", takes)
+        self.parts = nn.ModuleList(parts)
+
+    def set_attn_implementation(self, name):
+        for m in (self, *self.parts):
+            if m.takes:
+                m.config._attn_implementation = name
+
+
+def test_every_part_gets_its_own_attention_back():
+    model = _Whole(_Part("eager"), _Part("sdpa"))
+    of = lambda: [m.config._attn_implementation for m in (model, *model.parts)]
+    with B.fused_model_ops(model):
+        assert of() == ["bergson_amd"] * 3
+    assert of() == ["sdpa", "eager", "sdpa"]
+    with pytest.raises(KeyError), B.fused_model_ops(model):
+        raise KeyError("inside")
+    assert of() == ["sdpa", "eager", "sdpa"]
