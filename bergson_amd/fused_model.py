@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import functools
 import threading
+import warnings
 from contextlib import contextmanager
 
 import torch
@@ -108,12 +109,26 @@ def _attention_settings(model: nn.Module) -> list[tuple[object, str]]:
     return [(c, c._attn_implementation) for c in configs.values()]
 
 
+def _name_what_is_left(model: nn.Module) -> None:
+    """transformers leaves alone what does not go through its registry."""
+    left = {id(c) for c, implementation in _attention_settings(model) if implementation != IMPLEMENTATION}
+    names = []
+    for m in model.modules():
+        config = getattr(m, "config", None)
+        if id(config) in left:
+            left.discard(id(config))
+            names.append(type(m).__name__)
+    if names:
+        warnings.warn(f"{', '.join(names)} keeps its own attention: it cannot be replaced through transformers' registry, "
+                      "only layer norms run on this package's kernels there", stacklevel=4)
+
+
 @contextmanager
 def fused_model_ops(model: nn.Module):
     """Layer norms and causal attention of `model` through `layer_norm` and `causal_attention` within the context.
 
-    Attention is replaced in transformers models (`set_attn_implementation`); any other module keeps its own and only
-    its layer norms change.  Not for two threads at once on one model."""
+    Attention is replaced in transformers models (`set_attn_implementation`; a warning names a model that does not take
+    it); any other module keeps its own and only its layer norms change.  Not for two threads at once on one model."""
     norms = [m for m in model.modules() if _fusable(m)]
     swap = callable(getattr(model, "set_attn_implementation", None))
     # parts of a composite model have configurations of their own, which the outer one's setting overwrites
@@ -124,6 +139,7 @@ def fused_model_ops(model: nn.Module):
         if swap:
             _register()
             model.set_attn_implementation(IMPLEMENTATION)
+            _name_what_is_left(model)
         yield model
     finally:
         for m in norms:

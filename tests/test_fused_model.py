@@ -1,4 +1,6 @@
 """Fused model operators around a model: what is replaced and put back, what is refused, and the teacher's columns."""
+import warnings
+
 import pytest
 import torch
 import torch.nn as nn
@@ -166,3 +168,19 @@ def test_every_part_gets_its_own_attention_back():
     with pytest.raises(KeyError), B.fused_model_ops(model):
         raise KeyError("inside")
     assert of() == ["sdpa", "eager", "sdpa"]
+
+
+def test_an_attention_that_is_not_replaced_is_named():
+    """Models outside transformers' registry keep their attention: said by a warning, once, and the rest goes on."""
+    with pytest.warns(UserWarning, match="_Whole.*keeps its own attention"), B.fused_model_ops(_Whole(takes=False)):
+        pass
+    with pytest.warns(UserWarning, match="_Part.*keeps its own attention"), B.fused_model_ops(_Whole(_Part("eager", takes=False))):
+        pass
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        with B.fused_model_ops(_Whole(_Part("eager"))):
+            pass
+        with B.fused_model_ops(make_gpt_neox("pythia-14m", torch.float32, "cpu", layers=1)):
+            pass
+        with B.fused_model_ops(nn.Sequential(nn.LayerNorm(8))):     # nothing there to replace
+            pass
