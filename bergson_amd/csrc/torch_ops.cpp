@@ -42,6 +42,13 @@ void need_gpu(const Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), name, " must be a GPU tensor: bergson_amd has no CPU path (got device ", t.device(), ")");
 }
 
+// The kernels form no tangents, and an output without one is a derivative of zero to forward mode.  A gradient recorded
+// for the backward pass refuses by itself; a call that records none (frozen parameters, no_grad) would not.
+void no_tangent(const Tensor& t, const char* name) {
+  if (t.defined() && t._fw_grad(/*level=*/0).defined())
+    C10_THROW_ERROR(NotImplementedError, c10::str(name, " carries a tangent: forward-mode derivatives are not supported"));
+}
+
 void same_device(const Tensor& ref, const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.device() == ref.device(), name, " lives on ", t.device(), ", the input on ", ref.device());
 }
@@ -152,6 +159,9 @@ Tensor layer_norm(const Tensor& x, const optional<Tensor>& weight_in, const opti
   vector(weight, "weight");
   if (bias.defined()) vector(bias, "bias");
   TORCH_CHECK_VALUE(eps >= 0.0 && eps < INFINITY, "eps=", eps, " must be finite and not negative");
+  no_tangent(x, "x");
+  no_tangent(weight, "weight");
+  no_tangent(bias, "bias");
   need_gpu(x, "x");
   same_device(x, weight, "weight");
   if (bias.defined()) same_device(x, bias, "bias");
@@ -283,6 +293,9 @@ Tensor causal_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
     TORCH_CHECK_VALUE(!cu.defined(),
                       "cu_seqlens go with packed [T, heads, D] inputs; a batch [N, S, heads, D] takes lengths");
   }
+  no_tangent(q, "q");
+  no_tangent(k, "k");
+  no_tangent(v, "v");
   need_gpu(q, "q");
   same_device(q, k, "k");
   same_device(q, v, "v");
@@ -375,6 +388,8 @@ Tensor topk_distillation(const Tensor& logits, const Tensor& teacher_ids, const 
   if (valid.defined())
     TORCH_CHECK_VALUE(valid.scalar_type() == at::kBool && valid.sizes() == lead, "valid must be bool ", lead, ", got ",
                       valid.scalar_type(), " ", valid.sizes());
+  no_tangent(logits, "logits");
+  no_tangent(teacher_logits, "teacher_logits");
   need_gpu(logits, "logits");
   same_device(logits, teacher_ids, "teacher_ids");
   same_device(logits, teacher_logits, "teacher_logits");

@@ -6,7 +6,7 @@ bergson/collector/collector.py:926-985).  The arithmetic is the library's (inclu
 allocation and the autograd nodes are native too (csrc/torch_ops.cpp).  Everything is enqueued on torch's current
 stream of the tensors' device, allocates through torch only (so that a graph capture owns its memory), keeps nothing
 between calls and can be captured (a backward pass as torch has it: into leaves that no graph built before the
-capture still holds); gradients are not differentiable again.
+capture still holds); gradients are not differentiable again, and inputs with forward-mode tangents are refused.
 """
 from __future__ import annotations
 

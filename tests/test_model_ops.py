@@ -98,6 +98,36 @@ def test_topk_distillation_refusals():
         B.topk_distillation(z, ids, t, valid=torch.ones(2, dtype=torch.bool))
 
 
+def _plain_calls():
+    x, w = torch.zeros(3, 8), torch.ones(8)
+    q = torch.zeros(2, 5, 4, 16)
+    ids, t = torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 2)
+    return {"layer_norm": (B.layer_norm, (x, w, w.clone())),
+            "causal_attention": (B.causal_attention, (q, q.clone(), q.clone())),
+            "topk_distillation": (lambda z, t: B.topk_distillation(z, ids, t), (torch.zeros(3, 10), t))}
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("which", ["layer_norm", "causal_attention", "topk_distillation"])
+def test_forward_mode_derivatives_are_refused(which, grad):
+    """Every input's tangent: dropped, it would come out as a derivative of zero.  Also while no graph is recorded
+    (forward mode does not ask for one), and from torch.func.jvp."""
+    import torch.autograd.forward_ad as fwd
+
+    fn, args = _plain_calls()[which]
+    for i in range(len(args)):
+        with fwd.dual_level(), torch.set_grad_enabled(grad):
+            dual = [fwd.make_dual(a, torch.ones_like(a)) if j == i else a for j, a in enumerate(args)]
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                fn(*dual)
+        with pytest.raises(NotImplementedError, match="forward-mode"), torch.set_grad_enabled(grad):
+            torch.func.jvp(lambda a: fn(*args[:i], a, *args[i + 1:]), (args[i],), (torch.ones_like(args[i]),))
+    with fwd.dual_level():
+        dual = [fwd.make_dual(a, torch.ones_like(a)) for a in args]
+        with pytest.raises(RuntimeError, match="no CPU path"):     # what carries no tangent goes on to the other checks
+            fn(*(fwd.unpack_dual(d).primal for d in dual))
+
+
 def test_struct_layouts_match_the_header():
     # three pointers, int64, five int32, one float
     assert C.sizeof(_lib.AttentionShape) == 3 * 8 + 8 + 5 * 4 + 4
