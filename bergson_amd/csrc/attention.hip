@@ -60,7 +60,7 @@ struct AttnArgs {
   float* sum;             // [Hq][rows]
   void* rest;             // [rows][Hq][D], 16-bit types: o minus its rounded value, rounded
   float* delta;           // [Hq][rows]
-  float* peak;            // [Hq][rows]: largest |do| of the row (fp16 only)
+  float* peak;            // [Hq][rows]: no |dS| of the row is larger (fp16 only)
   float* part_k;          // [rows][Hq][D]: dk and dv of every query head by itself (attention_backward_join_kernel),
   float* part_v;          // NULL where a workgroup sums over the heads that share its keys
   const int4* table;      // packed: {first row, length, tile, limit} per tile of rows, heaviest first
@@ -219,8 +219,9 @@ struct Work {
   // sequence of two rows shows that of its one dS in every gradient): there both go in as two operands, the rounded
   // value and the rest, which gives them 16 or more bits.
   static constexpr bool FINE = RW == 1 && sizeof(T) == 2;
-  // waves a SIMD has room for without spilling registers to memory (the compiler's budget: 512 / 2 or 512)
-  static constexpr int PER_SIMD_Q = sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : (RW == 4 || DP <= 64 ? 2 : 1);
+  // waves a SIMD has room for without spilling registers to memory in the walk (the compiler's budget: 512 / 3, / 2 or
+  // 512; fp16's dq at heads of 64 keeps a few outside it: 73 us with two waves where three take 63, as above)
+  static constexpr int PER_SIMD_Q = sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 64 && RW == 4 ? 3 : (RW == 4 || DP <= 64 ? 2 : 1);
   static constexpr int PER_SIMD_KV = sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : (DP <= 64 || WAVES == 8 ? 2 : 1);
   static constexpr int BYTES = STEP * Tile<T, DP>::PITCH;
   static constexpr int BUFFERS = 4 * BYTES <= 65536 ? 2 : 1;  // two workgroups of a CU fit at 16 bits
@@ -610,7 +611,17 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
 }
 
 // ---- backward: queries -------------------------------------------------------------------------------------------
-// dq of 32 queries a wave; also leaves delta (and, for fp16, the largest |do| of a row) for the other kernel.
+// dq of 32 queries a wave; also leaves delta (and, for fp16, a bound of the row's |dS|) for the other kernel.
+//
+// fp16 holds numbers of 2^-14 to 2^16, and dS may be of any size: small with the gradients, large with the values, small
+// where the weights spread.  A row's dS is at most its largest |dp - delta| times the largest weight that a shift
+// which lags by 2^8 and the weights' sum allow.  It carries the power of two that brings this bound to 2^12, set by the row's first
+// block and, with what has been summed, lowered when a later one brings the bound past 2^15: what is lost among
+// the subnormals is 2^-37 of the bound.  The power stands in the exponent of P, at no cost; what this takes is the
+// largest of 16 values a block and a vote (24 documents of 16 to 2048 positions, 16 heads of 64: 58 -> 63 us).
+constexpr int DS_FIRST = 12, DS_MOST = 15;
+constexpr float DS_LIFT_MAX = 60.f;  // fp32 keeps weights up to 2^8 times |do| |v| of 2^40 times that
+
 template <typename T, int DP, int RW, bool BRIEF = false>
 __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void attention_backward_q_kernel(AttnArgs A) {
   using M = Attn<T>;
@@ -637,11 +648,11 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
   const int64_t stat = (int64_t)qh * A.rows + it.stat + row;
   // everything the walk starts with is on its way before the first value is used
   load_own<T, DP, W::ROWS>(attn_rows<T>(A.grad_o, it, qh) + first * A.grad_o.tok, A.grad_o.tok, own, left, A.D, lane, gf);
-  const float kept_shift = in ? A.shift[stat] : 0.f, sum = in ? A.sum[stat] : 1.f;
+  const float shift = in ? A.shift[stat] : 0.f, sum = in ? A.sum[stat] : 1.f;
   Staged<T, DP, BK> sk, sv;
   sk.init(A.k.tok, A.D);
   sv.init(A.v.tok, A.D);
-  float delta = 0.f, peak = 0.f;
+  float delta = 0.f;
   {
     uint4 of[KS], rf[KS];
     load_own<T, DP, W::ROWS>(attn_rows<T>(A.o, it, qh) + first * A.o.tok, A.o.tok, own, left, A.D, lane, of);
@@ -662,29 +673,16 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
         for (int e = 0; e < M::EPL; ++e) a[e] += r[e];
       }
 #pragma unroll
-      for (int e = 0; e < M::EPL; ++e) {
-        delta = fmaf(a[e], b[e], delta);
-        peak = fmaxf(peak, fabsf(b[e]));
-      }
+      for (int e = 0; e < M::EPL; ++e) delta = fmaf(a[e], b[e], delta);
     }
-    const float2 d = both_halves(delta), p = both_halves(peak);
+    const float2 d = both_halves(delta);
     delta = d.x + d.y;
-    peak = fmaxf(p.x, p.y);
   }
-  if (in && half == 0 && part == 0) {
-    A.delta[stat] = delta;
-    if constexpr (HALF) A.peak[stat] = peak;
-  }
-  // dS is P times something of the size of do: with small gradients it would fall among fp16's subnormals.  The
-  // row's power of two is taken out of it (in the exponent of P, at no cost) and put back on dq.  So is the one that
-  // brings the weights, which are not divided by their sum here and reach 2^8 (the shift may lag that far), below 1:
-  // dS then stays within 4 sum_d |v_d|.
-  float lift = 0.f;
-  if constexpr (HALF) {
-    lift = peak > 0.f && peak < INFINITY ? -(float)ilogbf(peak) : 0.f;
-    lift -= sum < 256.f ? (float)(ilogbf(sum) + 1) : 8.f;
-  }
-  const float shift = kept_shift - lift, over_sum = 1.0f / sum;
+  if (in && half == 0 && part == 0) A.delta[stat] = delta;
+  // fp16: the power of two of dS stands in `arg` (as far as fp32 holds their sum: it is what arg and the shift say, to the
+  // end); `room` is the |dp - delta| it has room for, `most` the largest so far
+  float arg = -shift, room = 0.f, most = 0.f;
+  const float over_sum = 1.0f / sum, heaviest = fminf(sum, 256.f);
   const float c = A.scale * AT_LOG2E;
   f32x16 dq[DT];
 #pragma unroll
@@ -720,11 +718,35 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
           Mma32<T>::mma(read_rows<T, DP>(tk, u * 32, ks, lane), qf[ks], s);
           Mma32<T>::mma(read_rows<T, DP>(tv, u * 32, ks, lane), gf[ks], dp);
         }
+        // a sequence's first row has one key and a constant softmax: its dS is 0, not the rounding of dp - delta
+        const bool diagonal = k0 + u * 32 + 31 > mine;
+        const int last = (row == 0 ? -1 : row) - k0 - u * 32 - 4 * half;
+        if constexpr (HALF) {
+          if (diagonal) {  // what is not seen does not count
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = exp2_of(fmaf(s[i], c, -shift)) * dp[i];
-        if (k0 + u * 32 + 31 > mine) {
-          // a sequence's first row has one key and a constant softmax: its dS is 0, not the rounding of dp - delta
-          const int last = (row == 0 ? -1 : row) - k0 - u * 32 - 4 * half;
+            for (int i = 0; i < 16; ++i)
+              if (8 * (i / 4) + i % 4 > last) dp[i] = 0.f;
+          }
+          float big = most;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(dp[i]));
+          const float2 halves = both_halves(big);
+          most = fmaxf(halves.x, halves.y);
+          if (__any(most > room)) {
+            const bool change = most > room && most < INFINITY;
+            const float lift = fminf((float)(DS_FIRST - ilogbf(most * heaviest)), DS_LIFT_MAX);
+            const float to = change ? lift - shift : arg, f = exp2_of(to - arg);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) dq[dt][i] *= f;
+            arg = to;
+            if (change) room = exp2_of(DS_MOST - lift) / heaviest;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = exp2_of(fmaf(s[i], c, arg)) * dp[i];
+        if (diagonal) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             if (8 * (i / 4) + i % 4 > last) s[i] = 0.f;
@@ -750,10 +772,28 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
       sv.store(next + W::BYTES);
     }
   }
+  float unlift = 1.f;
+  if constexpr (HALF) {
+    unlift = exp2_of(-(arg + shift));
+    if constexpr (W::SPLIT > 1) {  // the waves' powers of two may differ
+      __shared__ float largest[AT_WAVES][WAVE];
+      largest[wave][lane] = most;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dq[dt][i] *= unlift;
+      unlift = 1.f;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < W::SPLIT; ++w) most = fmaxf(most, largest[w * RW + wave % RW][lane]);
+    }
+    // (a row with infinities has no dS that would have to fit)
+    if (in && half == 0 && part == 0) A.peak[stat] = most < INFINITY ? most * heaviest * over_sum : 0.f;
+  }
   join_waves<W, DT>(dq, lds, part, wave % RW, lane);
   if (part > 0) return;
   T* out = attn_row<T>(A.dq, it, qh, row);
-  store_rows<T, DP>(out, nullptr, dq, A.scale * over_sum * exp2_of(-lift), in, A.D, lane);
+  store_rows<T, DP>(out, nullptr, dq, A.scale * over_sum * unlift, in, A.D, lane);
   if (!in && row < it.limit) zero_row<T, DP>(out, A.D, lane);
 }
 
@@ -859,8 +899,8 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
       if constexpr (sizeof(T) == 4) stats[b][2][threadIdx.x] = 1.0f / sum;
     }
   };
-  // fp16: dS carries a power of two that keeps it out of the subnormals, the one that fits the largest |do| seen so
-  // far; when a tile brings a larger one, what has been summed is rescaled (exactly) to the new power.
+  // fp16: dS carries a power of two here too, the one that brings the largest of the rows' bounds so far to 2^14; when a
+  // tile brings a larger one, what has been summed is rescaled (exactly) to the new power.
   int lift = 0;
   bool lifted = false;
   sq.init(A.q.tok, A.D);
@@ -883,7 +923,7 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
       if constexpr (HALF) {
         const float peak = wave_max(st[2][skip + lane % (SUB * 32)]);
         if (peak > 0.f && peak < INFINITY) {
-          const int want = -ilogbf(peak);
+          const int want = min(DS_MOST - 1 - ilogbf(peak), (int)DS_LIFT_MAX);
           if (!lifted || want < lift) {
             if (lifted) {
               const float f = exp2_of((float)(want - lift));

@@ -74,8 +74,10 @@ def norm_reference(x, weight, bias, eps, dy, out_dtype, w_dtype):
     return out
 
 
-def attention_reference(q, k, v, scale, do, dtype):
-    """One sequence, q [L, H, D], k and v [L, Hk, D] -> {name: (value, bound)} of o and, with do, dq, dk, dv."""
+def attention_reference(q, k, v, scale, do, dtype, ds_floor=None):
+    """One sequence, q [L, H, D], k and v [L, Hk, D] -> {name: (value, bound)} of o and, with do, dq, dk, dv.
+    ds_floor: what dS in fp16 may lose beside its relative rounding, in units of the largest |dp - delta| of its row
+    (dq) or sequence (dk); by default a multiple of the largest |do|."""
     h = half_step(dtype)
     q, k, v = (t.detach().cpu().double().transpose(0, 1) for t in (q, k, v))
     group = q.shape[0] // k.shape[0]
@@ -106,12 +108,17 @@ def attention_reference(q, k, v, scale, do, dtype):
     e_ds = (rel_p + h + 4 * U) * ds.abs() + p * (e_dp + e_delta)
     # the same loss of a probability below 2^-126, times dp - delta, and of dS itself
     e_ds = e_ds + torch.where(past, torch.finfo(torch.float32).tiny * ((dp - delta).abs() + 1), 0.0)
+    row_floor = floor = 0.0
     if dtype == torch.float16:
         # dS is rounded as a multiple of 2^-24 times the power of two nearest below the tile's largest |do|
-        e_ds = e_ds + torch.where(past, tiny(dtype) * 2 * do.abs().amax(), 0.0)
+        row_floor = floor = tiny(dtype) * 2 * do.abs().amax()
+        if ds_floor is not None:
+            gap = torch.where(past, (dp - delta).abs(), 0.0)
+            row_floor, floor = ds_floor * gap.amax(2, keepdim=True), ds_floor * gap.amax()
+    e_ds_q, e_ds_k = (e_ds + torch.where(past, f, 0.0) for f in (row_floor, floor))
     absq, absk = q.abs(), kq.abs()
-    dq, e_dq = ds @ kq * scale, (e_ds + (L + 8) * U * ds.abs()) @ absk * scale
-    dk, e_dk = ds.transpose(1, 2) @ q * scale, (e_ds + (group * L + 8) * U * ds.abs()).transpose(1, 2) @ absq * scale
+    dq, e_dq = ds @ kq * scale, (e_ds_q + (L + 8) * U * ds.abs()) @ absk * scale
+    dk, e_dk = ds.transpose(1, 2) @ q * scale, (e_ds_k + (group * L + 8) * U * ds.abs()).transpose(1, 2) @ absq * scale
     e_p = p * (rel_p + h + (group * L + 8) * U) + torch.where(past, tiny(dtype), 0.0)
     dv, e_dv = p.transpose(1, 2) @ do, e_p.transpose(1, 2) @ do.abs()
     fold = lambda t: t.unflatten(0, (-1, group)).sum(1)

@@ -317,6 +317,56 @@ def test_attention_large_values_in_fp16(device, bgx_env, rows):
     _check_sequences(q, k, v, do, out, grads, [(0, 260)], 1.0, torch.float16)
 
 
+# dS in fp16 goes in with the bound of its row (dq) or tile (dk) brought to 2^12 or more: what is rounded as a multiple
+# of 2^-24 loses at most 2^-25 2^-12 of that bound, which is no more than the largest |dp - delta|
+DS_FLOOR = 2.0 ** -37
+
+
+@pytest.mark.parametrize("rows", [128, 64, 32])
+def test_attention_ds_past_fp16(device, bgx_env, rows):
+    """Two positions whose dS is +-625 while the output gradients are small: dq is 156.25 and dk 0, though dS in
+    units of the output gradient's size does not fit fp16."""
+    bgx_env("BGX_ATTENTION_ROWS", rows)
+    sign = torch.tensor([1.0, -1.0], device=device).reshape(2, 1, 1)
+    ones = torch.ones(2, 1, 64, device=device)
+    q, k, v, do = ((t * ones).half() for t in (0.0, sign, 5000.0 * sign, 2.0 ** -8))
+    for t in (q, k, v):
+        t.requires_grad_()
+    cu = torch.tensor([0, 2], dtype=torch.int32, device=device)
+    out = B.causal_attention(q, k, v, cu_seqlens=cu)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), do)
+    assert (dq[0] == 0).all() and (dq[1] == 156.25).all() and (dk == 0).all()
+    _check_sequences(q, k, v, do, out, (dq, dk, dv), [(0, 2)], 0.125, torch.float16)
+
+
+@pytest.mark.parametrize("rows", [128, 64, 32])
+@pytest.mark.parametrize("size", ["thousands", "growing", "falling", "small"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 1, 64), (1, 1, 128)], ids=str)
+def test_attention_ds_of_any_size_in_fp16(device, bgx_env, heads, kv_heads, dim, size, rows):
+    """Values in the thousands under small output gradients, values that grow or fall by 2^20 along the sequence, and
+    small ones under weights that are spread over the sequence: dS is far from the size of the output gradients."""
+    bgx_env("BGX_ATTENTION_ROWS", rows)
+    L = 300
+    q, k, v, do = (t.float() for t in _qkv((L,), heads, kv_heads, dim, torch.float16, dim + rows, device, gain=0.8))
+    steps = torch.linspace(-10, 10, L, device=device).reshape(L, 1, 1)
+    if size == "thousands":
+        v, do = v * 4000, do * 2.0 ** -8
+    elif size == "small":
+        v, k, do = v * 2.0 ** -13, k * 64, do * 16
+    else:
+        v, do = v * 2.0 ** (steps if size == "growing" else -steps), do * 2.0 ** -4
+    q, k, v, do = (t.half() for t in (q, k, v, do))
+    scale = dim ** -0.5 * (2.0 ** -6 if size == "small" else 1.0)
+    assert all(t.isfinite().all() for t in (q, k, v, do))
+    for t in (q, k, v):
+        t.requires_grad_()
+    out = B.causal_attention(q, k, v, cu_seqlens=torch.tensor([0, L], dtype=torch.int32, device=device), scale=scale)
+    grads = torch.autograd.grad(out, (q, k, v), do)
+    ref = attention_reference(*(t.detach() for t in (q, k, v)), scale, do, torch.float16, ds_floor=DS_FLOOR)
+    for name, got in zip(("o", "dq", "dk", "dv"), (out, *grads)):
+        assert_within(got, *ref[name], name)
+
+
 @pytest.mark.parametrize("rows", [128, 32])
 def test_attention_offsets_past_32_bits(device, bgx_env, rows):
     """Positions 2 MiB apart: the sequence spans more than 4 GiB of each operand, a tile far less."""
