@@ -816,6 +816,9 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
   constexpr bool FINE = W::FINE || BRIEF;       // dS as two operands
   constexpr bool OWN = W::THREADS > AT_THREADS;  // k and v of the workgroup's keys live in LDS
   constexpr bool HALF = std::is_same<T, f16_t>::value;
+  // fp16: P goes in 2^14 times its value, or the weights of long flat sequences would be subnormal numbers (at 32768
+  // positions alike dv was 2.5 times as far off as its own rounding; 2^14 leaves room for a P that rounding takes past 1)
+  constexpr float P_LIFT = HALF ? 14.f : 0.f;
   constexpr int BQ = W::STEP, KS = DP / (2 * M::EPL), SUB = W::SUB, G = 32 / M::GROUP, DT = DP / 32;
   constexpr int KEEP = OWN ? W::ROWS * Tile<T, DP>::PITCH : 0;
   __shared__ __attribute__((aligned(16))) char lds[W::LDS];
@@ -893,7 +896,7 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
     if (threadIdx.x < BQ) {
       const float sum = stage[2] == 0.f ? 1.f : stage[2];  // rows past the end read as zeros
       // at 16 bits the sum joins the exponent (its rounding there is far below that of the weights); in fp32 it does not
-      stats[b][0][threadIdx.x] = sizeof(T) == 2 ? stage[0] + log2f(sum) : stage[0];
+      stats[b][0][threadIdx.x] = sizeof(T) == 2 ? stage[0] + log2f(sum) - P_LIFT : stage[0];
       stats[b][1][threadIdx.x] = stage[1];
       if constexpr (HALF) stats[b][2][threadIdx.x] = stage[3];
       if constexpr (sizeof(T) == 4) stats[b][2][threadIdx.x] = 1.0f / sum;
@@ -936,7 +939,7 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
             lifted = true;
           }
         }
-        raise = exp2_of((float)lift);
+        raise = exp2_of((float)lift - P_LIFT);
       }
 #pragma unroll 1
       for (int u = 0; u < SUB; ++u) {
@@ -1012,13 +1015,13 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
   join_waves<W, DT>(dk, lds, part, wave % RW, lane);
   join_waves<W, DT>(dv, lds, part, wave % RW, lane);
   if (part > 0) return;
-  const float scale = A.scale * exp2_of(-(float)lift);
+  const float scale = A.scale * exp2_of(-(float)lift), scale_v = exp2_of(-P_LIFT);
   if (alone) {
     store_rows<float, DP>(A.part_k + part_row, nullptr, dk, scale, in, A.D, lane);
-    store_rows<float, DP>(A.part_v + part_row, nullptr, dv, 1.0f, in, A.D, lane);
+    store_rows<float, DP>(A.part_v + part_row, nullptr, dv, scale_v, in, A.D, lane);
   } else {
     store_rows<T, DP>(attn_row<T>(A.dk, it, kvh, row), nullptr, dk, scale, in, A.D, lane);
-    store_rows<T, DP>(attn_row<T>(A.dv, it, kvh, row), nullptr, dv, 1.0f, in, A.D, lane);
+    store_rows<T, DP>(attn_row<T>(A.dv, it, kvh, row), nullptr, dv, scale_v, in, A.D, lane);
   }
   if (!in && row < it.limit) clear();
 }
