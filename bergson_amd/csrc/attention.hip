@@ -823,7 +823,7 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
   constexpr int KEEP = OWN ? W::ROWS * Tile<T, DP>::PITCH : 0;
   __shared__ __attribute__((aligned(16))) char lds[W::LDS];
   __shared__ __attribute__((aligned(16))) char keep[OWN ? 2 * KEEP : 16];
-  constexpr int NSTAT = std::is_same<T, bf16_t>::value ? 2 : 3;
+  constexpr int NSTAT = HALF ? 4 : 3;
   __shared__ __attribute__((aligned(16))) float stats[W::BUFFERS][NSTAT][BQ];
   AttnItem it;
   int kvh, qh0;
@@ -895,11 +895,10 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
     sg.store(lds + b * 2 * W::BYTES + W::BYTES);
     if (threadIdx.x < BQ) {
       const float sum = stage[2] == 0.f ? 1.f : stage[2];  // rows past the end read as zeros
-      // at 16 bits the sum joins the exponent (its rounding there is far below that of the weights); in fp32 it does not
-      stats[b][0][threadIdx.x] = sizeof(T) == 2 ? stage[0] + log2f(sum) - P_LIFT : stage[0];
+      stats[b][0][threadIdx.x] = stage[0];
       stats[b][1][threadIdx.x] = stage[1];
-      if constexpr (HALF) stats[b][2][threadIdx.x] = stage[3];
-      if constexpr (sizeof(T) == 4) stats[b][2][threadIdx.x] = 1.0f / sum;
+      stats[b][2][threadIdx.x] = exp2_of(P_LIFT) / sum;  // a factor of its own: see AttnArgs
+      if constexpr (HALF) stats[b][3][threadIdx.x] = stage[3];
     }
   };
   // fp16: dS carries a power of two here too, the one that brings the largest of the rows' bounds so far to 2^14; when a
@@ -924,7 +923,7 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
     if (q0 + SUB * 32 > mine && mine < it.len) {
       float raise = 1.f;
       if constexpr (HALF) {
-        const float peak = wave_max(st[2][skip + lane % (SUB * 32)]);
+        const float peak = wave_max(st[3][skip + lane % (SUB * 32)]);
         if (peak > 0.f && peak < INFINITY) {
           const int want = min(DS_MOST - 1 - ilogbf(peak), (int)DS_LIFT_MAX);
           if (!lifted || want < lift) {
@@ -945,17 +944,13 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
       for (int u = 0; u < SUB; ++u) {
         if (q0 + u * 32 + 31 < mine) continue;  // all of these queries come before this wave's keys
         f32x16 s, dp;
-        float lse[16], over_sum[sizeof(T) == 4 ? 16 : 1];
+        float shift[16];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           const float4 a = *reinterpret_cast<const float4*>(&st[0][skip + u * 32 + 8 * b + 4 * half]);
           const float4 d = *reinterpret_cast<const float4*>(&st[1][skip + u * 32 + 8 * b + 4 * half]);
-          lse[4 * b] = a.x, lse[4 * b + 1] = a.y, lse[4 * b + 2] = a.z, lse[4 * b + 3] = a.w;
+          shift[4 * b] = a.x, shift[4 * b + 1] = a.y, shift[4 * b + 2] = a.z, shift[4 * b + 3] = a.w;
           dp[4 * b] = -d.x, dp[4 * b + 1] = -d.y, dp[4 * b + 2] = -d.z, dp[4 * b + 3] = -d.w;
-          if constexpr (sizeof(T) == 4) {
-            const float4 w = *reinterpret_cast<const float4*>(&st[2][skip + u * 32 + 8 * b + 4 * half]);
-            over_sum[4 * b] = w.x, over_sum[4 * b + 1] = w.y, over_sum[4 * b + 2] = w.z, over_sum[4 * b + 3] = w.w;
-          }
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = 0.f;
@@ -970,10 +965,18 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
           }
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[i] = exp2_of(fmaf(s[i], c, -lse[i]));
-          if constexpr (sizeof(T) == 4) s[i] *= over_sum[i];
-          dp[i] = HALF ? s[i] * raise * dp[i] : s[i] * dp[i];
+        for (int b = 0; b < 4; ++b) {
+          // read here and no earlier: beside the products there are no registers for it at heads of 128 (2 x 4096 positions,
+          // 32 / 8 heads, bf16: 691 us with the read in front of them, 638 where the compiler puts it, 598 this way)
+          __builtin_amdgcn_sched_barrier(0);
+          const float4 w = *reinterpret_cast<const float4*>(&st[2][skip + u * 32 + 8 * b + 4 * half]);
+          const float over_sum[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = 4 * b + e;
+            s[i] = exp2_of(fmaf(s[i], c, -shift[i])) * over_sum[e];
+            dp[i] = HALF ? s[i] * raise * dp[i] : s[i] * dp[i];
+          }
         }
         if (q0 + u * 32 < mine + 31) {
           const int first_query = row - q0 - u * 32 - 4 * half;

@@ -407,19 +407,21 @@ def test_attention_gradients_of_short_sequences(device, length, dim, dtype):
         assert (got.cpu().double() - want).norm() <= 1.05 * rounding, name
 
 
-def _flat_case(L, dim, dtype, offset, device):
-    """One sequence whose scores are all alike: q and k share no dimension but the first, where q k = offset^2.  Returns
-    the inputs and o, dq, dk, dv of the definition in 64 bits, which has a closed form: the weights of row i are
-    1 / (i + 1).  (dq's first column is left out: there the dS of a row, which add up to zero, are all that is added.)"""
+def _flat_inputs(L, dim, dtype, offset, device):
+    """One sequence whose scores are all alike: q and k share no dimension but the first, where q k = offset^2."""
     g = _gen(L + dim)
     q, k, v, do = (torch.zeros(L, dim, dtype=torch.float64) for _ in range(4))
     q[:, 1:32] = torch.randn(L, 31, generator=g)
     k[:, 32:] = torch.randn(L, dim - 32, generator=g)
     q[:, 0] = k[:, 0] = offset
     v[:], do[:] = torch.randn(L, dim, generator=g), torch.randn(L, dim, generator=g)
-    q, k, v, do = (t.to(dtype) for t in (q, k, v, do))
-    inputs = [t.unsqueeze(1).to(device) for t in (q, k, v, do)]
-    q, k, v, do = (t.double() for t in (q, k, v, do))
+    return [t.to(dtype).unsqueeze(1).to(device) for t in (q, k, v, do)]
+
+
+def _flat_results(q, k, v, do, dtype):
+    """o, dq, dk, dv of the definition in 64 bits, which has a closed form: the weights of row i are 1 / (i + 1)."""
+    q, k, v, do = (t[:, 0].cpu().double() for t in (q, k, v, do))
+    L, dim = q.shape
     seen = torch.arange(1, L + 1, dtype=torch.float64).reshape(L, 1)
     o = v.cumsum(0) / seen
     delta = (do * o).sum(1, keepdim=True)
@@ -432,39 +434,56 @@ def _flat_case(L, dim, dtype, offset, device):
         dk[:, d] = (back(w * do) * v).sum(1) - back(w * delta)[:, 0]
     # dv with every weight rounded to 2^-8 or 2^-11 of its value, whatever its size
     rounded = (2.0 ** 14 / seen).to(dtype).double() * 2.0 ** -14
-    return inputs, {"o": o, "dq": dq, "dk": dk, "dv": back(do / seen), "rounded dv": back(rounded * do)}
-
-
-def _check_flat(device, L, dim, dtype, offset, rows):
-    """What the operands' roundings cost, against the results' own.  Of dq and dk: a row's or column's dS have random signs,
-    so that the sum of their roundings has the size of one rounding of the sum, and the two are independent: 2^(1/2) of
-    it.  Of dv: a row has one weight for all its keys, whose rounding error comes back in the whole column sum behind it;
-    a few dozen of such errors (of the last rows, in 64 or 128 columns) make the norm, which then varies by a tenth from
-    case to case.  So dv is held to what the exact weights' roundings make of these inputs.  In the 32-row workgroups,
-    whose operands keep their rests, 1 for all of them.  A twentieth on top for what else is fp32."""
-    (q, k, v, do), want = _flat_case(L, dim, dtype, offset, device)
-    for t in (q, k, v):
-        t.requires_grad_()
-    out = B.causal_attention(q, k, v, cu_seqlens=torch.tensor([0, L], dtype=torch.int32, device=device), scale=1.0)
-    grads = torch.autograd.grad(out, (q, k, v), do)
-    for name, got in zip(("o", "dq", "dk", "dv"), (out, *grads)):
-        got, ref = got[:, 0].detach().cpu().double(), want[name]
-        if name == "dq":
-            got, ref = got[:, 32:], ref[:, 32:]
-        error, rounding, most = got - ref, ref.to(dtype).double() - ref, 1.05 * (1.0 if rows == 32 else 2 ** 0.5)
-        if name == "dv" and rows != 32:
-            rounding, most = want["rounded dv"].to(dtype).double() - ref, 1.05
-        for part in (slice(None), slice(L // 2, None)):    # the later half has the smallest weights only
-            assert error[part].norm() <= most * rounding[part].norm(), (name, float(error[part].norm() / rounding[part].norm()))
+    return {"o": o, "dq": dq, "dk": dk, "dv": back(do / seen), "rounded dv": back(rounded * do)}
 
 
 @pytest.mark.parametrize("rows", [128, 64, 32])
 @pytest.mark.parametrize("dtype", DTYPES[:2], ids=ids_of)
 @pytest.mark.parametrize("L,dim", [(32768, 64), (16384, 128)], ids=str)
 def test_attention_of_long_flat_sequences(device, bgx_env, L, dim, dtype, rows):
-    """Weights of 2^-15: dk and dv are made from operands below fp16's normal numbers."""
+    """Weights of 2^-15: dk and dv are made from operands below fp16's normal numbers.
+
+    What the operands' roundings cost, against the results' own, in the later half (the smallest weights, and values of one
+    size: the first rows alone would make the norms of all).  Of dq and dk: a row's or column's dS have random signs, so that the sum
+    of their roundings has the size of one rounding of the sum, and the two are independent: 2^(1/2) of it.  Of dv: a row
+    has one weight for all its keys, whose rounding error comes back in the whole column sum behind it; a few dozen of such
+    errors (of the last rows, in 64 or 128 columns) make the norm, which then varies by a tenth from case to case.  So dv
+    is held to what the exact weights' roundings make of these inputs.  In the 32-row workgroups, whose operands keep their
+    rests, 1 for all of them.  A twentieth on top for what else is fp32."""
     bgx_env("BGX_ATTENTION_ROWS", rows)
-    _check_flat(device, L, dim, dtype, 0.0, rows)
+    q, k, v, do = _flat_inputs(L, dim, dtype, 0.0, device)
+    want = _flat_results(q, k, v, do, dtype)
+    for t in (q, k, v):
+        t.requires_grad_()
+    out = B.causal_attention(q, k, v, cu_seqlens=torch.tensor([0, L], dtype=torch.int32, device=device), scale=1.0)
+    grads = torch.autograd.grad(out, (q, k, v), do)
+    for name, got in zip(("o", "dq", "dk", "dv"), (out, *grads)):
+        got, ref = got[L // 2:, 0].detach().cpu().double(), want[name][L // 2:]
+        rounding, most = ref.to(dtype).double() - ref, 1.0 if rows == 32 else 2 ** 0.5
+        if name == "dv" and rows != 32:
+            rounding, most = want["rounded dv"][L // 2:].to(dtype).double() - ref, 1.0
+        ratio = float((got - ref).norm() / rounding.norm())
+        assert ratio <= 1.05 * most, (name, ratio)
+
+
+@pytest.mark.parametrize("rows", [128, 64, 32])
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_large_flat_scores(device, bgx_env, dim, dtype, rows):
+    """Scores that are all 2^16 give the bits of scores that are all 0, in every gradient: products, exponents and weights
+    are exact in fp32 in both, whatever a shift of that size would lose in one number with the logarithm of the sum."""
+    bgx_env("BGX_ATTENTION_ROWS", rows)
+    cu, results = torch.tensor([0, 600], dtype=torch.int32, device=device), []
+    for offset in (0.0, 256.0):
+        q, k, v, do = _flat_inputs(600, dim, dtype, offset, device)
+        for t in (q, k, v):
+            t.requires_grad_()
+        out = B.causal_attention(q, k, v, cu_seqlens=cu, scale=1.0)
+        dq, dk, dv = torch.autograd.grad(out, (q, k, v), do)
+        # the dimension of the offset itself apart
+        results.append({"o": out, "dq": dq[..., 1:], "dk": dk[..., 1:], "dv": dv})
+    for name, first in results[0].items():
+        assert torch.equal(first, results[1][name]), name
 
 
 def test_attention_plan_of_many_sequences(device):
