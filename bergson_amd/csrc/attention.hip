@@ -1187,8 +1187,8 @@ static AttnArgs attn_args(const bgx_attention_shape* a) {
 // are with 128 rows (2 x 2048, 8 key/value heads: 2653 / 1201 / 2510) and have no such variant.
 // 16-bit sequences of up to 64 rows on average take workgroups of 128 rows however many there are, unless they take 32
 // (forward and backward of sequences of 64 / 32 / 8 positions, 4096 in all, 8 heads of 128, 128 against 64 rows:
-// 59 and 65, 71 and 94, 211 and 299 us; 12 heads of 64: the same).  Where gradients are wanted, P in the forward pass
-// and dS go in as two operands (Work): dq and dk of 2 to 8 positions are 1.5 to 1.6 times as far off as their own
+// 59 and 65, 71 and 94, 211 and 299 us; 12 heads of 64: the same).  P in the forward pass
+// and dS go in as two operands there (Work): dq and dk of 2 to 8 positions are 1.5 to 1.6 times as far off as their own
 // rounding without that, 1.0 times with it (3 to 8 % of the time); of 64 and more 1.45 times.
 static bool attn_brief(const bgx_attention_shape* a) {
   return a->dtype != BGX_F32 && a->rows <= 64 * (int64_t)a->n_seqs;
@@ -1358,7 +1358,7 @@ int attention_forward_impl(const bgx_attention_shape* a, const bgx_attention_row
   A.o = attn_view(o);
   attn_saved(A, a, saved);
   int which;
-  const bool brief = saved != nullptr && attn_brief(a);  // its gain is the gradients'
+  const bool brief = attn_brief(a);  // its gain is the gradients', but the output has the same bits with and without them
   const unsigned grid = attn_grid(A, a, ATTN_FORWARD, &which);
   BGX_REQUIRE(grid > 0, BGX_E_SHAPE, "attention: %lld rows of %d heads", (long long)a->rows, a->heads);
   BGX_ATTN_LAUNCH(attention_forward_kernel, a->dtype, a->head_dim, which, grid, (hipStream_t)stream, A);

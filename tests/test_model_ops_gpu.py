@@ -486,6 +486,17 @@ def test_attention_of_large_flat_scores(device, bgx_env, dim, dtype, rows):
         assert torch.equal(first, results[1][name]), name
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("length,n", [(3, 90), (48, 40), (64, 80), (65, 80), (300, 30)], ids=str)
+def test_attention_output_does_not_depend_on_a_graph(device, dtype, length, n):
+    """The same bits while a gradient is recorded and while none is (a checkpointed block runs both)."""
+    q, k, v, _ = _qkv((n * length,), 8, 4, 64, dtype, length, device)
+    cu = torch.arange(0, n * length + 1, length, dtype=torch.int32, device=device)
+    plain = B.causal_attention(q, k, v, cu_seqlens=cu)
+    kept = B.causal_attention(q.requires_grad_(), k, v, cu_seqlens=cu)
+    assert kept.requires_grad and torch.equal(plain, kept)
+
+
 def test_attention_plan_of_many_sequences(device):
     """More sequences than the planning workgroup has threads, empty ones among them, long ones at the end."""
     g = _gen(2)
