@@ -17,7 +17,7 @@
 // Scores, softmax statistics, probabilities' sums and all accumulators are fp32.  For 16-bit inputs P and dS are
 // rounded to the inputs' type as operands of the matrix instructions (the products of 16-bit operands are what runs
 // at the card's rate; each rounding is relative to the value, and their sum over a row averages out; small calls and
-// the gradients of short sequences keep the rests, see Work and attn_brief).  delta is formed from o as it was before its
+// short sequences keep the rests, see Work).  delta is formed from o as it was before its
 // rounding: dp - delta cancels.
 //
 // What bounds them: a 32 x 32 block of scores costs a wave 16 exponentials a lane beside 2 (forward), 3 (dq) or 4 (dk,
@@ -210,6 +210,7 @@ struct Staged {
 // STEP rows.  RW = 4: every wave owns 32 rows and takes each tile whole.  RW = 2, 1: two or all four waves share 32
 // rows, each takes its part of every tile, and their sums are joined through LDS at the end -- more workgroups with
 // shorter walks, at twice or four times the traffic to LDS: for calls that would not fill the chip otherwise.
+constexpr int AT_SHORT = 64;
 template <typename T, int DP, int RW, int WAVES = AT_WAVES>
 struct Work {
   static constexpr int THREADS = WAVES * WAVE, ROWS = 32 * RW, SPLIT = WAVES / RW;
@@ -219,6 +220,13 @@ struct Work {
   // sequence of two rows shows that of its one dS in every gradient): there both go in as two operands, the rounded
   // value and the rest, which gives them 16 or more bits.
   static constexpr bool FINE = RW == 1 && sizeof(T) == 2;
+  // Elsewhere P (in the forward pass) and dS of 16-bit sequences of up to AT_SHORT rows go in like that, whatever the call holds
+  // beside them: dq and dk of 2 to 8 positions are 1.5 to 1.6 times as far off as their own rounding without it, 1.0 times
+  // with it; of 64 and more 1.45 times.  A workgroup of a kernel for calls that may hold such sequences (MIXED) goes by
+  // its own sequence's length and then runs a body without a walk (SHORT).  (Second products behind a branch in one body
+  // spill the registers of the walk.  24 documents of 16 to 2048 positions, 16 heads of 64, bf16, forward, dq, dk and dv:
+  // 42, 56 and 80 us in a kernel without the short body, 43, 57 and 82 with it.)
+  static_assert(sizeof(T) == 4 || STEP >= AT_SHORT || RW == 1, "a short sequence is one tile");
   // waves a SIMD has room for without spilling registers to memory in the walk (the compiler's budget: 512 / 3, / 2 or
   // 512; fp16's dq at heads of 64 keeps a few outside it: 73 us with two waves where three take 63, as above)
   static constexpr int PER_SIMD_Q = sizeof(T) == 4 ? (DP <= 32 ? 2 : 1) : DP <= 64 && RW == 4 ? 3 : (RW == 4 || DP <= 64 ? 2 : 1);
@@ -453,17 +461,15 @@ __device__ inline void load_own(const T* base, int64_t tok, int row, int rows, i
 __device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ---- forward -----------------------------------------------------------------------------------------------------
-// BRIEF: P (here) and dS (in the backward kernels) as two operands whatever RW is (see attn_brief).
-template <typename T, int DP, int RW, bool BRIEF = false>
-__global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void attention_forward_kernel(AttnArgs A) {
+// SHORT: of a sequence of up to AT_SHORT rows, MIXED: for the kernel that has both kinds (here and in the backward pass; see
+// Work).  MIXED only keeps the code of the two kernels apart: shared between them, the compiler spilled registers in
+// both (dq of 2 x 4096 positions, 32 / 8 heads of 128, bf16: 428 -> 480 us).
+template <typename T, int DP, int RW, bool MIXED, bool SHORT>
+__device__ __forceinline__ void forward_rows(const AttnArgs& A, const AttnItem& it, int kvh, int qh, char* lds) {
   using M = Attn<T>;
   using W = Work<T, DP, RW>;
-  constexpr bool FINE = W::FINE || BRIEF;
+  constexpr bool FINE = W::FINE || SHORT;
   constexpr int BK = W::STEP, KS = DP / (2 * M::EPL), SUB = W::SUB, G = 32 / M::GROUP, DT = DP / 32;
-  __shared__ __attribute__((aligned(16))) char lds[W::LDS];
-  AttnItem it;
-  int kvh, qh;
-  if (!attn_item<W::ROWS>(A, false, it, kvh, qh)) return;
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
   const int part = wave / RW;  // which of the waves that share rows
   const int first = it.tile * W::ROWS, mine = first + (wave % RW) * 32, row = mine + (lane & 31), half = lane >> 5;
@@ -483,7 +489,7 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
   float m = -INFINITY, l = 0.f;
   const float c = A.scale * AT_LOG2E;
-  const int n_tiles = (min(first + W::ROWS, it.len) + BK - 1) / BK;
+  const int n_tiles = SHORT ? 1 : (min(first + W::ROWS, it.len) + BK - 1) / BK;
   Staged<T, DP, BK> sk, sv;
   sk.init(A.k.tok, A.D);
   sv.init(A.v.tok, A.D);
@@ -610,6 +616,22 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
   if (!in && row < it.limit) zero_row<T, DP>(out, A.D, lane);
 }
 
+template <typename T, int DP, int RW, bool MIXED>
+__global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void attention_forward_kernel(AttnArgs A) {
+  using W = Work<T, DP, RW>;
+  __shared__ __attribute__((aligned(16))) char lds[W::LDS];
+  AttnItem it;
+  int kvh, qh;
+  if (!attn_item<W::ROWS>(A, false, it, kvh, qh)) return;
+  if constexpr (MIXED) {
+    if (it.len <= AT_SHORT) {
+      forward_rows<T, DP, RW, MIXED, true>(A, it, kvh, qh, lds);
+      return;
+    }
+  }
+  forward_rows<T, DP, RW, MIXED, false>(A, it, kvh, qh, lds);
+}
+
 // ---- backward: queries -------------------------------------------------------------------------------------------
 // dq of 32 queries a wave; also leaves delta (and, for fp16, a bound of the row's |dS|) for the other kernel.
 //
@@ -622,21 +644,17 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
 constexpr int DS_FIRST = 12, DS_MOST = 15;
 constexpr float DS_LIFT_MAX = 60.f;  // fp32 keeps weights up to 2^8 times |do| |v| of 2^40 times that
 
-template <typename T, int DP, int RW, bool BRIEF = false>
-__global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void attention_backward_q_kernel(AttnArgs A) {
+template <typename T, int DP, int RW, bool MIXED, bool SHORT>
+__device__ __forceinline__ void backward_q_rows(const AttnArgs& A, const AttnItem& it, int kvh, int qh, char* lds) {
   using M = Attn<T>;
   using W = Work<T, DP, RW>;
-  constexpr bool FINE = W::FINE || BRIEF;
+  constexpr bool FINE = W::FINE || SHORT;
   constexpr bool HALF = std::is_same<T, f16_t>::value;
   constexpr int BK = W::STEP, KS = DP / (2 * M::EPL), SUB = W::SUB, G = 32 / M::GROUP, DT = DP / 32;
-  __shared__ __attribute__((aligned(16))) char lds[W::LDS];
-  AttnItem it;
-  int kvh, qh;
-  if (!attn_item<W::ROWS>(A, false, it, kvh, qh)) return;
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
   const int part = wave / RW;  // which of the waves that share rows
   const int first = it.tile * W::ROWS, mine = first + (wave % RW) * 32, row = mine + (lane & 31), half = lane >> 5;
-  if (first >= it.len) {
+  if (first >= it.len) {  // nothing of the sequence in this tile
     if (row < it.limit) zero_row<T, DP>(attn_row<T>(A.dq, it, qh, row), A.D, lane);
     return;
   }
@@ -689,7 +707,7 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dq[dt][i] = 0.f;
-  const int n_tiles = (min(first + W::ROWS, it.len) + BK - 1) / BK;
+  const int n_tiles = SHORT ? 1 : (min(first + W::ROWS, it.len) + BK - 1) / BK;
   sk.store(lds);
   sv.store(lds + W::BYTES);
   for (int t = 0; t < n_tiles; ++t) {
@@ -705,7 +723,7 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
     const char* tv = tk + W::BYTES;
     const int k0 = t * BK + part * (SUB * 32);
     if (k0 <= mine + 31 && mine < it.len) {
-#pragma unroll DP > 96 ? 1 : SUB
+#pragma unroll DP > 96 || (HALF && MIXED && DP == 64) ? 1 : SUB  // registers
       for (int u = 0; u < SUB; ++u) {
         f32x16 s, dp;
 #pragma unroll
@@ -797,6 +815,22 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
   if (!in && row < it.limit) zero_row<T, DP>(out, A.D, lane);
 }
 
+template <typename T, int DP, int RW, bool MIXED>
+__global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void attention_backward_q_kernel(AttnArgs A) {
+  using W = Work<T, DP, RW>;
+  __shared__ __attribute__((aligned(16))) char lds[W::LDS];
+  AttnItem it;
+  int kvh, qh;
+  if (!attn_item<W::ROWS>(A, false, it, kvh, qh)) return;
+  if constexpr (MIXED) {
+    if (it.len <= AT_SHORT) {
+      backward_q_rows<T, DP, RW, MIXED, true>(A, it, kvh, qh, lds);
+      return;
+    }
+  }
+  backward_q_rows<T, DP, RW, MIXED, false>(A, it, kvh, qh, lds);
+}
+
 // ---- backward: keys and values -----------------------------------------------------------------------------------
 // Wide heads at 16 bits with enough keys (RW = 4, DP > 64): dk and dv of 32 keys take half of a wave's registers, and with
 // k, v and a tile on its way in the other half only one wave fits a SIMD, which then waits for every LDS read and every
@@ -808,42 +842,53 @@ constexpr int kv_waves() {
   return RW == 4 && DP > 64 && sizeof(T) == 2 ? 8 : AT_WAVES;
 }
 
-template <typename T, int DP, int RW, bool BRIEF = false>
-__global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
-                             (Work<T, DP, RW, kv_waves<T, DP, RW>()>::PER_SIMD_KV)) void attention_backward_kv_kernel(AttnArgs A) {
-  using M = Attn<T>;
+// What the workgroup has in LDS.
+template <typename T, int DP, int RW>
+struct KvStore {
   using W = Work<T, DP, RW, kv_waves<T, DP, RW>()>;
-  constexpr bool FINE = W::FINE || BRIEF;       // dS as two operands
-  constexpr bool OWN = W::THREADS > AT_THREADS;  // k and v of the workgroup's keys live in LDS
+  static constexpr bool OWN = W::THREADS > AT_THREADS;  // k and v of the workgroup's keys live here
+  static constexpr int KEEP = OWN ? W::ROWS * Tile<T, DP>::PITCH : 0;
+  static constexpr int NSTAT = std::is_same<T, f16_t>::value ? 4 : 3;
+  __attribute__((aligned(16))) char lds[W::LDS];
+  __attribute__((aligned(16))) char keep[OWN ? 2 * KEEP : 16];
+  __attribute__((aligned(16))) float stats[W::BUFFERS][NSTAT][W::STEP];
+};
+
+// dk and dv of one key tile become zero: of the key/value head, or the parts of one query head (alone)
+template <typename T, int DP>
+__device__ inline void clear_kv(const AttnArgs& A, const AttnItem& it, int kvh, int qh, int row, int lane) {
+  if (A.part_k != nullptr) {
+    const int64_t part_row = ((it.stat + row) * A.Hq + qh) * A.D;
+    zero_row<float, DP>(A.part_k + part_row, A.D, lane);
+    zero_row<float, DP>(A.part_v + part_row, A.D, lane);
+  } else {
+    zero_row<T, DP>(attn_row<T>(A.dk, it, kvh, row), A.D, lane);
+    zero_row<T, DP>(attn_row<T>(A.dv, it, kvh, row), A.D, lane);
+  }
+}
+
+template <typename T, int DP, int RW, bool MIXED, bool SHORT>
+__device__ __forceinline__ void backward_kv_rows(const AttnArgs& A, const AttnItem& it, int kvh, int qh0, KvStore<T, DP, RW>& store_in) {
+  using M = Attn<T>;
+  using Store = KvStore<T, DP, RW>;
+  using W = typename Store::W;
+  constexpr bool FINE = W::FINE || SHORT;  // dS as two operands
+  constexpr bool OWN = Store::OWN;
   constexpr bool HALF = std::is_same<T, f16_t>::value;
   // fp16: P goes in 2^14 times its value, or the weights of long flat sequences would be subnormal numbers (at 32768
   // positions alike dv was 2.5 times as far off as its own rounding; 2^14 leaves room for a P that rounding takes past 1)
   constexpr float P_LIFT = HALF ? 14.f : 0.f;
   constexpr int BQ = W::STEP, KS = DP / (2 * M::EPL), SUB = W::SUB, G = 32 / M::GROUP, DT = DP / 32;
-  constexpr int KEEP = OWN ? W::ROWS * Tile<T, DP>::PITCH : 0;
-  __shared__ __attribute__((aligned(16))) char lds[W::LDS];
-  __shared__ __attribute__((aligned(16))) char keep[OWN ? 2 * KEEP : 16];
-  constexpr int NSTAT = HALF ? 4 : 3;
-  __shared__ __attribute__((aligned(16))) float stats[W::BUFFERS][NSTAT][BQ];
-  AttnItem it;
-  int kvh, qh0;
-  if (!attn_item<W::ROWS>(A, true, it, kvh, qh0)) return;
+  constexpr int KEEP = Store::KEEP;
+  char *lds = store_in.lds, *keep = store_in.keep;
+  auto& stats = store_in.stats;
   const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
   const int part = wave / RW;  // which of the waves that share rows
   const int first = it.tile * W::ROWS, mine = first + (wave % RW) * 32, row = mine + (lane & 31), half = lane >> 5;
   const bool alone = A.part_k != nullptr;  // one query head of the group
   const int64_t part_row = ((it.stat + row) * A.Hq + qh0) * A.D;
-  auto clear = [&]() {
-    if (alone) {
-      zero_row<float, DP>(A.part_k + part_row, A.D, lane);
-      zero_row<float, DP>(A.part_v + part_row, A.D, lane);
-    } else {
-      zero_row<T, DP>(attn_row<T>(A.dk, it, kvh, row), A.D, lane);
-      zero_row<T, DP>(attn_row<T>(A.dv, it, kvh, row), A.D, lane);
-    }
-  };
   if (first >= it.len) {
-    if (row < it.limit) clear();
+    if (row < it.limit) clear_kv<T, DP>(A, it, kvh, qh0, row, lane);
     return;
   }
   const bool in = row < it.len;
@@ -869,7 +914,7 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
 #pragma unroll
     for (int i = 0; i < 16; ++i) dk[dt][i] = dv[dt][i] = 0.f;
   const float c = A.scale * AT_LOG2E;
-  const int t0 = first / BQ, per_head = (it.len + BQ - 1) / BQ - t0, n_tiles = alone ? per_head : per_head * A.group;
+  const int t0 = SHORT ? 0 : first / BQ, per_head = SHORT ? 1 : (it.len + BQ - 1) / BQ - t0, n_tiles = alone ? per_head : per_head * A.group;
   Staged<T, DP, BQ, W::THREADS> sq, sg;
   float stage[4];
   // tile t is tile t % per_head of the queries, for query head t / per_head of the group
@@ -1026,7 +1071,24 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
     store_rows<T, DP>(attn_row<T>(A.dk, it, kvh, row), nullptr, dk, scale, in, A.D, lane);
     store_rows<T, DP>(attn_row<T>(A.dv, it, kvh, row), nullptr, dv, scale_v, in, A.D, lane);
   }
-  if (!in && row < it.limit) clear();
+  if (!in && row < it.limit) clear_kv<T, DP>(A, it, kvh, qh0, row, lane);
+}
+
+template <typename T, int DP, int RW, bool MIXED>
+__global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
+                             (Work<T, DP, RW, kv_waves<T, DP, RW>()>::PER_SIMD_KV)) void attention_backward_kv_kernel(AttnArgs A) {
+  using W = typename KvStore<T, DP, RW>::W;
+  __shared__ KvStore<T, DP, RW> store;
+  AttnItem it;
+  int kvh, qh;
+  if (!attn_item<W::ROWS>(A, true, it, kvh, qh)) return;
+  if constexpr (MIXED) {
+    if (it.len <= AT_SHORT) {
+      backward_kv_rows<T, DP, RW, MIXED, true>(A, it, kvh, qh, store);
+      return;
+    }
+  }
+  backward_kv_rows<T, DP, RW, MIXED, false>(A, it, kvh, qh, store);
 }
 
 // dk and dv of every key/value head: the sums over its query heads in their order, rounded once.  One thread per 16
@@ -1187,11 +1249,15 @@ static AttnArgs attn_args(const bgx_attention_shape* a) {
 // are with 128 rows (2 x 2048, 8 key/value heads: 2653 / 1201 / 2510) and have no such variant.
 // 16-bit sequences of up to 64 rows on average take workgroups of 128 rows however many there are, unless they take 32
 // (forward and backward of sequences of 64 / 32 / 8 positions, 4096 in all, 8 heads of 128, 128 against 64 rows:
-// 59 and 65, 71 and 94, 211 and 299 us; 12 heads of 64: the same).  P in the forward pass
-// and dS go in as two operands there (Work): dq and dk of 2 to 8 positions are 1.5 to 1.6 times as far off as their own
-// rounding without that, 1.0 times with it (3 to 8 % of the time); of 64 and more 1.45 times.
+// 59 and 65, 71 and 94, 211 and 299 us; 12 heads of 64: the same).
 static bool attn_brief(const bgx_attention_shape* a) {
-  return a->dtype != BGX_F32 && a->rows <= 64 * (int64_t)a->n_seqs;
+  return a->dtype != BGX_F32 && a->rows <= AT_SHORT * (int64_t)a->n_seqs;
+}
+
+// Whether sequences of up to AT_SHORT rows may be among the call's, as far as the host can tell.
+static bool attn_mixed(const bgx_attention_shape* a) {
+  const bool one_width = a->plan_dev == nullptr && a->cu_seqlens_dev == nullptr && a->lengths_dev == nullptr;
+  return a->dtype != BGX_F32 && !(one_width && a->rows > AT_SHORT * (int64_t)a->n_seqs);
 }
 
 enum AttnKernel { ATTN_FORWARD, ATTN_Q, ATTN_KV };
@@ -1235,21 +1301,6 @@ static AttnView attn_view(const bgx_attention_rows* t) {
   return v;
 }
 
-// 128 rows, BRIEF
-template <typename T, int DP>
-static void attention_forward_kernel_brief(unsigned grid, hipStream_t s, const AttnArgs& A) {
-  if constexpr (sizeof(T) == 2) attention_forward_kernel<T, DP, 4, true><<<grid, AT_THREADS, 0, s>>>(A);
-}
-template <typename T, int DP>
-static void attention_backward_q_kernel_brief(unsigned grid, hipStream_t s, const AttnArgs& A) {
-  if constexpr (sizeof(T) == 2) attention_backward_q_kernel<T, DP, 4, true><<<grid, AT_THREADS, 0, s>>>(A);
-}
-template <typename T, int DP>
-static void attention_backward_kv_kernel_brief(unsigned grid, hipStream_t s, const AttnArgs& A) {
-  if constexpr (sizeof(T) == 2)
-    attention_backward_kv_kernel<T, DP, 4, true><<<grid, kv_waves<T, DP, 4>() * WAVE, 0, s>>>(A);
-}
-
 // the tallest variant of each kernel and its threads
 template <typename T, int DP>
 constexpr int attention_forward_kernel_tall() {
@@ -1278,14 +1329,18 @@ constexpr int attention_backward_kv_kernel_threads() {
 
 #define BGX_ATTN_ROWS(KERNEL, T, DP, WHICH, GRID, S, A)                    \
   do {                                                                     \
-    if ((WHICH) == 0 && brief)                                             \
-      KERNEL##_brief<T, DP>((GRID), (S), A);                               \
+    constexpr int tall = KERNEL##_tall<T, DP>(), threads = KERNEL##_threads<T, DP>(); \
+    constexpr bool can = sizeof(T) == 2; /* fp32 has nothing to decide */  \
+    if ((WHICH) == 0 && mixed)                                             \
+      KERNEL<T, DP, tall, can><<<(GRID), threads, 0, (S)>>>(A);            \
     else if ((WHICH) == 0)                                                 \
-      KERNEL<T, DP, KERNEL##_tall<T, DP>()><<<(GRID), KERNEL##_threads<T, DP>(), 0, (S)>>>(A); \
+      KERNEL<T, DP, tall, false><<<(GRID), threads, 0, (S)>>>(A);          \
+    else if ((WHICH) == 1 && mixed)                                        \
+      KERNEL<T, DP, 2, can><<<(GRID), AT_THREADS, 0, (S)>>>(A);            \
     else if ((WHICH) == 1)                                                 \
-      KERNEL<T, DP, 2><<<(GRID), AT_THREADS, 0, (S)>>>(A);                 \
+      KERNEL<T, DP, 2, false><<<(GRID), AT_THREADS, 0, (S)>>>(A);          \
     else                                                                   \
-      KERNEL<T, DP, 1><<<(GRID), AT_THREADS, 0, (S)>>>(A);                 \
+      KERNEL<T, DP, 1, false><<<(GRID), AT_THREADS, 0, (S)>>>(A);          \
   } while (0)
 #define BGX_ATTN_WIDTHS(KERNEL, T, D, WHICH, GRID, S, A)      \
   do {                                                        \
@@ -1358,7 +1413,7 @@ int attention_forward_impl(const bgx_attention_shape* a, const bgx_attention_row
   A.o = attn_view(o);
   attn_saved(A, a, saved);
   int which;
-  const bool brief = attn_brief(a);  // its gain is the gradients', but the output has the same bits with and without them
+  const bool mixed = attn_mixed(a);
   const unsigned grid = attn_grid(A, a, ATTN_FORWARD, &which);
   BGX_REQUIRE(grid > 0, BGX_E_SHAPE, "attention: %lld rows of %d heads", (long long)a->rows, a->heads);
   BGX_ATTN_LAUNCH(attention_forward_kernel, a->dtype, a->head_dim, which, grid, (hipStream_t)stream, A);
@@ -1412,7 +1467,7 @@ int attention_backward_impl(const bgx_attention_shape* a, const bgx_attention_ro
   BGX_REQUIRE((uintptr_t)ws % 16 == 0, BGX_E_ALIGN, "attention backward: workspace not aligned to 16 bytes");
   hipStream_t s = (hipStream_t)stream;
   int which;
-  const bool brief = attn_brief(a);
+  const bool mixed = attn_mixed(a);
   unsigned grid = attn_grid(A, a, ATTN_Q, &which);
   BGX_REQUIRE(grid > 0, BGX_E_SHAPE, "attention backward: %lld rows of %d heads", (long long)a->rows, a->heads);
   BGX_ATTN_LAUNCH(attention_backward_q_kernel, a->dtype, a->head_dim, which, grid, s, A);

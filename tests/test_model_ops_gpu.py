@@ -497,6 +497,44 @@ def test_attention_output_does_not_depend_on_a_graph(device, dtype, length, n):
     assert kept.requires_grad and torch.equal(plain, kept)
 
 
+def _rounding_ratios(q, k, v, do, grads, spans, scale, dtype):
+    """How far dq and dk of the given rows are from the definition, in units of their own rounding."""
+    flat = lambda t: t.detach().reshape(-1, *t.shape[-2:])
+    q, k, v, do = map(flat, (q, k, v, do))
+    refs = [attention_reference(q[a:b], k[a:b], v[a:b], scale, do[a:b], dtype) for a, b in spans]
+    for got, name in zip(map(flat, grads), ("dq", "dk")):
+        want = torch.cat([r[name][0] for r in refs])
+        got = torch.cat([got[a:b] for a, b in spans]).cpu().double()
+        yield name, float((got - want).norm() / (want.to(dtype).double() - want).norm())
+
+
+@pytest.mark.parametrize("rows", [128, 64, 32])
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=ids_of)
+@pytest.mark.parametrize("length,dim", [(2, 64), (5, 128)], ids=str)
+def test_attention_gradients_of_short_sequences_beside_long_ones(device, bgx_env, length, dim, dtype, rows):
+    """A short document's gradients are as near as in a call of short documents (the bound of
+    test_attention_gradients_of_short_sequences), whatever it is packed or padded with."""
+    bgx_env("BGX_ATTENTION_ROWS", rows)
+    n, scale = 80, dim ** -0.5
+    T = n * length + 9000
+    q, k, v, do = _qkv((T,), 4, 2, dim, dtype, length, device, gain=1.0)
+    ends = list(range(0, n * length + 1, length))
+    for t in (q, k, v):
+        t.requires_grad_()
+    out = B.causal_attention(q, k, v, cu_seqlens=torch.tensor(ends + [T], dtype=torch.int32, device=device))
+    grads = torch.autograd.grad(out, (q, k), do)
+    for name, ratio in _rounding_ratios(q, k, v, do, grads, list(zip(ends, ends[1:])), scale, dtype):
+        assert ratio <= 1.05, (name, ratio, "packed")
+    q, k, v, do = _qkv((n, 130), 4, 2, dim, dtype, length, device, gain=1.0)
+    for t in (q, k, v):
+        t.requires_grad_()
+    out = B.causal_attention(q, k, v, lengths=torch.full((n,), length, dtype=torch.int32, device=device))
+    grads = torch.autograd.grad(out, (q, k), do)
+    spans = [(i * 130, i * 130 + length) for i in range(n)]
+    for name, ratio in _rounding_ratios(q, k, v, do, grads, spans, scale, dtype):
+        assert ratio <= 1.05, (name, ratio, "padded")
+
+
 def test_attention_plan_of_many_sequences(device):
     """More sequences than the planning workgroup has threads, empty ones among them, long ones at the end."""
     g = _gen(2)
