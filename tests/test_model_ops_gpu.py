@@ -551,6 +551,77 @@ def test_attention_plan_of_many_sequences(device):
     assert (out[ends[-1]:] == 0).all()
 
 
+def test_attention_plan_with_folded_levels(device):
+    """More tiles than the planning workgroup has threads, so that a level is several tile indices: every tile of every
+    sequence once, higher levels first, then the rows outside the sequences."""
+    from bergson_amd import _lib
+
+    lengths, head, rows = [70000, 5, 0, 40000, 129, 20000], 17, 140000
+    ends = [head]
+    for l in lengths:
+        ends.append(ends[-1] + l)
+    lib, bounds = _lib.load(), torch.tensor(ends, dtype=torch.int32, device=device)
+    nbytes = lib.bgx_attention_plan_bytes(rows, len(lengths))
+    plan = torch.full((nbytes,), 0x55, dtype=torch.uint8, device=device)
+    _lib.check(lib.bgx_attention_plan(bounds.data_ptr(), len(lengths), rows, plan.data_ptr(), nbytes,
+                                      torch.cuda.current_stream().cuda_stream), "plan")
+    table, at = plan.cpu().view(torch.int32).reshape(-1, 4).tolist(), 0
+    for height in (128, 64, 32):
+        tiles, n = lambda l: -(-l // height), rows // height + len(lengths) + 2
+        entries, at = [tuple(e) for e in table[at:at + n]], at + n
+        fold = 0
+        while tiles(rows) >> fold >= 1024:
+            fold += 1
+        assert fold > 0 or height != 128
+        want = [(a, l, t, l) for a, l in zip(ends, lengths) for t in range(tiles(l))]
+        work = entries[:len(want)]
+        assert sorted(work) == sorted(want)
+        levels = [t >> fold for _, _, t, _ in work]
+        assert levels == sorted(levels, reverse=True)
+        clear = ([(0, 0, i, head) for i in range(tiles(head))]
+                 + [(ends[-1], 0, i, rows - ends[-1]) for i in range(tiles(rows - ends[-1]))])
+        assert entries[len(want):] == clear + [(0, 0, 0, 0)] * (n - len(want) - len(clear))
+
+
+def test_attention_of_folded_levels(device, bgx_env):
+    """Documents packed into more than 1024 tiles of 32 rows: the bits of a call of each document by itself."""
+    bgx_env("BGX_ATTENTION_ROWS", 32)
+    lengths = [20000, 5, 0, 15000, 7001]
+    q, k, v, do = _qkv((sum(lengths),), 4, 4, 32, torch.bfloat16, 40, device)
+    ends = [0] + torch.tensor(lengths).cumsum(0).tolist()
+
+    def run(q, k, v, do, ends):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = B.causal_attention(*leaves, cu_seqlens=torch.tensor(ends, dtype=torch.int32, device=device))
+        return (out.detach(), *torch.autograd.grad(out, leaves, do))
+
+    packed = run(q, k, v, do, ends)
+    for a, b in zip(ends, ends[1:]):
+        if b > a:
+            for whole, alone in zip(packed, run(q[a:b], k[a:b], v[a:b], do[a:b], [0, b - a])):
+                assert torch.equal(whole[a:b], alone)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_many_tiles(device, bgx_env, dim, dtype):
+    """2048 rows, scores and output gradients growing along them, so that maxima move on and the powers of two in fp16's dS
+    are lowered many times: outputs and gradients against the definition, in every workgroup height."""
+    L = 2048
+    q, k, v, do = (t.float() for t in _qkv((L,), 2, 1, dim, dtype, dim, device, gain=1.0))
+    along = torch.linspace(0, 1, L, device=device).reshape(L, 1, 1)
+    q, k, v, do = (t.to(dtype) for t in (q, k * (0.25 + 4 * along), v, do * 2.0 ** (12 * along - 6)))
+    for t in (q, k, v):
+        t.requires_grad_()
+    ref = attention_reference(*(t.detach() for t in (q, k, v)), dim ** -0.5, do, dtype)
+    cu = torch.tensor([0, L], dtype=torch.int32, device=device)
+    for rows in (128, 64, 32):
+        bgx_env("BGX_ATTENTION_ROWS", rows)
+        out = B.causal_attention(q, k, v, cu_seqlens=cu)
+        for name, got in zip(("o", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, (q, k, v), do))):
+            assert_within(got, *ref[name], f"{name} with {rows} rows")
+
+
 def test_attention_malformed_boundaries_stay_in_bounds(device):
     """Boundaries that are not ascending or lie outside the rows: nothing is promised of the rows, but the call ends,
     and a following call on the same memory is right."""
@@ -940,6 +1011,30 @@ def test_differentiable_once(device, which):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     with pytest.raises(RuntimeError, match="differentiable once"):
         got[0].float().sum().backward()
+
+
+@pytest.mark.parametrize("which", ["norm", "attention", "distill"])
+def test_saved_tensors_may_travel(device, which):
+    """What a forward pass saves may be packed away and brought back by saved-tensor hooks."""
+    fn, leaves, grad = _calls(device)[which]
+    leaves = [t.requires_grad_() for t in leaves]
+    want = torch.autograd.grad(fn(*leaves), leaves, grad)
+    with torch.autograd.graph.save_on_cpu():
+        out = fn(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, grad), want))
+
+
+@pytest.mark.parametrize("which", ["norm", "attention", "distill"])
+def test_transforms_are_refused(device, which):
+    """torch.func's vmap and grad hand over tensors without memory of their own: an error, and nothing is launched."""
+    fn, leaves, grad = _calls(device)[which]
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(fn)(*(torch.stack([t, t]) for t in leaves))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda *a: fn(*a).float().sum())(*leaves)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(fn, tuple(leaves), tuple(torch.ones_like(t) for t in leaves))
+    torch.cuda.synchronize()
 
 
 @pytest.mark.parametrize("rows", [128, 64, 32])
