@@ -830,7 +830,9 @@ def forward_loss_factory(cfg: IndexConfig) -> Callable:
         raise ValueError("label_smoothing belongs to the cross-entropy loss, not to loss_fn='topk_kl'")
 
     def run_model(model, x: Tensor, batch: dict) -> Tensor:
-        if not cfg.fused_model_ops:
+        # a checkpointed block runs again on the backward pass' threads, where the lengths are not known: it runs on the
+        # padding, whose outputs nothing sees
+        if not cfg.fused_model_ops or (model.training and getattr(model, "is_gradient_checkpointing", False)):
             return model(x).logits
         lengths = torch.tensor([len(seq) for seq in batch["input_ids"]], dtype=torch.int32)
         with sequence_lengths(lengths.to(x.device, non_blocking=True)):

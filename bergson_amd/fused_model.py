@@ -34,7 +34,11 @@ _current = threading.local()
 @contextmanager
 def sequence_lengths(lengths: Tensor | None):
     """Document lengths (int32 [N] on the GPU) of the right-padded batch whose forward pass runs inside: fused
-    attention then skips the padding.  Per thread; None changes nothing."""
+    attention then skips the padding.  Per thread; None changes nothing.
+
+    Not with activation checkpointing: a checkpointed block runs again on the backward pass' threads, outside this
+    context, and torch refuses what it then saves (CheckpointError).  Without the lengths it is right, too: attention is
+    causal, the padding only costs its time."""
     before = getattr(_current, "lengths", None)
     _current.lengths = lengths
     try:

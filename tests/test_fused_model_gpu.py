@@ -46,6 +46,24 @@ def test_grouped_heads_match_the_library(device):
     assert rel_l2(rows[1], rows[0]) <= 1e-3
 
 
+@pytest.mark.parametrize("overlap", [True, False])
+def test_checkpointed_model(device, overlap):
+    """Activation checkpointing recomputes blocks on the backward pass' threads: the rows of the run without it."""
+    lengths = [50, 130, 7, 90]
+    docs = random_docs(lengths, vocab=500, seed=1)
+    rows = []
+    for checkpointed in (False, True):
+        model = make_llama(torch.float32, device, layers=2, d=128, heads=4, kv_heads=2, mlp=256, vocab=500, seed=3)
+        model.train()
+        if checkpointed:
+            model.gradient_checkpointing_enable({"use_reentrant": False})
+        cfg = B.IndexConfig(run_path="", projection_dim=8, projection_type="normal", fused_model_ops=True)
+        col = B.collect_gradients(model, ListDataset(docs), _processor(8), cfg, batches=[[0, 1], [2, 3]],
+                                  overlap_backward=overlap)
+        rows.append(torch.from_numpy(np.array(col.builder.grad_buffer)))
+    assert rel_l2(rows[1], rows[0]) <= 1e-3
+
+
 def test_sixteen_bit_model(device):
     """bf16: fused and library rows are two roundings of the same fp32 rows -- the fused run is no further from them
     than the library's, up to half as much again."""
