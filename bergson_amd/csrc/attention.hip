@@ -490,6 +490,9 @@ __device__ __forceinline__ void forward_rows(const AttnArgs& A, const AttnItem& 
   float m = -INFINITY, l = 0.f;
   const float c = A.scale * AT_LOG2E;
   const int n_tiles = SHORT ? 1 : (min(first + W::ROWS, it.len) + BK - 1) / BK;
+  // (a guard around the walk lets the compiler put q's loads behind it, and then every tile waits for the next one's: 4 x 1024
+  // positions, 12 heads of 64, in the kernel for sequences of any length: 20.4 us with the guard, 19.4 without)
+  if constexpr (sizeof(T) == 2) __builtin_assume(n_tiles > 0);
   Staged<T, DP, BK> sk, sv;
   sk.init(A.k.tok, A.D);
   sv.init(A.v.tok, A.D);
