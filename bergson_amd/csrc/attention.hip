@@ -205,6 +205,20 @@ struct Staged {
   }
 };
 
+// ---- which sequences a kernel takes ------------------------------------------------------------------------------
+// Short sequences (AT_SHORT) have a body of their own: second products behind a branch in the others' walk would take the
+// walk's registers.  Where the host cannot tell that there are none, one kernel has both bodies (AT_MIXED), which costs the
+// walk some registers all the same, or each has a kernel: AT_BRIEF the first tile of every short sequence, AT_LONG
+// everything else.  A launch more is the better at heads of more than 64 and 128 rows a workgroup.  Measured (us; without
+// the short body / one kernel / two): 24 documents of 16 to 2048 positions, 16 heads of 64, fp16, forward and backward 369 / 385 /
+// 390; 2 x 4096 positions with lengths, 32 / 8 heads of 128, the same 1332 / 1370 / 1337; 1 x 16384, forward 2166 / 2225 / 2203.
+enum AttnKind {
+  AT_ALL,    // fp32, and workgroups that take every sequence like a short one (Work::FINE)
+  AT_LONG,
+  AT_BRIEF,
+  AT_MIXED,
+};
+
 // ---- how a workgroup's waves divide the work ---------------------------------------------------------------------
 // A workgroup owns 32 * RW rows (queries, or keys in the kernel for dk and dv) and walks the other side in tiles of
 // STEP rows.  RW = 4: every wave owns 32 rows and takes each tile whole.  RW = 2, 1: two or all four waves share 32
@@ -222,10 +236,7 @@ struct Work {
   static constexpr bool FINE = RW == 1 && sizeof(T) == 2;
   // Elsewhere P (in the forward pass) and dS of 16-bit sequences of up to AT_SHORT rows go in like that, whatever the call holds
   // beside them: dq and dk of 2 to 8 positions are 1.5 to 1.6 times as far off as their own rounding without it, 1.0 times
-  // with it; of 64 and more 1.45 times.  A workgroup of a kernel for calls that may hold such sequences (MIXED) goes by
-  // its own sequence's length and then runs a body without a walk (SHORT).  (Second products behind a branch in one body
-  // spill the registers of the walk.  24 documents of 16 to 2048 positions, 16 heads of 64, bf16, forward, dq, dk and dv:
-  // 42, 56 and 80 us in a kernel without the short body, 43, 57 and 82 with it.)
+  // with it; of 64 and more 1.45 times.  See AttnKind.
   static_assert(sizeof(T) == 4 || STEP >= AT_SHORT || RW == 1, "a short sequence is one tile");
   // waves a SIMD has room for without spilling registers to memory in the walk (the compiler's budget: 512 / 3, / 2 or
   // 512; fp16's dq at heads of 64 keeps a few outside it: 73 us with two waves where three take 63, as above)
@@ -460,11 +471,17 @@ __device__ inline void load_own(const T* base, int64_t tok, int row, int rows, i
 
 __device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
+template <AttnKind KIND>
+__device__ inline bool leaves_out(const AttnItem& it) {
+  const bool brief = it.tile == 0 && it.len > 0 && it.len <= AT_SHORT;
+  return KIND == AT_LONG ? brief : KIND == AT_BRIEF ? !brief : false;
+}
+
 // ---- forward -----------------------------------------------------------------------------------------------------
-// SHORT: of a sequence of up to AT_SHORT rows, MIXED: for the kernel that has both kinds (here and in the backward pass; see
-// Work).  MIXED only keeps the code of the two kernels apart: shared between them, the compiler spilled registers in
-// both (dq of 2 x 4096 positions, 32 / 8 heads of 128, bf16: 428 -> 480 us).
-template <typename T, int DP, int RW, bool MIXED, bool SHORT>
+// SHORT: of a sequence of up to AT_SHORT rows; KIND: for which kernel (here and in the backward pass).  KIND only keeps the
+// code of the kernels apart: shared between them, the compiler spilled registers in both (dq of 2 x 4096 positions, 32 / 8
+// heads of 128, bf16: 428 -> 480 us).
+template <typename T, int DP, int RW, AttnKind KIND, bool SHORT>
 __device__ __forceinline__ void forward_rows(const AttnArgs& A, const AttnItem& it, int kvh, int qh, char* lds) {
   using M = Attn<T>;
   using W = Work<T, DP, RW>;
@@ -491,8 +508,8 @@ __device__ __forceinline__ void forward_rows(const AttnArgs& A, const AttnItem& 
   const float c = A.scale * AT_LOG2E;
   const int n_tiles = SHORT ? 1 : (min(first + W::ROWS, it.len) + BK - 1) / BK;
   // (a guard around the walk lets the compiler put q's loads behind it, and then every tile waits for the next one's: 4 x 1024
-  // positions, 12 heads of 64, in the kernel for sequences of any length: 20.4 us with the guard, 19.4 without)
-  if constexpr (sizeof(T) == 2) __builtin_assume(n_tiles > 0);
+  // positions, 12 heads of 64, in the kernel of both kinds: 20.4 us with the guard, 19.4 without)
+  if constexpr (KIND == AT_MIXED) __builtin_assume(n_tiles > 0);
   Staged<T, DP, BK> sk, sv;
   sk.init(A.k.tok, A.D);
   sv.init(A.v.tok, A.D);
@@ -619,20 +636,21 @@ __device__ __forceinline__ void forward_rows(const AttnArgs& A, const AttnItem& 
   if (!in && row < it.limit) zero_row<T, DP>(out, A.D, lane);
 }
 
-template <typename T, int DP, int RW, bool MIXED>
+template <typename T, int DP, int RW, AttnKind KIND>
 __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void attention_forward_kernel(AttnArgs A) {
   using W = Work<T, DP, RW>;
   __shared__ __attribute__((aligned(16))) char lds[W::LDS];
   AttnItem it;
   int kvh, qh;
   if (!attn_item<W::ROWS>(A, false, it, kvh, qh)) return;
-  if constexpr (MIXED) {
-    if (it.len <= AT_SHORT) {
-      forward_rows<T, DP, RW, MIXED, true>(A, it, kvh, qh, lds);
+  if (leaves_out<KIND>(it)) return;
+  if constexpr (KIND == AT_MIXED || KIND == AT_BRIEF) {
+    if (KIND == AT_BRIEF || it.len <= AT_SHORT) {
+      forward_rows<T, DP, RW, KIND, true>(A, it, kvh, qh, lds);
       return;
     }
   }
-  forward_rows<T, DP, RW, MIXED, false>(A, it, kvh, qh, lds);
+  if constexpr (KIND != AT_BRIEF) forward_rows<T, DP, RW, KIND, false>(A, it, kvh, qh, lds);
 }
 
 // ---- backward: queries -------------------------------------------------------------------------------------------
@@ -647,7 +665,7 @@ __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void att
 constexpr int DS_FIRST = 12, DS_MOST = 15;
 constexpr float DS_LIFT_MAX = 60.f;  // fp32 keeps weights up to 2^8 times |do| |v| of 2^40 times that
 
-template <typename T, int DP, int RW, bool MIXED, bool SHORT>
+template <typename T, int DP, int RW, AttnKind KIND, bool SHORT>
 __device__ __forceinline__ void backward_q_rows(const AttnArgs& A, const AttnItem& it, int kvh, int qh, char* lds) {
   using M = Attn<T>;
   using W = Work<T, DP, RW>;
@@ -726,7 +744,7 @@ __device__ __forceinline__ void backward_q_rows(const AttnArgs& A, const AttnIte
     const char* tv = tk + W::BYTES;
     const int k0 = t * BK + part * (SUB * 32);
     if (k0 <= mine + 31 && mine < it.len) {
-#pragma unroll DP > 96 || (HALF && MIXED && DP == 64) ? 1 : SUB  // registers
+#pragma unroll DP > 96 || (HALF && KIND == AT_MIXED && DP == 64) ? 1 : SUB  // registers
       for (int u = 0; u < SUB; ++u) {
         f32x16 s, dp;
 #pragma unroll
@@ -818,20 +836,21 @@ __device__ __forceinline__ void backward_q_rows(const AttnArgs& A, const AttnIte
   if (!in && row < it.limit) zero_row<T, DP>(out, A.D, lane);
 }
 
-template <typename T, int DP, int RW, bool MIXED>
+template <typename T, int DP, int RW, AttnKind KIND>
 __global__ __launch_bounds__(AT_THREADS, (Work<T, DP, RW>::PER_SIMD_Q)) void attention_backward_q_kernel(AttnArgs A) {
   using W = Work<T, DP, RW>;
   __shared__ __attribute__((aligned(16))) char lds[W::LDS];
   AttnItem it;
   int kvh, qh;
   if (!attn_item<W::ROWS>(A, false, it, kvh, qh)) return;
-  if constexpr (MIXED) {
-    if (it.len <= AT_SHORT) {
-      backward_q_rows<T, DP, RW, MIXED, true>(A, it, kvh, qh, lds);
+  if (leaves_out<KIND>(it)) return;
+  if constexpr (KIND == AT_MIXED || KIND == AT_BRIEF) {
+    if (KIND == AT_BRIEF || it.len <= AT_SHORT) {
+      backward_q_rows<T, DP, RW, KIND, true>(A, it, kvh, qh, lds);
       return;
     }
   }
-  backward_q_rows<T, DP, RW, MIXED, false>(A, it, kvh, qh, lds);
+  if constexpr (KIND != AT_BRIEF) backward_q_rows<T, DP, RW, KIND, false>(A, it, kvh, qh, lds);
 }
 
 // ---- backward: keys and values -----------------------------------------------------------------------------------
@@ -870,7 +889,7 @@ __device__ inline void clear_kv(const AttnArgs& A, const AttnItem& it, int kvh, 
   }
 }
 
-template <typename T, int DP, int RW, bool MIXED, bool SHORT>
+template <typename T, int DP, int RW, AttnKind KIND, bool SHORT>
 __device__ __forceinline__ void backward_kv_rows(const AttnArgs& A, const AttnItem& it, int kvh, int qh0, KvStore<T, DP, RW>& store_in) {
   using M = Attn<T>;
   using Store = KvStore<T, DP, RW>;
@@ -1077,7 +1096,7 @@ __device__ __forceinline__ void backward_kv_rows(const AttnArgs& A, const AttnIt
   if (!in && row < it.limit) clear_kv<T, DP>(A, it, kvh, qh0, row, lane);
 }
 
-template <typename T, int DP, int RW, bool MIXED>
+template <typename T, int DP, int RW, AttnKind KIND>
 __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
                              (Work<T, DP, RW, kv_waves<T, DP, RW>()>::PER_SIMD_KV)) void attention_backward_kv_kernel(AttnArgs A) {
   using W = typename KvStore<T, DP, RW>::W;
@@ -1085,13 +1104,14 @@ __global__ __launch_bounds__((kv_waves<T, DP, RW>() * WAVE),
   AttnItem it;
   int kvh, qh;
   if (!attn_item<W::ROWS>(A, true, it, kvh, qh)) return;
-  if constexpr (MIXED) {
-    if (it.len <= AT_SHORT) {
-      backward_kv_rows<T, DP, RW, MIXED, true>(A, it, kvh, qh, store);
+  if (leaves_out<KIND>(it)) return;
+  if constexpr (KIND == AT_MIXED || KIND == AT_BRIEF) {
+    if (KIND == AT_BRIEF || it.len <= AT_SHORT) {
+      backward_kv_rows<T, DP, RW, KIND, true>(A, it, kvh, qh, store);
       return;
     }
   }
-  backward_kv_rows<T, DP, RW, MIXED, false>(A, it, kvh, qh, store);
+  if constexpr (KIND != AT_BRIEF) backward_kv_rows<T, DP, RW, KIND, false>(A, it, kvh, qh, store);
 }
 
 // dk and dv of every key/value head: the sums over its query heads in their order, rounded once.  One thread per 16
@@ -1257,10 +1277,23 @@ static bool attn_brief(const bgx_attention_shape* a) {
   return a->dtype != BGX_F32 && a->rows <= AT_SHORT * (int64_t)a->n_seqs;
 }
 
-// Whether sequences of up to AT_SHORT rows may be among the call's, as far as the host can tell.
-static bool attn_mixed(const bgx_attention_shape* a) {
+// What the kernels of a call are: AT_LONG where the host can tell that no sequence is short, AT_BRIEF for that and a second one
+// (in workgroups of 128 rows), AT_MIXED for one that has both.
+static AttnKind attn_kind(const bgx_attention_shape* a) {
   const bool one_width = a->plan_dev == nullptr && a->cu_seqlens_dev == nullptr && a->lengths_dev == nullptr;
-  return a->dtype != BGX_F32 && !(one_width && a->rows > AT_SHORT * (int64_t)a->n_seqs);
+  if (one_width && !attn_brief(a)) return AT_LONG;
+  return a->head_dim > 64 && !attn_brief(a) ? AT_BRIEF : AT_MIXED;
+}
+
+// The launch for short sequences: in the batch layout the first tile of every sequence, else the list of all tiles.
+static AttnArgs attn_brief_args(const AttnArgs& A, unsigned grid, unsigned* few) {
+  AttnArgs B = A;
+  *few = grid;
+  if (A.table == nullptr && A.bounds == nullptr) {
+    *few = grid / (unsigned)A.tiles;
+    B.tiles = 1;
+  }
+  return B;
 }
 
 enum AttnKernel { ATTN_FORWARD, ATTN_Q, ATTN_KV };
@@ -1333,17 +1366,23 @@ constexpr int attention_backward_kv_kernel_threads() {
 #define BGX_ATTN_ROWS(KERNEL, T, DP, WHICH, GRID, S, A)                    \
   do {                                                                     \
     constexpr int tall = KERNEL##_tall<T, DP>(), threads = KERNEL##_threads<T, DP>(); \
-    constexpr bool can = sizeof(T) == 2; /* fp32 has nothing to decide */  \
-    if ((WHICH) == 0 && mixed)                                             \
-      KERNEL<T, DP, tall, can><<<(GRID), threads, 0, (S)>>>(A);            \
+    constexpr bool full = sizeof(T) == 4; /* nothing to decide */          \
+    if ((WHICH) == 0 && kind == AT_MIXED)                                  \
+      KERNEL<T, DP, tall, full ? AT_ALL : AT_MIXED><<<(GRID), threads, 0, (S)>>>(A); \
     else if ((WHICH) == 0)                                                 \
-      KERNEL<T, DP, tall, false><<<(GRID), threads, 0, (S)>>>(A);          \
-    else if ((WHICH) == 1 && mixed)                                        \
-      KERNEL<T, DP, 2, can><<<(GRID), AT_THREADS, 0, (S)>>>(A);            \
+      KERNEL<T, DP, tall, full ? AT_ALL : AT_LONG><<<(GRID), threads, 0, (S)>>>(A); \
+    else if ((WHICH) == 1 && kind != AT_LONG)                              \
+      KERNEL<T, DP, 2, full ? AT_ALL : AT_MIXED><<<(GRID), AT_THREADS, 0, (S)>>>(A); \
     else if ((WHICH) == 1)                                                 \
-      KERNEL<T, DP, 2, false><<<(GRID), AT_THREADS, 0, (S)>>>(A);          \
+      KERNEL<T, DP, 2, full ? AT_ALL : AT_LONG><<<(GRID), AT_THREADS, 0, (S)>>>(A); \
     else                                                                   \
-      KERNEL<T, DP, 1, false><<<(GRID), AT_THREADS, 0, (S)>>>(A);          \
+      KERNEL<T, DP, 1, AT_ALL><<<(GRID), AT_THREADS, 0, (S)>>>(A);         \
+    if constexpr (!full && DP > 64)                                        \
+      if ((WHICH) == 0 && kind == AT_BRIEF) {                              \
+        unsigned few;                                                      \
+        const AttnArgs brief = attn_brief_args((A), (GRID), &few);         \
+        KERNEL<T, DP, tall, AT_BRIEF><<<few, threads, 0, (S)>>>(brief);    \
+      }                                                                    \
   } while (0)
 #define BGX_ATTN_WIDTHS(KERNEL, T, D, WHICH, GRID, S, A)      \
   do {                                                        \
@@ -1416,7 +1455,7 @@ int attention_forward_impl(const bgx_attention_shape* a, const bgx_attention_row
   A.o = attn_view(o);
   attn_saved(A, a, saved);
   int which;
-  const bool mixed = attn_mixed(a);
+  const AttnKind kind = attn_kind(a);
   const unsigned grid = attn_grid(A, a, ATTN_FORWARD, &which);
   BGX_REQUIRE(grid > 0, BGX_E_SHAPE, "attention: %lld rows of %d heads", (long long)a->rows, a->heads);
   BGX_ATTN_LAUNCH(attention_forward_kernel, a->dtype, a->head_dim, which, grid, (hipStream_t)stream, A);
@@ -1470,7 +1509,7 @@ int attention_backward_impl(const bgx_attention_shape* a, const bgx_attention_ro
   BGX_REQUIRE((uintptr_t)ws % 16 == 0, BGX_E_ALIGN, "attention backward: workspace not aligned to 16 bytes");
   hipStream_t s = (hipStream_t)stream;
   int which;
-  const bool mixed = attn_mixed(a);
+  const AttnKind kind = attn_kind(a);
   unsigned grid = attn_grid(A, a, ATTN_Q, &which);
   BGX_REQUIRE(grid > 0, BGX_E_SHAPE, "attention backward: %lld rows of %d heads", (long long)a->rows, a->heads);
   BGX_ATTN_LAUNCH(attention_backward_q_kernel, a->dtype, a->head_dim, which, grid, s, A);

@@ -486,6 +486,32 @@ def test_attention_of_large_flat_scores(device, bgx_env, dim, dtype, rows):
         assert torch.equal(first, results[1][name]), name
 
 
+@pytest.mark.parametrize("rows", [128, 64])
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=ids_of)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 128), (2, 2, 96), (4, 2, 64)], ids=str)
+def test_attention_of_short_and_long_sequences(device, bgx_env, heads, kv_heads, dim, dtype, rows):
+    """Lengths on both sides of 64 in one call, empty ones among them, rows around them: found from the boundaries, from a
+    plan, and cut by lengths -- short and long ones may have kernels of their own, and every row is written by one."""
+    bgx_env("BGX_ATTENTION_ROWS", rows)
+    lengths = [3, 300, 64, 0, 65, 1, 700]
+    for head, tail, more in ((0, 0, 0), (70, 140, 0), (5, 3, 70)):      # 70 sequences more than go without a plan
+        spread = lengths + [200] * 3 * (more > 0) + [1, 90] * (more // 2)
+        ends = [head] + [head + int(e) for e in torch.tensor(spread).cumsum(0)]
+        q, k, v, do = _qkv((ends[-1] + tail,), heads, kv_heads, dim, dtype, dim + head, device)
+        for t in (q, k, v):
+            t.requires_grad_()
+        out = B.causal_attention(q, k, v, cu_seqlens=torch.tensor(ends, dtype=torch.int32, device=device))
+        grads = torch.autograd.grad(out, (q, k, v), do)
+        _check_sequences(q, k, v, do, out, grads, list(zip(ends, ends[1:])), dim ** -0.5, dtype)
+    q, k, v, do = _qkv((6, 200), heads, kv_heads, dim, dtype, dim, device)
+    for t in (q, k, v):
+        t.requires_grad_()
+    cut = [64, 200, 1, 0, 65, 33]
+    out = B.causal_attention(q, k, v, lengths=torch.tensor(cut, dtype=torch.int32, device=device))
+    grads = torch.autograd.grad(out, (q, k, v), do)
+    _check_sequences(q, k, v, do, out, grads, [(200 * i, 200 * i + l) for i, l in enumerate(cut)], dim ** -0.5, dtype)
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
 @pytest.mark.parametrize("length,n", [(3, 90), (48, 40), (64, 80), (65, 80), (300, 30)], ids=str)
 def test_attention_output_does_not_depend_on_a_graph(device, dtype, length, n):
