@@ -17,17 +17,17 @@
 // Scores, softmax statistics, probabilities' sums and all accumulators are fp32.  For 16-bit inputs P and dS are
 // rounded to the inputs' type as operands of the matrix instructions (the products of 16-bit operands are what runs
 // at the card's rate; each rounding is relative to the value, and their sum over a row averages out; small calls and
-// short sequences keep the rests, see Work).  delta is formed from o as it was before its
-// rounding: dp - delta cancels.
+// short sequences keep the rests, see Work; fp16 operands carry powers of two that keep them within the type, see DS_FIRST
+// and P_LIFT).  delta is formed from o as it was before its rounding: dp - delta cancels.
 //
 // What bounds them: a 32 x 32 block of scores costs a wave 16 exponentials a lane beside 2 (forward), 3 (dq) or 4 (dk,
 // dv) products.  At heads of 128 the products win: forward 303 us for 2 x 4096 positions, 32 query on 8 key/value heads
-// (0.27 TFLOP of the causal half: 0.91 PFLOP/s), 2.2 ms for 1 x 16384 (1.0), dq 440 us (three products: 0.94), dk and
-// dv 642 us (four: 0.86), where a large library product reaches 1.11.  At heads of 64 a block has half the products for
+// (0.27 TFLOP of the causal half: 0.91 PFLOP/s), 2.2 ms for 1 x 16384 (1.0), dq 432 us (three products: 0.95), dk and
+// dv 615 us (four: 0.89), where a large library product reaches 1.11.  At heads of 64 a block has half the products for
 // the same vector work, which then takes longer than they do; long walks still overlap the two: 2 x 16384 positions, 16
-// heads, fp16: forward 1.24 ms (0.88 PFLOP/s), dq, dk and dv 4.15 ms (seven products: 0.93).  Short walks do not hide
-// what comes before and after them: 24 documents of 16 to 2048 positions (nine tiles a workgroup) take 84 us forward
-// (0.55 PFLOP/s), 111 for dq (0.62), 167 for dk and dv (0.56), and without the walks, loading and storing the rows
+// heads, fp16: forward 1.28 ms (0.86 PFLOP/s), dq, dk and dv 4.79 ms (seven products: 0.80).  Short walks do not hide
+// what comes before and after them: 24 documents of 16 to 2048 positions (nine tiles a workgroup) take 85 us forward
+// (0.55 PFLOP/s), 122 for dq (0.56), 185 for dk and dv (0.51), and without the walks, loading and storing the rows
 // alone (4 to 5 TB/s), 28, 40 and 44.  There tiles of 32 or 128 keys instead of 64, four waves a SIMD instead of three,
 // and raised wave priority around the products were no faster (forward 86, 93, 87, 84 us), nor long and short walks in
 // turn instead of longest first (105), results turned through LDS to whole rows (84) or stored past the caches (97);

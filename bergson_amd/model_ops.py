@@ -49,7 +49,11 @@ def causal_attention(q: Tensor, k: Tensor, v: Tensor, *, cu_seqlens: Tensor | No
     cu_seqlens[n + 1] (`cu_seqlens` int32 [N + 1] on the GPU, ascending; its values are not read back).
     H is a multiple of Hk and query head h uses key/value head h // (H // Hk).  D from 1 to 128, one dtype of float32,
     float16, bfloat16; any strides (only a non-contiguous last dimension is copied).  scale (default D ** -0.5) must
-    be positive.  Positions and rows that belong to no sequence are not read: their output and gradients are 0."""
+    be positive.  Positions and rows that belong to no sequence are not read: their output and gradients are 0.
+
+    Scores, softmax statistics and sums are fp32.  With 16-bit inputs the probabilities, and in the backward pass their
+    gradients, are operands rounded to that type -- for sequences of up to 64 positions with a second operand for what the
+    rounding cut off.  The output is the same with and without a gradient recorded."""
     return (_module or _native()).causal_attention(q, k, v, cu_seqlens, lengths, scale)
 
 
