@@ -106,16 +106,15 @@ def _register() -> None:
     AttentionMaskInterface.register(IMPLEMENTATION, _mask)
 
 
-def _attention_settings(model: nn.Module) -> list[tuple[object, str]]:
+def _attention_settings(model: nn.Module) -> list[tuple[object, str | None]]:
     """(configuration, attention implementation) of the model and of every part that has its own, outer ones first."""
-    configs = {id(c): c for c in (getattr(m, "config", None) for m in model.modules())
-               if getattr(c, "_attn_implementation", None) is not None}
+    configs = {id(c): c for c in (getattr(m, "config", None) for m in model.modules()) if hasattr(c, "_attn_implementation")}
     return [(c, c._attn_implementation) for c in configs.values()]
 
 
 def _name_what_is_left(model: nn.Module) -> None:
     """transformers leaves alone what does not go through its registry."""
-    left = {id(c) for c, implementation in _attention_settings(model) if implementation != IMPLEMENTATION}
+    left = {id(c) for c, implementation in _attention_settings(model) if implementation not in (IMPLEMENTATION, None)}
     names = []
     for m in model.modules():
         config = getattr(m, "config", None)
@@ -149,6 +148,7 @@ def fused_model_ops(model: nn.Module):
         for m in norms:
             vars(m).pop("forward", None)
         if swap:
-            model.set_attn_implementation(before[0][1])
+            if before and before[0][1] is not None:
+                model.set_attn_implementation(before[0][1])
             for config, implementation in before:
                 config._attn_implementation = implementation

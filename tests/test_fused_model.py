@@ -168,6 +168,11 @@ def test_every_part_gets_its_own_attention_back():
     with pytest.raises(KeyError), B.fused_model_ops(model):
         raise KeyError("inside")
     assert of() == ["sdpa", "eager", "sdpa"]
+    unset = _Whole(_Part(None))
+    unset.config._attn_implementation = None
+    with B.fused_model_ops(unset):
+        assert unset.config._attn_implementation == unset.parts[0].config._attn_implementation == "bergson_amd"
+    assert unset.config._attn_implementation is None and unset.parts[0].config._attn_implementation is None
 
 
 def test_an_attention_that_is_not_replaced_is_named():
